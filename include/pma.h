@@ -464,6 +464,54 @@ PMA_API int pma_swiglu(int64_t rows, int inter, const void *gate, int64_t gate_s
                        const void *up, int64_t up_stride, void *out, int64_t out_stride,
                        int dtype, pma_stream_t stream);
 
+/*
+ * Gated linear recurrence over L tokens of B rows and C independent channels:
+ *
+ *     a_t = sigmoid(f_t + bias)     h_t = a_t h_{t-1} + (1 - a_t) x_t
+ *     y_t = h_t                     or, with a gate,  y_t = h_t silu(gate_t)
+ *
+ * x, f, gate and y are pma_seq_tensor views of [B, L, C] arrays (stride_h unused; the
+ * channel axis is contiguous, other strides are any non-negative number of elements, so
+ * column slices of one projection are taken as they are), all of one dtype.  gate, bias
+ * (float32 [C]), h0 (float32 [B, C], else zero) and reset (uint8 [B, L]; nonzero
+ * replaces h_{t-1} by zero: a document starts at t) may be NULL.  h_last (float32
+ * [B, C]) may be NULL and receives h_L (h0, or zero, where L is 0).  States are float32;
+ * y is rounded once to its dtype.  Results do not depend on timing.
+ * The workspace (256-byte aligned) holds one float32 state per channel and 128 tokens,
+ * among others; pma_gated_scan_backward of the same call takes it back as `forward_ws`.
+ */
+PMA_API size_t pma_gated_scan_workspace_bytes(int B, int L, int C);
+PMA_API int pma_gated_scan(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_tensor *f,
+                           const pma_seq_tensor *gate, const float *bias, const float *h0,
+                           const uint8_t *reset, const pma_seq_tensor *y, float *h_last,
+                           void *workspace, size_t workspace_bytes, pma_stream_t stream);
+
+/*
+ * Gradients of pma_gated_scan: dy as y, dh_last [B, C] or NULL (zero) in; dx, df and
+ * dgate (given exactly when gate is) as y, dbias [C] and dh0 [B, C] (each NULL where it
+ * is not wanted) out.  The states are recomputed tile by tile from forward_ws, which is
+ * only read.
+ */
+PMA_API size_t pma_gated_scan_backward_workspace_bytes(int B, int L, int C);
+PMA_API int pma_gated_scan_backward(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_tensor *f,
+                                    const pma_seq_tensor *gate, const float *bias, const float *h0,
+                                    const uint8_t *reset, const pma_seq_tensor *dy, const float *dh_last,
+                                    const pma_seq_tensor *dx, const pma_seq_tensor *df,
+                                    const pma_seq_tensor *dgate, float *dbias, float *dh0,
+                                    const void *forward_ws, size_t forward_ws_bytes,
+                                    void *workspace, size_t workspace_bytes, pma_stream_t stream);
+
+/*
+ * One token of the recurrence for N rows (x, f, gate, y: [N, C], stride_b the row
+ * stride).  h_in and h_out are float32 [N, C] and may be the same array; with `rows`
+ * (int32 [N], distinct) batch row n uses state row rows[n] of pool_rows, and a row
+ * outside the pool leaves no state and an output of zero.
+ */
+PMA_API int pma_gated_scan_step(int N, int C, const pma_seq_tensor *x, const pma_seq_tensor *f,
+                                const pma_seq_tensor *gate, const float *bias, const float *h_in,
+                                float *h_out, const int32_t *rows, int pool_rows,
+                                const pma_seq_tensor *y, pma_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,22 @@ def load() -> ctypes.CDLL:
     L.pma_swiglu.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p]
     L.pma_swiglu.restype = ctypes.c_int
+    for name in ("pma_gated_scan_workspace_bytes", "pma_gated_scan_backward_workspace_bytes"):
+        fn = getattr(L, name)
+        fn.argtypes = [ctypes.c_int] * 3
+        fn.restype = ctypes.c_size_t
+    L.pma_gated_scan.argtypes = ([ctypes.c_int] * 3 + [_P(SeqTensor)] * 3 + [ctypes.c_void_p] * 3
+                                 + [_P(SeqTensor), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                    ctypes.c_void_p])
+    L.pma_gated_scan.restype = ctypes.c_int
+    L.pma_gated_scan_backward.argtypes = ([ctypes.c_int] * 3 + [_P(SeqTensor)] * 3 + [ctypes.c_void_p] * 3
+                                          + [_P(SeqTensor), ctypes.c_void_p] + [_P(SeqTensor)] * 3
+                                          + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p,
+                                                                     ctypes.c_size_t, ctypes.c_void_p])
+    L.pma_gated_scan_backward.restype = ctypes.c_int
+    L.pma_gated_scan_step.argtypes = ([ctypes.c_int] * 2 + [_P(SeqTensor)] * 3 + [ctypes.c_void_p] * 4
+                                      + [ctypes.c_int, _P(SeqTensor), ctypes.c_void_p])
+    L.pma_gated_scan_step.restype = ctypes.c_int
     _lib = L
     return L
 

@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "prefill.cuh"
+#include "recurrence.cuh"
 
 using namespace pma;
 
@@ -109,6 +110,64 @@ struct Plan {
     int seg_len = 0;
     size_t ws_bytes = 0;
 };
+
+// A [B, L, C] array of the recurrence: elements on their own boundary, strides not negative, the
+// dtype of `like`.
+int check_blc(const pma_seq_tensor *t, const pma_seq_tensor *like, bool empty) {
+    if (!t || !like) return PMA_ERR_ARGUMENT;
+    if (!supported_dtype(t->dtype) || t->dtype != like->dtype) return PMA_ERR_DTYPE;
+    if (!t->data) return empty ? PMA_OK : PMA_ERR_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(t->data) % esize(t->dtype) || t->stride_b < 0 || t->stride_l < 0)
+        return PMA_ERR_LAYOUT;
+    return PMA_OK;
+}
+Blc blc_of(const pma_seq_tensor *t) { return t ? Blc{t->data, t->stride_b, t->stride_l} : Blc{nullptr, 0, 0}; }
+
+// Workspace of the recurrence: [256 B: counter, abort flag][states][runs][partial bias sums].
+// A sequence of one tile needs no words.
+struct ScanWs {
+    int chunks;
+    size_t nwords, runs_at, part_at;
+    static ScanWs of(int B, int L, int C) {
+        ScanWs w;
+        w.chunks = scan_chunks(L);
+        w.nwords = (size_t)B * w.chunks * C;
+        const bool one = w.chunks <= 1;
+        w.runs_at = one ? 0 : (256 + 4 * w.nwords + 255) / 256 * 256;
+        w.part_at = one ? 0 : (w.runs_at + 8 * w.nwords + 255) / 256 * 256;
+        return w;
+    }
+    size_t bytes(bool backward) const { return part_at + (backward ? 4 * nwords : 0); }
+    uint32_t *incl(void *ws) const { return reinterpret_cast<uint32_t *>((char *)ws + 256); }
+    float *part(void *ws) const { return reinterpret_cast<float *>((char *)ws + part_at); }
+    // Every word unwritten (all ones), the counter and the abort flag at -1.
+    cudaError_t arm(ScanParams &p, void *ws, cudaStream_t st) const {
+        if (chunks <= 1) return cudaSuccess;
+        p.counter = reinterpret_cast<int *>(ws);
+        p.incl = incl(ws);
+        p.agg = reinterpret_cast<unsigned long long *>((char *)ws + runs_at);
+        return cudaMemsetAsync(ws, 0xff, part_at, st);
+    }
+};
+
+ScanParams scan_params(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_tensor *f,
+                       const pma_seq_tensor *gate, const float *bias, const float *h0, const uint8_t *reset) {
+    ScanParams p{};
+    p.B = B;
+    p.L = L;
+    p.C = C;
+    p.chunks = scan_chunks(L);
+    p.x = blc_of(x);
+    p.f = blc_of(f);
+    p.gate = blc_of(gate);
+    p.bias = bias;
+    p.h0 = h0;
+    p.reset = reset;
+    p.fault = g_fault_word.load(std::memory_order_acquire);
+    p.wait_ns = 2000000000ull;  // as the tensor-core kernels: 2 s per wait
+    p.test_wait_ns = g_test_wait_ns.load(std::memory_order_acquire);
+    return p;
+}
 
 bool bf16_exact(float f) {
     uint32_t u;
@@ -724,6 +783,113 @@ int pma_swiglu(int64_t rows, int inter, const void *gate, int64_t gate_stride, c
     if ((rc = device_info(&di))) return rc;
     cudaError_t e = launch_swiglu(dtype, gate, gate_stride, up, up_stride, out, out_stride, rows, inter, di.sms,
                                   reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+size_t pma_gated_scan_workspace_bytes(int B, int L, int C) {
+    return B <= 0 || L <= 0 || C <= 0 ? 0 : ScanWs::of(B, L, C).bytes(false);
+}
+size_t pma_gated_scan_backward_workspace_bytes(int B, int L, int C) {
+    return B <= 0 || L <= 0 || C <= 0 ? 0 : ScanWs::of(B, L, C).bytes(true);
+}
+
+int pma_gated_scan(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_tensor *f, const pma_seq_tensor *gate,
+                   const float *bias, const float *h0, const uint8_t *reset, const pma_seq_tensor *y, float *h_last,
+                   void *workspace, size_t workspace_bytes, pma_stream_t stream) {
+    if (B < 0 || L < 0 || C <= 0) return PMA_ERR_ARGUMENT;
+    int rc;
+    const bool empty = B == 0 || L == 0;
+    if ((rc = check_blc(x, x, empty)) || (rc = check_blc(f, x, empty)) || (gate && (rc = check_blc(gate, x, empty))) ||
+        (rc = check_blc(y, x, empty)))
+        return rc;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    if (B == 0) return PMA_OK;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (L == 0) {  // the state passes through
+        if (!h_last || h_last == h0) return PMA_OK;
+        const size_t n = (size_t)B * C * sizeof(float);
+        e = h0 ? cudaMemcpyAsync(h_last, h0, n, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(h_last, 0, n, st);
+        return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+    }
+    const ScanWs w = ScanWs::of(B, L, C);
+    if (workspace_bytes < w.bytes(false) || (w.bytes(false) && (!workspace || (uintptr_t)workspace % 256)))
+        return PMA_ERR_WORKSPACE;
+    ScanParams p = scan_params(B, L, C, x, f, gate, bias, h0, reset);
+    p.y = blc_of(y);
+    p.h_last = h_last;
+    if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
+    e = launch_gated_scan(p, x->dtype, st);
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_gated_scan_backward(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_tensor *f,
+                            const pma_seq_tensor *gate, const float *bias, const float *h0, const uint8_t *reset,
+                            const pma_seq_tensor *dy, const float *dh_last, const pma_seq_tensor *dx,
+                            const pma_seq_tensor *df, const pma_seq_tensor *dgate, float *dbias, float *dh0,
+                            const void *forward_ws, size_t forward_ws_bytes, void *workspace, size_t workspace_bytes,
+                            pma_stream_t stream) {
+    if (B < 0 || L < 0 || C <= 0 || (gate == nullptr) != (dgate == nullptr)) return PMA_ERR_ARGUMENT;
+    int rc;
+    const bool empty = B == 0 || L == 0;
+    for (const pma_seq_tensor *t : {x, f, dy, dx, df})
+        if ((rc = check_blc(t, x, empty))) return rc;
+    if (gate && ((rc = check_blc(gate, x, empty)) || (rc = check_blc(dgate, x, empty)))) return rc;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (empty) {
+        if (dbias && (e = cudaMemsetAsync(dbias, 0, (size_t)C * sizeof(float), st)) != cudaSuccess) return cuda_fail(e);
+        if (!dh0 || B == 0 || dh0 == dh_last) return PMA_OK;
+        const size_t n = (size_t)B * C * sizeof(float);
+        e = dh_last ? cudaMemcpyAsync(dh0, dh_last, n, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(dh0, 0, n, st);
+        return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+    }
+    const ScanWs w = ScanWs::of(B, L, C);
+    if (forward_ws_bytes < w.bytes(false) || (w.bytes(false) && (!forward_ws || (uintptr_t)forward_ws % 256)))
+        return PMA_ERR_WORKSPACE;
+    if (workspace_bytes < w.bytes(true) || !workspace || (uintptr_t)workspace % 256) return PMA_ERR_WORKSPACE;
+    ScanParams p = scan_params(B, L, C, x, f, gate, bias, h0, reset);
+    p.dy = blc_of(dy);
+    p.dh_last = dh_last;
+    p.dx = blc_of(dx);
+    p.df = blc_of(df);
+    p.dgate = blc_of(dgate);
+    p.dh0 = dh0;
+    p.states = w.nwords && w.chunks > 1 ? w.incl(const_cast<void *>(forward_ws)) : nullptr;
+    p.dbias_part = dbias ? w.part(workspace) : nullptr;
+    if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
+    e = launch_gated_scan_backward(p, x->dtype, dbias, st);
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_gated_scan_step(int N, int C, const pma_seq_tensor *x, const pma_seq_tensor *f, const pma_seq_tensor *gate,
+                        const float *bias, const float *h_in, float *h_out, const int32_t *rows, int pool_rows,
+                        const pma_seq_tensor *y, pma_stream_t stream) {
+    if (N < 0 || C <= 0 || (rows && pool_rows < 0)) return PMA_ERR_ARGUMENT;
+    int rc;
+    if ((rc = check_blc(x, x, N == 0)) || (rc = check_blc(f, x, N == 0)) || (gate && (rc = check_blc(gate, x, N == 0))) ||
+        (rc = check_blc(y, x, N == 0)))
+        return rc;
+    if (N && (!h_in || !h_out)) return PMA_ERR_ARGUMENT;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    if (N == 0) return PMA_OK;
+    ScanStepParams p{};
+    p.N = N;
+    p.C = C;
+    p.x = blc_of(x);
+    p.f = blc_of(f);
+    p.gate = blc_of(gate);
+    p.y = blc_of(y);
+    p.bias = bias;
+    p.h_in = h_in;
+    p.h_out = h_out;
+    p.rows = rows;
+    p.pool_rows = pool_rows;
+    cudaError_t e = launch_gated_scan_step(p, x->dtype, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 

@@ -1,0 +1,44 @@
+"""Argument checks of the gated recurrence: nothing here touches a device."""
+import ctypes
+
+import pytest
+import torch
+
+from prime_moment_attention_b200 import _lib, recurrence
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(1, 2, 3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        recurrence.gated_scan(x, x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        recurrence.gated_scan_step(x[0], x[0], torch.zeros(2, 3))
+
+
+def _t(dt=_lib.PMA_BF16, ptr=256, sb=64, sl=64):
+    return ctypes.byref(_lib.SeqTensor(ptr, dt, sb, 0, sl))
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"B": -1}, 1), ({"C": 0}, 1), ({"x": None}, 1), ({"f": _t(_lib.PMA_F32)}, 3), ({"x": _t(9)}, 3),
+    ({"y": _t(ptr=0)}, 1), ({"gate": _t(ptr=257)}, 4), ({"f": _t(sl=-64)}, 4),
+])
+def test_forward_argument_errors(change, status):
+    a = {"B": 1, "L": 300, "C": 64, "x": _t(), "f": _t(), "gate": None, "y": _t(), **change}
+    rc = _lib.load().pma_gated_scan(a["B"], a["L"], a["C"], a["x"], a["f"], a["gate"], None, None, None, a["y"], None,
+                                    None, 0, None)
+    assert rc == status
+
+
+def test_backward_gate_and_its_gradient_go_together():
+    rc = _lib.load().pma_gated_scan_backward(1, 300, 64, _t(), _t(), _t(), None, None, None, _t(), None, _t(), _t(),
+                                             None, None, None, None, 0, None, 0, None)
+    assert rc == 1
+
+
+def test_workspace_sizes():
+    L = _lib.load()
+    assert L.pma_gated_scan_workspace_bytes(4, 128, 64) == 0  # one tile: nothing to hand over
+    assert L.pma_gated_scan_workspace_bytes(4, 129, 64) >= 4 * 2 * 64 * 12
+    # 64-bit sizes: 2^20 tokens of 4096 channels in 16 rows
+    assert L.pma_gated_scan_workspace_bytes(16, 1 << 20, 4096) > 6 << 30
