@@ -512,6 +512,31 @@ PMA_API int pma_gated_scan_step(int N, int C, const pma_seq_tensor *x, const pma
                                 float *h_out, const int32_t *rows, int pool_rows,
                                 const pma_seq_tensor *y, pma_stream_t stream);
 
+/*
+ * One token per row of logits [B, V] (row stride in elements, PMA_BF16 or PMA_F32,
+ * V at most 360448), from one given uniform number per row, u [B] in [0, 1):
+ *
+ *     z = (x - max x) / T      w = round(exp(z) 2^32)
+ *     keep, in the order (x descending, index ascending): the first top_k tokens; of
+ *     them those before which less than top_p of their weight lies; of those the ones
+ *     with exp(z) >= min_p.  The most likely token is always kept.
+ *     token = first kept index whose cumulated kept weight exceeds u times their total
+ *     logprob = z_token - log(sum of all w / 2^32)
+ *
+ * Each setting is a device array of B values or, where that is NULL, one value for all
+ * rows.  temperature <= 0 takes the most likely token (logprob then at T = 1); top_k <= 0,
+ * top_p >= 1 and min_p <= 0 switch a filter off.  -inf and NaN logits are never taken; a
+ * row of nothing else gives token -1 and logprob -inf.  +inf logits share the row.  Sums
+ * are whole numbers: the same row and u give the same token in any batch.  logprobs may
+ * be NULL.
+ */
+PMA_API int pma_sample(int B, int V, const void *logits, int64_t row_stride, int dtype, const float *u,
+                       const float *temperature, float temperature_value,
+                       const int32_t *top_k, int top_k_value,
+                       const float *top_p, float top_p_value,
+                       const float *min_p, float min_p_value,
+                       int64_t *tokens, float *logprobs, pma_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -151,6 +151,11 @@ def load() -> ctypes.CDLL:
     L.pma_gated_scan_step.argtypes = ([ctypes.c_int] * 2 + [_P(SeqTensor)] * 3 + [ctypes.c_void_p] * 4
                                       + [ctypes.c_int, _P(SeqTensor), ctypes.c_void_p])
     L.pma_gated_scan_step.restype = ctypes.c_int
+    L.pma_sample.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
+                             ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
+                             ctypes.c_void_p, ctypes.c_void_p]
+    L.pma_sample.restype = ctypes.c_int
     _lib = L
     return L
 

@@ -6,6 +6,7 @@
 
 #include "prefill.cuh"
 #include "recurrence.cuh"
+#include "sampling.cuh"
 
 using namespace pma;
 
@@ -890,6 +891,35 @@ int pma_gated_scan_step(int N, int C, const pma_seq_tensor *x, const pma_seq_ten
     p.rows = rows;
     p.pool_rows = pool_rows;
     cudaError_t e = launch_gated_scan_step(p, x->dtype, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_sample(int B, int V, const void *logits, int64_t row_stride, int dtype, const float *u,
+               const float *temperature, float temperature_value, const int32_t *top_k, int top_k_value,
+               const float *top_p, float top_p_value, const float *min_p, float min_p_value, int64_t *tokens,
+               float *logprobs, pma_stream_t stream) {
+    if (B < 0 || B > (1 << 27) || V <= 0 || V > SAMPLE_MAX_V || row_stride < 0 || (B > 1 && row_stride < V))
+        return PMA_ERR_ARGUMENT;
+    if (!supported_dtype(dtype)) return PMA_ERR_DTYPE;
+    if (B == 0) return PMA_OK;
+    if (!logits || !u || !tokens) return PMA_ERR_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(logits) % esize(dtype)) return PMA_ERR_LAYOUT;
+    int rc;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    SampleParams p{};
+    p.B = B;
+    p.V = V;
+    p.logits = logits;
+    p.stride = row_stride;
+    p.u = u;
+    p.temperature = {temperature, temperature_value};
+    p.top_k = {top_k, top_k_value};
+    p.top_p = {top_p, top_p_value};
+    p.min_p = {min_p, min_p_value};
+    p.token = tokens;
+    p.logprob = logprobs;
+    cudaError_t e = launch_sample(p, dtype, di.sms, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 

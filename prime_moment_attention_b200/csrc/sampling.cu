@@ -1,0 +1,646 @@
+// sampling.cu -- one token per row of logits: temperature, top-k, top-p, min-p, and the inverse
+// transform of one given uniform number.
+//
+//   z_i = (x_i - max x) / T        w_i = round(exp(z_i) 2^32), a whole number
+//   order the tokens by (x descending, index ascending); a filter keeps a prefix of that order:
+//     top-k   the first k
+//     top-p   rank r while the weight of the ranks before it is below p times the top-k's weight
+//     min-p   exp(z) >= min_p
+//   token = the first kept i, by index, whose cumulated kept weight exceeds u times their total
+//   logprob = z_token - log(sum of all w / 2^32)
+//
+// Weights are whole numbers so that every sum is exact: no result depends on the order of an
+// addition, on atomics or on how a row is split, and two rows with the same logits and u get the
+// same token in any batch.  (A token below 2^-33 of the most likely one has weight 0.)
+//
+// A cluster of 1 to 8 CTAs holds one row in shared memory, read from HBM once.  Nothing is
+// sorted.  A cut of the order is a logit and how many of its equals are kept; it is found by
+// histograms: first over z (1024 bins), then, inside the bin that holds the cut, over the logits'
+// ordered bits until a bin is one value.  Only tokens that can be near a cut enter a histogram:
+//     top-k   with G >= k disjoint groups of tokens, the smallest of the groups' maxima is at most
+//             the k-th largest logit (the groups are fixed lanes, so this comes with the maximum)
+//     top-p   the tokens below z weigh less than V exp(z): those with V exp(z) <= (1 - p) W are cut
+// The kept weights are then summed by ranges of consecutive tokens, one a warp; the warp whose
+// range holds the goal walks it.
+#include <cooperative_groups.h>
+
+#include "sampling.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace pma {
+namespace {
+
+constexpr int NW = 16;       // warps of a CTA
+constexpr int NB = 1024;     // histogram bins
+constexpr int MAXC = 8;      // CTAs of a cluster
+constexpr float ZMIN = -23.0f;  // exp(-23) 2^32 < 1/2: weight 0 below
+constexpr unsigned long long ONE = 1ull << 32;
+
+struct Found {
+    int bin;                       // -1: the goal lies past the last bin
+    uint32_t count;                // tokens before the bin
+    unsigned long long weight;     // their weight
+};
+
+struct Shared {
+    uint32_t cnt[NB], lo[NB], hi[NB];  // this CTA's histogram (weights as two 32-bit halves)
+    uint32_t m_cnt[2][NB];             // this CTA's slice of the merged histogram: [0] over z, [1] over bits
+    unsigned long long m_w[2][NB];
+    // written by the CTAs of the cluster, one slot each
+    float x_max[MAXC], x_bound[MAXC];
+    unsigned long long x_sum[MAXC];
+    uint32_t x_klo[MAXC], x_khi[MAXC];
+    uint32_t x_cnt[MAXC];
+    unsigned long long x_w[MAXC];
+    Found found;
+    // per warp
+    float w_max[NW], w_bound[NW];
+    unsigned long long w_sum[NW];
+    uint32_t w_klo[NW], w_khi[NW];
+    unsigned long long f_gt[NW];       // weight of the tokens before the cut in the warp's range
+    uint32_t f_eq[NW];                 // tokens equal to it
+    int owner;                         // warp of this CTA that holds the goal, or -1
+    unsigned long long goal;           // goal left when its range starts
+    uint32_t eq_left;                  // equals that may still be kept there
+};
+
+template <typename T> struct Row;
+template <> struct Row<float> {
+    static constexpr int VEC = 4;
+    static __device__ __forceinline__ void get(const float *s, float (&x)[4]) {
+        const float4 v = *reinterpret_cast<const float4 *>(s);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    }
+    static __device__ __forceinline__ float lowest() { return -INFINITY; }
+};
+template <> struct Row<__nv_bfloat16> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ void get(const __nv_bfloat16 *s, float (&x)[8]) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(s);
+        const uint32_t a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(a[i] << 16);
+            x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xff80); }
+};
+
+// Bits of x in an order that matches <, with -0 as +0.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) - 1u | 0x80000000u));
+}
+
+// z and weights of one row
+struct Scale {
+    float top, inv;
+    bool inf_top;  // the largest logit is +inf: its equals share the row
+    __device__ __forceinline__ float z(float x) const {
+        if (inf_top) return x == top ? 0.f : -INFINITY;
+        return __fmul_rn(__fsub_rn(x, top), inv);
+    }
+};
+// round(e 2^32) for e in [0, 1]; the conversion saturates only at e = 1
+__device__ __forceinline__ uint32_t weight32(float e) { return __float2uint_rn(__fmul_rn(e, 4294967296.0f)); }
+__device__ __forceinline__ unsigned long long weight(float e) {
+    const uint32_t w = weight32(e);
+    return w == 0xffffffffu ? ONE : w;
+}
+
+template <typename T> __device__ __forceinline__ T warp_add(T v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <typename T> __device__ __forceinline__ T warp_before(T v, int lane) {  // exclusive prefix sum
+    T s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+    }
+    return s - v;
+}
+
+// One row's CTA.
+template <typename T> struct Sampler {
+    static constexpr int VEC = Row<T>::VEC;
+    Shared &s;
+    const T *seg;       // NW * range tokens
+    cg::cluster_group cl;
+    int nc, rank, warp, lane, range;
+
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        const T *w = seg + warp * range;
+        for (int i = lane * VEC; i < range; i += 32 * VEC) {
+            float x[VEC];
+            Row<T>::get(w + i, x);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) f(x[v]);
+        }
+    }
+
+    __device__ __forceinline__ void clear() {
+        for (int i = threadIdx.x; i < NB; i += NW * 32) s.cnt[i] = s.lo[i] = s.hi[i] = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void count(int bin, uint32_t w32) {
+        atomicAdd(&s.cnt[bin], 1u);
+        if (w32) {
+            const uint32_t old = atomicAdd(&s.lo[bin], w32);
+            // 2^32 is held as 2^32 - 1 by the conversion: the one left over goes to the carry
+            uint32_t up = old + w32 < old;
+            if (w32 == 0xffffffffu) {
+                const uint32_t o2 = atomicAdd(&s.lo[bin], 1u);
+                up += o2 == 0xffffffffu;
+            }
+            if (up) atomicAdd(&s.hi[bin], up);
+        }
+    }
+    // Sum the CTAs' histograms: this CTA keeps the slice [rank, rank + 1) * NB / nc, and everybody
+    // gets the slices' totals.
+    __device__ __forceinline__ void merge(int which) {
+        cl.sync();
+        const int per = NB / nc;
+        for (int i = threadIdx.x; i < per; i += NW * 32) {
+            uint32_t c = 0;
+            unsigned long long w = 0;
+            for (int r = 0; r < nc; ++r) {
+                const Shared *o = cl.map_shared_rank(&s, r);
+                const int at = rank * per + i;
+                c += o->cnt[at];
+                w += ((unsigned long long)o->hi[at] << 32) + o->lo[at];
+            }
+            s.m_cnt[which][i] = c;
+            s.m_w[which][i] = w;
+        }
+        __syncthreads();
+        totals(which);
+    }
+    __device__ __forceinline__ void totals(int which) {
+        const int per = NB / nc;
+        if (warp == 0) {
+            uint32_t c = 0;
+            unsigned long long w = 0;
+            for (int i = lane; i < per; i += 32) {
+                c += s.m_cnt[which][i];
+                w += s.m_w[which][i];
+            }
+            c = warp_add(c);
+            w = warp_add(w);
+            if (lane < nc) {
+                Shared *o = cl.map_shared_rank(&s, lane);
+                o->x_cnt[rank] = c;
+                o->x_w[rank] = w;
+            }
+        }
+        cl.sync();
+    }
+    // The first bin whose tokens reach past `by_rank` tokens (or past the weight `goal`), given what
+    // comes before the first bin.
+    __device__ __forceinline__ Found find(int which, bool by_count, uint32_t by_rank, double goal, uint32_t c0,
+                                          unsigned long long w0) {
+        int owner = -1;
+        uint32_t c = c0;
+        unsigned long long w = w0;
+        for (int r = 0; r < nc; ++r) {
+            const uint32_t c2 = c + s.x_cnt[r];
+            const unsigned long long w2 = w + s.x_w[r];
+            if (by_count ? c2 > by_rank : !((double)w2 < goal)) {
+                owner = r;
+                break;
+            }
+            c = c2;
+            w = w2;
+        }
+        if (owner == rank && warp == 0) {
+            const int per = NB / nc, each_lane = per / 32;
+            uint32_t lc = 0;
+            unsigned long long lw = 0;
+            for (int i = 0; i < each_lane; ++i) {
+                lc += s.m_cnt[which][lane * each_lane + i];
+                lw += s.m_w[which][lane * each_lane + i];
+            }
+            uint32_t bc = c + warp_before(lc, lane);
+            unsigned long long bw = w + warp_before(lw, lane);
+            const bool past = by_count ? bc + lc > by_rank : !((double)(bw + lw) < goal);
+            const uint32_t who = __ballot_sync(0xffffffffu, past);
+            if (lane == __ffs(who) - 1) {
+                int i = 0;
+                for (; i < each_lane - 1; ++i) {
+                    const uint32_t c2 = bc + s.m_cnt[which][lane * each_lane + i];
+                    const unsigned long long w2 = bw + s.m_w[which][lane * each_lane + i];
+                    if (by_count ? c2 > by_rank : !((double)w2 < goal)) break;
+                    bc = c2;
+                    bw = w2;
+                }
+                const Found f{rank * per + lane * each_lane + i, bc, bw};
+                for (int r = 0; r < nc; ++r) cl.map_shared_rank(&s, r)->found = f;
+            }
+        }
+        cl.sync();
+        return owner < 0 ? Found{-1, c, w} : s.found;
+    }
+};
+
+struct Cut {
+    uint32_t key;    // ordered bits of the last kept logit
+    uint32_t keep;   // how many of its equals are kept
+    unsigned long long before;  // weight before it
+};
+
+template <typename T>
+__global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
+    constexpr int VEC = Row<T>::VEC;
+    extern __shared__ __align__(16) unsigned char raw[];
+    Shared &s = *reinterpret_cast<Shared *>(raw);
+    T *seg = reinterpret_cast<T *>(raw + (sizeof(Shared) + 15) / 16 * 16);
+    cg::cluster_group cl = cg::this_cluster();
+    const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int b = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int range = p.range;
+    Sampler<T> S{s, seg, cl, nc, rank, warp, lane, range};
+
+    // ---- the row into shared memory, its maximum, and the top-k bound
+    const int first = (rank * NW + warp) * range;  // this warp's tokens of the row
+    const T *row = static_cast<const T *>(p.logits) + (int64_t)b * p.stride;
+    const int n = max(0, min(range, p.V - first));
+    float mx = -INFINITY;
+    {
+        T *w = seg + warp * range;
+        const T *src = row + first;
+        if (reinterpret_cast<uintptr_t>(row) % 16 == 0) {  // ranges are whole vectors
+            const int whole = n / VEC * VEC;
+            for (int i = lane * VEC; i < whole; i += 32 * VEC)
+                *reinterpret_cast<uint4 *>(w + i) = __ldcs(reinterpret_cast<const uint4 *>(src + i));
+            for (int i = whole + lane; i < n; i += 32) w[i] = src[i];
+        } else {
+            for (int i = lane; i < n; i += 32) w[i] = src[i];
+        }
+        for (int i = n + lane; i < range; i += 32) w[i] = Row<T>::lowest();
+        __syncwarp();
+        S.each([&](float x) { mx = fmaxf(mx, x); });  // NaN loses
+    }
+    const float temp = p.temperature.at(b);
+    const bool greedy = !(temp > 0.f);
+    const float top_p = p.top_p.at(b), min_p = p.min_p.at(b);
+    int top_k = p.top_k.at(b);
+    if (top_k <= 0 || top_k >= p.V) top_k = 0;
+    // lanes of a group: as many as leave top_k groups
+    int group = 32;
+    while (group > 1 && nc * NW * 32 / group < top_k) group >>= 1;
+    const bool bounded = top_k > 0 && nc * NW * 32 / group >= top_k;
+    {
+        float bound = mx;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, bound, o), m2 = __shfl_xor_sync(0xffffffffu, mx, o);
+            bound = o < group ? fmaxf(bound, other) : fminf(bound, other);
+            mx = fmaxf(mx, m2);
+        }
+        if (lane == 0) {
+            s.w_max[warp] = mx;
+            s.w_bound[warp] = bound;
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        mx = s.w_max[lane & (NW - 1)];
+        float bound = s.w_bound[lane & (NW - 1)];
+#pragma unroll
+        for (int o = 1; o < NW; o <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            bound = fminf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+        }
+        if (lane < nc) {
+            Shared *o = cl.map_shared_rank(&s, lane);
+            o->x_max[rank] = mx;
+            o->x_bound[rank] = bound;
+        }
+    }
+    cl.sync();
+    float bound = INFINITY;
+    mx = -INFINITY;
+    for (int r = 0; r < nc; ++r) {
+        mx = fmaxf(mx, s.x_max[r]);
+        bound = fminf(bound, s.x_bound[r]);
+    }
+    if (mx == -INFINITY) {  // every token is masked (the same in every CTA of the cluster)
+        if (rank == 0 && threadIdx.x == 0) {
+            p.token[b] = -1;
+            if (p.logprob) p.logprob[b] = -INFINITY;
+        }
+        cl.sync();
+        return;
+    }
+    const Scale sc{mx, greedy ? 1.f : fminf(__frcp_rn(temp), 3.402823466e38f), mx == INFINITY};
+
+    // ---- the weight of all tokens
+    unsigned long long total = 0;
+    {
+        uint32_t ones = 0;
+        S.each([&](float x) {
+            const uint32_t w = weight32(expf(sc.z(x)));  // NaN converts to 0
+            total += w;
+            ones += w == 0xffffffffu;
+        });
+        total = warp_add(total + ones);
+        if (lane == 0) s.w_sum[warp] = total;
+        __syncthreads();
+        if (warp == 0) {
+            total = warp_add(lane < NW ? s.w_sum[lane] : 0ull);
+            if (lane < nc) cl.map_shared_rank(&s, lane)->x_sum[rank] = total;
+        }
+        cl.sync();
+        total = 0;
+        for (int r = 0; r < nc; ++r) total += s.x_sum[r];
+    }
+
+    // ---- the cut
+    Cut cut{0, 0xffffffffu, 0};  // keeps every token
+    const bool only_first = greedy || !(top_p > 0.f) || !(min_p <= 1.f);
+    if (only_first) {
+        cut = Cut{ordered(mx), 1, 0};
+    } else if (top_k || top_p < 1.f) {
+        float low = -INFINITY;  // tokens below it are behind every cut
+        if (top_k) {
+            if (bounded) low = bound;
+        } else {
+            // weights are rounded up by at most 1/2 each; the margin covers the logarithm's error
+            const float room = (1.f - top_p) * (float)total * (1.f / 4294967296.f) / (float)p.V - 1.f / 8589934592.f;
+            if (room > 0.f) {
+                const float zl = logf(room) - 0.02f;
+                if (zl > ZMIN && !sc.inf_top) low = mx + zl / sc.inv - 4e-7f * fabsf(mx);
+            }
+        }
+        float span = -sc.z(low);
+        span = fminf(fmaxf(span, 1e-6f), -ZMIN);  // farther tokens share the last bin
+        const float fine = (float)NB / span;
+        auto bin_of = [&](float z) { return (int)fminf(-z * fine, (float)(NB - 1)); };
+        S.clear();
+        S.each([&](float x) {
+            if (x >= low && x > -INFINITY) {
+                const float z = sc.z(x);
+                S.count(bin_of(z), weight32(expf(z)));
+            }
+        });
+        S.merge(0);
+
+        // Narrow the bin that holds the goal down to one logit.
+        auto narrow = [&](bool by_count, uint32_t by_rank, double goal, Found f) {
+            uint32_t klo = 0xffffffffu, khi = 0;
+            S.each([&](float x) {
+                if (x >= low && x > -INFINITY && bin_of(sc.z(x)) == f.bin) {
+                    const uint32_t k = ordered(x);
+                    klo = min(klo, k);
+                    khi = max(khi, k);
+                }
+            });
+            klo = __reduce_min_sync(0xffffffffu, klo);
+            khi = __reduce_max_sync(0xffffffffu, khi);
+            if (lane == 0) {
+                s.w_klo[warp] = klo;
+                s.w_khi[warp] = khi;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                klo = __reduce_min_sync(0xffffffffu, s.w_klo[lane & (NW - 1)]);
+                khi = __reduce_max_sync(0xffffffffu, s.w_khi[lane & (NW - 1)]);
+                if (lane < nc) {
+                    Shared *o = cl.map_shared_rank(&s, lane);
+                    o->x_klo[rank] = klo;
+                    o->x_khi[rank] = khi;
+                }
+            }
+            cl.sync();
+            klo = 0xffffffffu;
+            khi = 0;
+            for (int r = 0; r < nc; ++r) {
+                klo = min(klo, s.x_klo[r]);
+                khi = max(khi, s.x_khi[r]);
+            }
+            for (int level = 0; level < 4 && klo < khi; ++level) {  // 10 of 32 bits each
+                int shift = 0;
+                while ((khi - klo) >> shift >= NB) ++shift;
+                S.clear();
+                S.each([&](float x) {
+                    const uint32_t k = ordered(x);
+                    if (k >= klo && k <= khi && x == x) S.count((int)((khi - k) >> shift), weight32(expf(sc.z(x))));
+                });
+                S.merge(1);
+                f = S.find(1, by_count, by_rank, goal, f.count, f.weight);
+                if (f.bin < 0) break;  // not reached: the goal lies in this range
+                khi -= (uint32_t)f.bin << shift;
+                const uint32_t width = (1u << shift) - 1;
+                if (khi - klo > width) klo = khi - width;
+            }
+            Cut c;
+            c.key = khi;
+            c.before = f.weight;
+            if (by_count) {
+                c.keep = by_rank + 1 - f.count;
+            } else {
+                // the largest m with before + (m - 1) w < goal
+                const unsigned long long w = weight(expf(sc.z(unordered(khi))));
+                if (w == 0) {
+                    c.keep = 0xffffffffu;
+                } else {
+                    const double m = ceil((goal - (double)f.weight) / (double)w);
+                    uint32_t k = (uint32_t)fmin(fmax(m, 1.0), (double)p.V);
+                    // the quotient may be off by its rounding
+                    if (k > 1 && !((double)(f.weight + (unsigned long long)(k - 1) * w) < goal)) --k;
+                    if ((double)(f.weight + (unsigned long long)k * w) < goal) ++k;
+                    c.keep = k;
+                }
+            }
+            return c;
+        };
+
+        unsigned long long wk = total;  // weight of the top-k tokens
+        if (top_k) {
+            const Found f = S.find(0, true, (uint32_t)top_k - 1, 0.0, 0, 0);
+            if (f.bin >= 0) {
+                cut = narrow(true, (uint32_t)top_k - 1, 0.0, f);
+                wk = cut.before + cut.keep * weight(expf(sc.z(unordered(cut.key))));
+            }
+        }
+        if (top_p < 1.f) {
+            const double goal = (double)top_p * (double)wk;
+            if (top_k) S.totals(0);  // the slices' totals over z again
+            const Found f = S.find(0, false, 0, goal, 0, 0);
+            if (f.bin >= 0) {
+                const Cut c = narrow(false, 0, goal, f);
+                if (c.key > cut.key || (c.key == cut.key && c.keep < cut.keep)) cut = c;
+            }
+        }
+    }
+
+    // ---- kept weight by ranges of consecutive tokens
+    const float xcut = cut.key == 0 ? -INFINITY : unordered(cut.key);
+    const float need = only_first ? 0.f : min_p;
+    unsigned long long gt = 0;
+    uint32_t eq = 0;
+    S.each([&](float x) {
+        if (x >= xcut && x > -INFINITY) {
+            const float e = expf(sc.z(x));
+            if (!(e < need)) {
+                if (x > xcut)
+                    gt += weight(e);
+                else
+                    ++eq;
+            }
+        }
+    });
+    gt = warp_add(gt);
+    eq = warp_add(eq);
+    if (lane == 0) {
+        s.f_gt[warp] = gt;
+        s.f_eq[warp] = eq;
+    }
+    cl.sync();
+    const float ecut = expf(sc.z(xcut));
+    const unsigned long long wcut = cut.key == 0 ? 0 : weight(ecut);
+    if (warp == 0) {
+        // every CTA goes through all ranges: 4 lanes' worth of 32 at most
+        uint32_t eqs[MAXC * NW / 32];
+        unsigned long long gts[MAXC * NW / 32];
+        const int ranges = nc * NW, each_lane = (ranges + 31) / 32;
+        uint32_t le = 0;
+#pragma unroll
+        for (int i = 0; i < MAXC * NW / 32; ++i) {
+            const int r = lane * each_lane + i;
+            const bool on = i < each_lane && r < ranges;
+            const Shared *o = cl.map_shared_rank(&s, on ? r / NW : rank);
+            eqs[i] = on ? o->f_eq[r % NW] : 0;
+            gts[i] = on ? o->f_gt[r % NW] : 0;
+            le += eqs[i];
+        }
+        uint32_t seen = warp_before(le, lane);
+        unsigned long long sum = 0;
+        uint32_t left[MAXC * NW / 32];
+#pragma unroll
+        for (int i = 0; i < MAXC * NW / 32; ++i) {
+            left[i] = cut.keep > seen ? cut.keep - seen : 0;
+            seen += eqs[i];
+            gts[i] += (unsigned long long)min(left[i], eqs[i]) * wcut;
+            sum += gts[i];
+        }
+        unsigned long long at = warp_before(sum, lane);
+        const unsigned long long all = warp_add(sum);
+        // `all` is at least the most likely token's 2^32
+        const double t = (double)p.u[b] * (double)all;
+        unsigned long long goal = t > 0.0 ? (t < (double)all ? (unsigned long long)t : all - 1) : 0;
+        if (goal > all - 1) goal = all - 1;
+        if (lane == 0) s.owner = -1;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < MAXC * NW / 32; ++i) {
+            const int r = lane * each_lane + i;
+            if (gts[i] && goal >= at && goal - at < gts[i] && r / NW == rank) {
+                s.owner = r % NW;
+                s.goal = goal - at;
+                s.eq_left = left[i];
+            }
+            at += gts[i];
+        }
+    }
+    __syncthreads();
+    if (s.owner == warp) {
+        unsigned long long at = 0;
+        const unsigned long long goal = s.goal;
+        uint32_t left = s.eq_left;
+        const T *w = seg + warp * range;
+        for (int i0 = 0; i0 < range; i0 += 32 * VEC) {
+            const int i = i0 + lane * VEC;
+            float x[VEC], z[VEC];
+            unsigned long long wt[VEC], sum = 0;
+            uint32_t eqn = 0;
+            if (i < range) {
+                Row<T>::get(w + i, x);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) x[v] = -INFINITY;
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                wt[v] = 0;
+                z[v] = sc.z(x[v]);
+                if (x[v] >= xcut && x[v] > -INFINITY) {
+                    const float e = expf(z[v]);
+                    if (!(e < need)) {
+                        wt[v] = weight(e);
+                        eqn += x[v] == xcut;
+                    }
+                }
+            }
+            uint32_t before = warp_before(eqn, lane);
+            const uint32_t eq_all = warp_add(eqn);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if (x[v] == xcut && wt[v]) {
+                    if (before >= left) wt[v] = 0;
+                    ++before;
+                }
+                sum += wt[v];
+            }
+            left = left > eq_all ? left - eq_all : 0;
+            unsigned long long c = at + warp_before(sum, lane);
+            if (goal >= c && goal - c < sum) {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    if (goal >= c && goal - c < wt[v]) {
+                        p.token[b] = first + i + v;
+                        if (p.logprob) p.logprob[b] = z[v] - logf((float)total * (1.f / 4294967296.f));
+                    }
+                    c += wt[v];
+                }
+            }
+            at += warp_add(sum);
+            if (at > goal) break;
+        }
+    }
+    cl.sync();  // nobody leaves while its shared memory is read
+}
+
+}  // namespace
+
+cudaError_t launch_sample(SampleParams p, int dtype, int sms, cudaStream_t st) {
+    const int vec = dtype == PMA_F32 ? 4 : 8, esize = dtype == PMA_F32 ? 4 : 2;
+    // CTAs of a row: enough that a segment is at most 64 KB (two or three CTAs fit an SM), more while
+    // the batch leaves SMs without one and a warp keeps a vector a lane.
+    int nc = 1;
+    while (nc < MAXC && ((int64_t)p.V * esize > (int64_t)nc * 65536 ||
+                         ((int64_t)p.B * nc < sms && p.V >= nc * 2 * NW * 32 * vec)))
+        nc *= 2;
+    p.range = ((p.V + nc * NW - 1) / (nc * NW) + vec - 1) / vec * vec;
+    const int smem = (int)((sizeof(Shared) + 15) / 16 * 16) + NW * p.range * esize;
+    cudaError_t e;
+    constexpr int most = 227 * 1024;
+    if (dtype == PMA_F32)
+        e = set_smem_once<sample_kernel<float>>(most);
+    else
+        e = set_smem_once<sample_kernel<__nv_bfloat16>>(most);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.B * nc));
+    cfg.blockDim = dim3(NW * 32);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)nc;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = dtype == PMA_F32 ? cudaLaunchKernelEx(&cfg, sample_kernel<float>, p)
+                         : cudaLaunchKernelEx(&cfg, sample_kernel<__nv_bfloat16>, p);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace pma
