@@ -537,6 +537,37 @@ PMA_API int pma_sample(int B, int V, const void *logits, int64_t row_stride, int
                        const float *min_p, float min_p_value,
                        int64_t *tokens, float *logprobs, pma_stream_t stream);
 
+/*
+ * e4m3 products with float32 scales per block of 128.  A quantised array is its bytes
+ * (rows on 16-byte boundaries, row stride in bytes a multiple of 16, K contiguous) and its scales; the value of an
+ * element is its e4m3 value times its block's scale.
+ *
+ *   rows of activations: one scale per row and 128 of K, scale[m * scale_stride_m +
+ *     j * scale_stride_k]; weights: one per 128 rows and 128 of K, [ceil(N/128), ceil(K/128)]
+ *     with a row stride.
+ *   quantisation: amax over the block (at least 2^-100), scale = amax / 448, element =
+ *     e4m3(448 x / amax), rounded to nearest even.  A block with a NaN or an infinity
+ *     gives NaN.
+ *   pma_fp8_matmul: y[m, n] = sum_k x[m, k] w[n, k], each K block summed by the tensor
+ *     cores, scaled and accumulated in float32, rounded once to y's dtype.
+ *   pma_fp8_linear: quantises x [M, K] (PMA_BF16 or PMA_F32) and multiplies, with scratch
+ *     of pma_fp8_linear_workspace_bytes(M, K) on a 256-byte boundary.
+ */
+PMA_API int pma_fp8_quantize(int M, int K, const void *x, int64_t x_stride, int dtype,
+                             void *q, int64_t q_stride, float *scale,
+                             int64_t scale_stride_m, int64_t scale_stride_k, pma_stream_t stream);
+PMA_API int pma_fp8_quantize_weight(int N, int K, const void *w, int64_t w_stride, int dtype,
+                                    void *q, int64_t q_stride, float *scale, pma_stream_t stream);
+PMA_API int pma_fp8_matmul(int M, int N, int K, const void *xq, int64_t xq_stride, const float *x_scale,
+                           int64_t x_scale_stride_m, int64_t x_scale_stride_k,
+                           const void *wq, int64_t wq_stride, const float *w_scale, int64_t w_scale_stride,
+                           void *y, int64_t y_stride, int y_dtype, pma_stream_t stream);
+PMA_API size_t pma_fp8_linear_workspace_bytes(int M, int K);
+PMA_API int pma_fp8_linear(int M, int N, int K, const void *x, int64_t x_stride, int x_dtype,
+                           const void *wq, int64_t wq_stride, const float *w_scale, int64_t w_scale_stride,
+                           void *y, int64_t y_stride, int y_dtype,
+                           void *workspace, size_t workspace_bytes, pma_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -156,6 +156,16 @@ def load() -> ctypes.CDLL:
                              ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
                              ctypes.c_void_p, ctypes.c_void_p]
     L.pma_sample.restype = ctypes.c_int
+    i, l, v = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+    for name, args in (("pma_fp8_quantize", [i, i, v, l, i, v, l, v, l, l, v]),
+                       ("pma_fp8_quantize_weight", [i, i, v, l, i, v, l, v, v]),
+                       ("pma_fp8_matmul", [i, i, i, v, l, v, l, l, v, l, v, l, v, l, i, v]),
+                       ("pma_fp8_linear", [i, i, i, v, l, i, v, l, v, l, v, l, i, v, ctypes.c_size_t, v])):
+        fn = getattr(L, name)
+        fn.argtypes = args
+        fn.restype = ctypes.c_int
+    L.pma_fp8_linear_workspace_bytes.argtypes = [i, i]
+    L.pma_fp8_linear_workspace_bytes.restype = ctypes.c_size_t
     _lib = L
     return L
 

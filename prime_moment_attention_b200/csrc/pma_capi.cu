@@ -4,9 +4,11 @@
 #include <cstring>
 #include <mutex>
 
+#include "fp8.cuh"
 #include "prefill.cuh"
 #include "recurrence.cuh"
 #include "sampling.cuh"
+#include "tc_common.cuh"
 
 using namespace pma;
 
@@ -168,6 +170,49 @@ ScanParams scan_params(int B, int L, int C, const pma_seq_tensor *x, const pma_s
     p.wait_ns = 2000000000ull;  // as the tensor-core kernels: 2 s per wait
     p.test_wait_ns = g_test_wait_ns.load(std::memory_order_acquire);
     return p;
+}
+
+// Rows of e4m3 bytes for a tensor map: 16-byte base and stride.
+int check_e4m3(const void *q, int64_t stride, int K) {
+    if (!q) return PMA_ERR_ARGUMENT;
+    if (stride < K || (uintptr_t)q % 16 || stride % 16) return PMA_ERR_LAYOUT;
+    return PMA_OK;
+}
+// The [M, K] or [N, K] input of a quantisation.
+int check_dense(const void *x, int64_t stride, int dtype, int rows, int K) {
+    if (!supported_dtype(dtype)) return PMA_ERR_DTYPE;
+    if (!x || (rows > 1 && stride < K)) return PMA_ERR_ARGUMENT;
+    return (uintptr_t)x % esize(dtype) ? PMA_ERR_LAYOUT : PMA_OK;
+}
+
+// Workspace of pma_fp8_linear: e4m3 rows of round16(K) bytes, then the scales [ceil(K/128), M].
+struct Fp8Ws {
+    int64_t stride;
+    size_t scale_at, bytes;
+    static Fp8Ws of(int M, int K) {
+        Fp8Ws w;
+        w.stride = ((int64_t)K + 15) / 16 * 16;
+        w.scale_at = ((size_t)M * w.stride + 255) / 256 * 256;
+        w.bytes = w.scale_at + (size_t)M * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4;
+        return w;
+    }
+};
+
+int fp8_product(int M, int N, int K, const Fp8Rows &x, const Fp8Rows &w, void *y, int64_t ys, int ydt, int sms,
+                cudaStream_t st) {
+    Fp8Params p{};
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.x = x;
+    p.w = w;
+    p.y = y;
+    p.ys = ys;
+    p.y_f32 = ydt == PMA_F32;
+    p.fault = g_fault_word.load(std::memory_order_acquire);
+    p.test_wait_ns = g_test_wait_ns.load(std::memory_order_acquire);
+    const cudaError_t e = launch_fp8_matmul(p, sms, st);
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 
 bool bf16_exact(float f) {
@@ -921,6 +966,69 @@ int pma_sample(int B, int V, const void *logits, int64_t row_stride, int dtype, 
     p.logprob = logprobs;
     cudaError_t e = launch_sample(p, dtype, di.sms, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_fp8_quantize(int M, int K, const void *x, int64_t x_stride, int dtype, void *q, int64_t q_stride, float *scale,
+                     int64_t scale_stride_m, int64_t scale_stride_k, pma_stream_t stream) {
+    if (M < 0 || K <= 0 || scale_stride_m < 0 || scale_stride_k < 0) return PMA_ERR_ARGUMENT;
+    if (M == 0) return PMA_OK;
+    int rc;
+    if ((rc = check_dense(x, x_stride, dtype, M, K)) || (rc = check_e4m3(q, q_stride, K))) return rc;
+    if (!scale) return PMA_ERR_ARGUMENT;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    const cudaError_t e = launch_fp8_quantize(x, x_stride, dtype, M, K, static_cast<uint8_t *>(q), q_stride, scale,
+                                              scale_stride_m, scale_stride_k, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_fp8_quantize_weight(int N, int K, const void *w, int64_t w_stride, int dtype, void *q, int64_t q_stride,
+                            float *scale, pma_stream_t stream) {
+    if (N < 0 || K <= 0) return PMA_ERR_ARGUMENT;
+    if (N == 0) return PMA_OK;
+    int rc;
+    if ((rc = check_dense(w, w_stride, dtype, N, K)) || (rc = check_e4m3(q, q_stride, K))) return rc;
+    if (!scale) return PMA_ERR_ARGUMENT;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    const cudaError_t e = launch_fp8_quantize_weight(w, w_stride, dtype, N, K, static_cast<uint8_t *>(q), q_stride,
+                                                     scale, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? PMA_OK : cuda_fail(e);
+}
+
+int pma_fp8_matmul(int M, int N, int K, const void *xq, int64_t xq_stride, const float *x_scale,
+                   int64_t x_scale_stride_m, int64_t x_scale_stride_k, const void *wq, int64_t wq_stride,
+                   const float *w_scale, int64_t w_scale_stride, void *y, int64_t y_stride, int y_dtype,
+                   pma_stream_t stream) {
+    if (M < 0 || N <= 0 || K <= 0 || x_scale_stride_m < 0 || x_scale_stride_k < 0) return PMA_ERR_ARGUMENT;
+    if (!supported_dtype(y_dtype)) return PMA_ERR_DTYPE;
+    if (M == 0) return PMA_OK;
+    int rc;
+    if ((rc = check_e4m3(xq, xq_stride, K)) || (rc = check_e4m3(wq, wq_stride, K))) return rc;
+    const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+    if (!x_scale || !w_scale || w_scale_stride < blocks || !y || (M > 1 && y_stride < N)) return PMA_ERR_ARGUMENT;
+    if ((uintptr_t)y % esize(y_dtype)) return PMA_ERR_LAYOUT;
+    DevInfo di;
+    if ((rc = device_info(&di))) return rc;
+    return fp8_product(M, N, K, {static_cast<const uint8_t *>(xq), xq_stride, x_scale, x_scale_stride_m, x_scale_stride_k},
+                       {static_cast<const uint8_t *>(wq), wq_stride, w_scale, w_scale_stride, 1}, y, y_stride, y_dtype,
+                       di.sms, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t pma_fp8_linear_workspace_bytes(int M, int K) { return M <= 0 || K <= 0 ? 0 : Fp8Ws::of(M, K).bytes; }
+
+int pma_fp8_linear(int M, int N, int K, const void *x, int64_t x_stride, int x_dtype, const void *wq, int64_t wq_stride,
+                   const float *w_scale, int64_t w_scale_stride, void *y, int64_t y_stride, int y_dtype,
+                   void *workspace, size_t workspace_bytes, pma_stream_t stream) {
+    if (M < 0 || N <= 0 || K <= 0) return PMA_ERR_ARGUMENT;
+    if (M == 0) return PMA_OK;
+    const Fp8Ws w = Fp8Ws::of(M, K);
+    if (workspace_bytes < w.bytes || !workspace || (uintptr_t)workspace % 256) return PMA_ERR_WORKSPACE;
+    float *scale = reinterpret_cast<float *>((char *)workspace + w.scale_at);
+    const int rc = pma_fp8_quantize(M, K, x, x_stride, x_dtype, workspace, w.stride, scale, 1, M, stream);
+    return rc ? rc
+              : pma_fp8_matmul(M, N, K, workspace, w.stride, scale, 1, M, wq, wq_stride, w_scale, w_scale_stride, y,
+                               y_stride, y_dtype, stream);
 }
 
 int pma_state_combine(int B, int H, int D, const float *lambda, int64_t lambda_stride_b, int64_t len,

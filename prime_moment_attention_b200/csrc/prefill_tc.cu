@@ -954,6 +954,19 @@ bool make_tile_map(CUtensorMap *m, const Seq &s, int B, int H, int L, int Dh) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// [rows, cols] bytes with a row stride in bytes: boxes of 128 bytes x box_rows, 128-byte swizzle.
+bool make_map_2d_u8(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
+    EncodeTiled enc = get_encode();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t str[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t es[2] = {1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, str, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool SO, typename TO, bool PRO, bool PT>
 static cudaError_t launch_t(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
                             const PrefillParams &p0, dim3 grid, cudaStream_t st) {

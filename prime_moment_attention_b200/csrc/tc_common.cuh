@@ -360,6 +360,8 @@ __device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 12
 // (d, l, h, b) over a [B,H,L,Dh] bf16 tensor with a 64 x 128 x 1 x 1 box and the 128-byte swizzle.
 bool tensor_maps_available();
 bool make_tile_map(CUtensorMap *m, const Seq &s, int B, int H, int L, int Dh);
+// [rows, cols] bytes, 128-byte-swizzled boxes of 128 bytes x box_rows (base and stride multiples of 16)
+bool make_map_2d_u8(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t stride, int box_rows);
 
 }  // namespace tc
 }  // namespace pma

@@ -1,0 +1,143 @@
+"""Block-scaled e4m3 quantisation and product against plain forms in float64.
+
+Tolerances.  Quantisation is exact in its definition: e4m3(448 x / amax) with one float32 division;
+the same expression in torch, tensor by tensor, gives the same bytes.  A product's terms are exact in
+float32 (two 4-bit significands); a K block's sum of 128 of them and the sum over J blocks round by at most (128 + J)
+2^-24 of the sum of magnitudes (any order; the tensor cores may truncate: 2^-23), and the scales'
+product and the multiply by 3 2^-24 more: (300 + 2 J) 2^-23 of sum |x w| bounds a float32 result.
+bf16 adds 2^-8 of the value.
+"""
+import pytest
+import torch
+
+from prime_moment_attention_b200 import _lib, fp8, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _pad(x, r, c):
+    return torch.nn.functional.pad(x, (0, c - x.shape[1], 0, r - x.shape[0]))
+
+
+def _over448(amax):
+    """The correctly rounded quotient (torch divides by a number through its reciprocal)."""
+    return (amax.double() / 448.0).float()
+
+
+def _plain_rows(x):
+    M, K = x.shape
+    kb = -(-K // 128)
+    g = _pad(x.float(), M, kb * 128).view(M, kb, 128)
+    amax = g.abs().amax(2, keepdim=True).clamp_min(2.0 ** -100)
+    return (g * 448.0 / amax).to(torch.float8_e4m3fn).view(M, -1)[:, :K], _over448(amax)[..., 0]
+
+
+def _plain_blocks(w):
+    N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    g = _pad(w.float(), nb * 128, kb * 128).view(nb, 128, kb, 128)
+    amax = g.abs().amax((1, 3), keepdim=True).clamp_min(2.0 ** -100)
+    q = (g * 448.0 / amax).to(torch.float8_e4m3fn).view(nb * 128, -1)[:N, :K]
+    return q, _over448(amax)[:, 0, :, 0]
+
+
+def _dequant(q, s, rows):
+    K = q.shape[1]
+    return q.double() * s.double().repeat_interleave(rows, 0)[: q.shape[0]].repeat_interleave(128, 1)[:, :K]
+
+
+def _data(M, N, K, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + M + 3 * N + 7 * K)
+    x = torch.randn(M, K, generator=g) * torch.exp(torch.randn(1, K, generator=g))
+    w = torch.randn(N, K, generator=g) / K ** 0.5 * torch.exp(torch.randn(N, 1, generator=g))
+    return x.to(dtype).cuda(), w.to(dtype).cuda()
+
+
+def _check_product(y, xq, xs, wq, ws):
+    x, w = _dequant(xq, xs, 1), _dequant(wq, ws, 128)
+    want, mag = x @ w.t(), x.abs() @ w.abs().t()
+    J = -(-xq.shape[1] // 128)
+    bar = (300 + 2 * J) * 2.0 ** -23 * mag + (2.0 ** -8 * want.abs() if y.dtype == torch.bfloat16 else 0.0)
+    err = (y.double() - want).abs()
+    assert (err <= bar).all(), (float((err / bar.clamp_min(1e-300)).max()), int((err > bar).sum()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 127), (5, 128), (64, 768), (33, 1000), (300, 2050)])
+def test_quantisation_is_bit_exact(M, K, dtype):
+    x, w = _data(M, M, K, dtype)
+    x[0] = 0                                     # an empty block
+    x[-1] *= 1e-3
+    if M > 2:
+        x[1] = x[1] * 1e36 if dtype == torch.float32 else x[1] * 1e35
+    q, s = fp8.quantize(x)
+    pq, ps = _plain_rows(x)
+    keep = x.float().abs().amax(1) < 1e35        # 448 x overflows in the plain form beyond
+    assert torch.equal(q[keep].float(), pq[keep].float()) and torch.equal(s, ps)
+    assert torch.isfinite(q.float()).all() and float(q.float().abs().max()) <= 448.0
+    q, s = fp8.quantize_weight(w)
+    pq, ps = _plain_blocks(w)
+    assert torch.equal(q.float(), pq.float()) and torch.equal(s, ps)
+
+
+SIZES = [(1, 1, 1), (1, 768, 2048), (2, 130, 128), (16, 128, 4096), (17, 100, 300), (32, 1000, 640), (50, 3000, 768),
+         (64, 32000, 768), (65, 129, 257), (128, 128, 128), (129, 257, 1000), (200, 64, 5000), (777, 1530, 1000),
+         (1024, 2048, 768), (2500, 2300, 512), (4096, 2560, 384), (8, 64, 8192)]
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_product(M, N, K, out):
+    x, w = _data(M, N, K, torch.bfloat16)
+    (xq, xs), (wq, ws) = fp8.quantize(x), fp8.quantize_weight(w)
+    _check_product(fp8.matmul(xq, xs, wq, ws, out_dtype=out), xq, xs, wq, ws)
+    y = fp8.linear(x, wq, ws, out_dtype=out)
+    _check_product(y, xq, xs, wq, ws)
+    assert torch.equal(y, fp8.linear(x, wq, ws, out_dtype=out))  # repeats bit for bit
+
+
+def test_layouts():
+    """Scales and rows with other strides, outputs inside wider arrays, unaligned weights (copied)."""
+    x, w = _data(70, 200, 500, torch.float32)
+    (xq, xs), (wq, ws) = fp8.quantize(x), fp8.quantize_weight(w)
+    want = fp8.matmul(xq, xs, wq, ws)
+    assert torch.equal(want, fp8.matmul(xq, xs.contiguous(), wq, ws))
+    wide = torch.zeros(70, 777, dtype=torch.bfloat16).cuda()
+    fp8.matmul(xq, xs, wq, ws, out=wide[:, 5:205])
+    assert torch.equal(wide[:, 5:205], want) and not wide[:, :5].any() and not wide[:, 205:].any()
+    assert torch.equal(want, fp8.matmul(xq, xs, wq.contiguous(), ws))  # rows of 500 bytes
+    assert torch.equal(want, fp8.matmul(xq, xs, wq, torch.cat([ws, ws], 1)[:, :4]))
+    assert torch.equal(want, fp8.linear(x, wq, ws))
+    cols = torch.zeros(70, 3 * 500).cuda()
+    cols[:, 500:1000] = x
+    assert torch.equal(want, fp8.linear(cols[:, 500:1000], wq, ws))
+    assert torch.equal(want, fp8.linear(x.view(7, 10, 500), wq, ws).view(70, 200))
+    assert torch.equal(want, fp8.linear(x.t().contiguous().t(), wq, ws))
+
+
+def test_empty_and_nan():
+    x, w = _data(4, 256, 256, torch.bfloat16)
+    wq, ws = fp8.quantize_weight(w)
+    assert fp8.linear(x[:0], wq, ws).shape == (0, 256)
+    x[1, 130] = float("nan")
+    x[2, 3] = float("inf")
+    y = fp8.linear(x, wq, ws)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all() and torch.isfinite(y[[0, 3]]).all()
+
+
+def test_expired_wait_is_reported():
+    x, w = _data(300, 256, 256, torch.bfloat16)
+    wq, ws = fp8.quantize_weight(w)
+    ops.check_faults(synchronize=True)
+    for m in (300, 8):
+        _lib.load().pma_test_expire_waits(1_000_000)
+        try:
+            fp8.linear(x[:m], wq, ws)
+        finally:
+            _lib.load().pma_test_expire_waits(0)
+        torch.cuda.synchronize()
+        with pytest.raises(ops.KernelFault) as e:
+            fp8.linear(x[:m], wq, ws)
+        assert e.value.code == 130
+        fp8.linear(x[:m], wq, ws)
+        ops.check_faults(synchronize=True)
