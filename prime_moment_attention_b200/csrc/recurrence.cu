@@ -48,58 +48,136 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
-// exp(min(u, 87)), NaN kept: finite, so that exp(u) sigmoid(-u) is a sigmoid and not inf * 0
-__device__ __forceinline__ float exp_sat(float u) {
+// 2^min(x, 126), NaN kept: finite, so that exp(u) sigmoid(-u) is a sigmoid and not inf * 0
+__device__ __forceinline__ float ex2_sat(float x) {
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(u * LOG2E), "f"(126.0f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(126.0f));
     return ex2(r);
 }
-__device__ __forceinline__ float sigmoid_neg(float u) { return rcp(1.0f + exp_sat(u)); }
-__device__ __forceinline__ float sigmoid(float u) { return rcp(1.0f + ex2(-u * LOG2E)); }
+
+// V float32 values of a lane (its channels): pairs go through the two-wide float32 instructions,
+// which halve the arithmetic a channel costs.
+template <int V> struct Vf;
+template <> struct Vf<1> {
+    float v;
+    static __device__ __forceinline__ Vf all(float a) { return {a}; }
+    __device__ __forceinline__ float at(int) const { return v; }
+    __device__ __forceinline__ void set(int, float a) { v = a; }
+};
+template <> struct Vf<2> {
+    unsigned long long v;
+    static __device__ __forceinline__ Vf of(float a, float b) {
+        Vf r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+        return r;
+    }
+    static __device__ __forceinline__ Vf all(float a) { return of(a, a); }
+    __device__ __forceinline__ float at(int i) const {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+        return i ? b : a;
+    }
+    __device__ __forceinline__ void set(int i, float a) { *this = i ? of(at(0), a) : of(a, at(1)); }
+};
+__device__ __forceinline__ Vf<1> fma(Vf<1> a, Vf<1> b, Vf<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Vf<1> mul(Vf<1> a, Vf<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Vf<1> add(Vf<1> a, Vf<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Vf<2> fma(Vf<2> a, Vf<2> b, Vf<2> c) {
+    Vf<2> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Vf<2> mul(Vf<2> a, Vf<2> b) {
+    Vf<2> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Vf<2> add(Vf<2> a, Vf<2> b) {
+    Vf<2> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+template <int V, typename F> __device__ __forceinline__ Vf<V> each(Vf<V> a, F f) {
+    if constexpr (V == 1)
+        return {f(a.v)};
+    else
+        return Vf<2>::of(f(a.at(0)), f(a.at(1)));
+}
+
+// sigmoid(-u) for u in units of log 2; sigmoid(g)
+template <int V> __device__ __forceinline__ Vf<V> sigmoid_neg2(Vf<V> u) {
+    return each(add(each(u, ex2_sat), Vf<V>::all(1.f)), rcp);
+}
+template <int V> __device__ __forceinline__ Vf<V> sigmoid(Vf<V> g) {
+    return each(add(each(mul(g, Vf<V>::all(-LOG2E)), ex2), Vf<V>::all(1.f)), rcp);
+}
 
 // One token.  This form is exact at both ends (z = 0 keeps h, z = 1 takes x); rounding 1 - z costs a
 // slow decay half an ulp a row, over the few rows between two joins.
-__device__ __forceinline__ float advance(float h, float z, float x) { return fmaf(1.f - z, h, z * x); }
+template <int V> __device__ __forceinline__ Vf<V> advance(Vf<V> h, Vf<V> z, Vf<V> x) {
+    return fma(fma(z, Vf<V>::all(-1.f), Vf<V>::all(1.f)), h, mul(z, x));
+}
 
-// the state h after a run (Q, H); Q = 1 cuts it off, whatever it was
-__device__ __forceinline__ float join(float h, float q, float hh) {
-    return q == 1.0f ? hh : h + fmaf(-q, h, hh);
+// A run of tokens: n = -Q and H
+template <int V> struct Run {
+    Vf<V> n, h;
+};
+template <int V> __device__ __forceinline__ Run<V> no_run() { return {Vf<V>::all(0.f), Vf<V>::all(0.f)}; }
+// the state after a run; with CUT, Q = 1 drops the state whatever it was (a reset, or a state handed on)
+template <bool CUT, int V> __device__ __forceinline__ Vf<V> join(Vf<V> h, const Run<V> &r) {
+    Vf<V> o = add(h, fma(r.n, h, r.h));
+    if (CUT) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (r.n.at(v) == -1.f) o.set(v, r.h.at(v));
+    }
+    return o;
+}
+// run a, then run b
+template <bool CUT, int V> __device__ __forceinline__ Run<V> join(const Run<V> &a, const Run<V> &b) {
+    Run<V> o{fma(b.n, add(a.n, Vf<V>::all(1.f)), a.n), join<CUT>(a.h, b)};
+    if (CUT) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (b.n.at(v) == -1.f) o.n.set(v, -1.f);
+    }
+    return o;
 }
 
 // V consecutive channels of one row as one load or store
 template <typename T, int V> struct Pack;
 template <> struct Pack<float, 1> {
     float r;
-    static constexpr int bytes = 4;
-    __device__ __forceinline__ void zero() { r = 0.f; }
-    __device__ __forceinline__ void load(const float *p, int) { r = __ldg(p); }
-    __device__ __forceinline__ float at(int) const { return r; }
-    static __device__ __forceinline__ void store(float *p, const float (&v)[1], int) { *p = v[0]; }
+    __device__ __forceinline__ void load(const float *p) { r = __ldg(p); }
+    __device__ __forceinline__ Vf<1> f() const { return {r}; }
+    static __device__ __forceinline__ void store(float *p, Vf<1> v) { *p = v.v; }
 };
 template <> struct Pack<__nv_bfloat16, 1> {
     uint16_t r;
-    __device__ __forceinline__ void zero() { r = 0; }
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p, int) {
-        r = __ldg(reinterpret_cast<const unsigned short *>(p));
-    }
-    __device__ __forceinline__ float at(int) const { return __uint_as_float((uint32_t)r << 16); }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[1], int) {
-        *p = __float2bfloat16_rn(v[0]);
-    }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = __ldg(reinterpret_cast<const unsigned short *>(p)); }
+    __device__ __forceinline__ Vf<1> f() const { return {__uint_as_float((uint32_t)r << 16)}; }
+    static __device__ __forceinline__ void store(__nv_bfloat16 *p, Vf<1> v) { *p = __float2bfloat16_rn(v.v); }
 };
 template <> struct Pack<__nv_bfloat16, 2> {
     uint32_t r;
-    __device__ __forceinline__ void zero() { r = 0; }
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p, int) {
-        r = __ldg(reinterpret_cast<const unsigned int *>(p));
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = __ldg(reinterpret_cast<const unsigned int *>(p)); }
+    __device__ __forceinline__ Vf<2> f() const {
+        return Vf<2>::of(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
     }
-    __device__ __forceinline__ float at(int i) const {
-        return __uint_as_float(i ? r & 0xffff0000u : r << 16);
-    }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[2], int) {
-        *reinterpret_cast<uint32_t *>(p) = tc::pack2(v[0], v[1]);
+    static __device__ __forceinline__ void store(__nv_bfloat16 *p, Vf<2> v) {
+        *reinterpret_cast<uint32_t *>(p) = tc::pack2(v.at(0), v.at(1));
     }
 };
+
+// The rows stay packed in registers between two passes: without this the compiler keeps the unpacked
+// float32 values as well and spills.
+__device__ __forceinline__ void keep_packed(float &) {}
+__device__ __forceinline__ void keep_packed(uint16_t &r) { asm volatile("" : "+h"(r)); }
+__device__ __forceinline__ void keep_packed(uint32_t &r) { asm volatile("" : "+r"(r)); }
+template <typename P, int R> __device__ __forceinline__ void keep_packed(P (&d)[R]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) keep_packed(d[r].r);
+}
 
 __device__ __forceinline__ uint32_t word_of(float v) {
     const uint32_t u = __float_as_uint(v);
@@ -108,8 +186,8 @@ __device__ __forceinline__ uint32_t word_of(float v) {
 __device__ __forceinline__ void put32(uint32_t *p, float v) {
     asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(word_of(v)) : "memory");
 }
-__device__ __forceinline__ void put64(unsigned long long *p, float q, float h) {
-    const unsigned long long v = ((unsigned long long)word_of(h) << 32) | word_of(q);
+__device__ __forceinline__ void put64(unsigned long long *p, float n, float h) {
+    const unsigned long long v = ((unsigned long long)word_of(h) << 32) | word_of(n);
     asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t get32(const uint32_t *p) {
@@ -123,17 +201,38 @@ __device__ __forceinline__ unsigned long long get64(const unsigned long long *p)
     return v;
 }
 
-// The run (Q, H) of a tile before this one, or the state leaving it as the run (1, state).
-// `must_end`: wait for the state.
-__device__ __forceinline__ float2 fetch(const ScanParams &p, int64_t at, bool must_end) {
+// The runs of V channels of a tile before this one, or the states leaving it as runs (-1, state).
+// `must_end`: wait for the states.
+template <int V> __device__ __forceinline__ Run<V> fetch(const ScanParams &p, int64_t at, bool must_end) {
     unsigned long long t0 = 0;
+    float n[V], h[V];
+    bool got[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) got[v] = false;
     for (uint32_t it = 1;; ++it) {
-        const uint32_t s = get32(p.incl + at);
-        if (s != EMPTY) return make_float2(1.0f, __uint_as_float(s));
-        if (!must_end) {
-            const unsigned long long a = get64(p.agg + at);
-            if (a != ~0ull) return make_float2(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)));
+        bool all = true;
+        uint32_t s[V];
+        unsigned long long a[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {  // every load is in flight before the first is looked at
+            s[v] = get32(p.incl + at + v);
+            a[v] = must_end ? ~0ull : get64(p.agg + at + v);
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (got[v]) continue;
+            if (s[v] != EMPTY) {
+                n[v] = -1.f;
+                h[v] = __uint_as_float(s[v]);
+                got[v] = true;
+            } else if (a[v] != ~0ull) {
+                n[v] = __uint_as_float((uint32_t)a[v]);
+                h[v] = __uint_as_float((uint32_t)(a[v] >> 32));
+                got[v] = true;
+            }
+            all = all && got[v];
+        }
+        if (all) break;
         if ((it & 255) == 0) {
             const unsigned long long now = tc::gtimer();
             if (!t0) t0 = now;
@@ -141,10 +240,22 @@ __device__ __forceinline__ float2 fetch(const ScanParams &p, int64_t at, bool mu
             if (gone || now - t0 > p.wait_ns) {
                 *reinterpret_cast<volatile int *>(p.counter + 1) = FAULT_CODE;
                 tc::report_fault(FAULT_CODE, p.fault);
-                return make_float2(1.0f, __uint_as_float(0x7fffffffu));
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    n[v] = -1.f;
+                    h[v] = __uint_as_float(0x7fffffffu);
+                }
+                break;
             }
         }
     }
+    Run<V> r = no_run<V>();
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        r.n.set(v, n[v]);
+        r.h.set(v, h[v]);
+    }
+    return r;
 }
 
 // Test hook: a wait that nothing ends runs out, and the launch gives up before any other work.
@@ -176,331 +287,292 @@ __device__ __forceinline__ Tile tile_of(const ScanParams &p, int t, int lane) {
     return k;
 }
 
-// Publish this tile's run, gather the runs of the W tiles that precede it in walking order (the
-// last of them as a state) and return the state that enters the tile; publish the one that leaves.
-// `slot(i)`: word of the tile i steps earlier.  Called by all warps; s_run holds W x 32 V runs.
-template <int V, int W, typename Slot, typename First>
-__device__ __forceinline__ void chain(const ScanParams &p, const Tile &k, const float (&q)[V], const float (&h)[V],
-                                      float (&in)[V], float2 (*s_run)[32 * V], float (*s_in), int warp, int lane,
-                                      bool live, bool publish, Slot slot, First first) {
+template <int V, int W> struct Scratch {
+    Run<V> run[W][32];
+    Vf<V> in[32];
+    int tile;
+};
+
+// Publish this tile's run (warp 0 holds it), gather the runs of the W tiles that precede it in
+// walking order (the last of them as a state) and return the state that enters the tile; publish
+// the one that leaves, which `last` receives (warp 0).
+template <bool CUT, int V, int W, typename First, typename Last>
+__device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const Run<V> &whole, Scratch<V, W> &sm,
+                                       int warp, int lane, bool live, First first, Last last) {
+    const int64_t slot = k.word0 + (int64_t)k.chunk * p.C;
+    Vf<V> in = Vf<V>::all(0.f);
     if (k.chunk == 0) {
+        if (live) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) in[v] = live ? first(v) : 0.f;
-        if (publish && warp == 0 && live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) put32(p.incl + slot(0) + v, join(in[v], q[v], h[v]));
+            for (int v = 0; v < V; ++v) in.set(v, first(v));
         }
-        return;
+    } else {
+        if (warp == 0 && live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) put64(p.agg + slot + v, whole.n.at(v), whole.h.at(v));
+        }
+        const int reach = k.chunk < W ? k.chunk : W;
+        if (warp < reach)
+            sm.run[warp][lane] =
+                live ? fetch<V>(p, slot - (int64_t)(warp + 1) * p.C, warp == reach - 1) : no_run<V>();
+        __syncthreads();
+        if (warp == 0) {
+            for (int i = reach - 1; i >= 0; --i) in = join<true>(in, sm.run[i][lane]);
+            sm.in[lane] = in;
+        }
     }
     if (warp == 0 && live) {
+        const Vf<V> out = join<CUT>(in, whole);
+        if (p.chunks > 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) put64(p.agg + slot(0) + v, q[v], h[v]);
-    }
-    const int reach = k.chunk < W ? k.chunk : W;
-    if (warp < reach) {
-        const bool end = warp == reach - 1;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            s_run[warp][lane * V + v] = live ? fetch(p, slot(warp + 1) + v, end) : make_float2(1.f, 0.f);
-    }
-    __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float s = 0.f;
-            for (int i = reach - 1; i >= 0; --i) {
-                const float2 r = s_run[i][lane * V + v];
-                s = join(s, r.x, r.y);
-            }
-            s_in[lane * V + v] = s;
-            if (live && publish) put32(p.incl + slot(0) + v, join(s, q[v], h[v]));
+            for (int v = 0; v < V; ++v) put32(p.incl + slot + v, out.at(v));
         }
+        if (k.chunk == p.chunks - 1) last(out);
     }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) in[v] = s_in[lane * V + v];
+    if (k.chunk) {
+        __syncthreads();
+        in = sm.in[lane];
+    }
+    return in;
 }
 
 __device__ __forceinline__ uint32_t reset_mask(const ScanParams &p, int b, int row0, int rows, int lane) {
-    if (!p.reset) return 0;
     const int l = row0 + lane;
     const bool r = lane < rows && l < p.L && p.reset[(int64_t)b * p.L + l] != 0;
     return __ballot_sync(0xffffffffu, r);
 }
 
+// R rows of a lane's channels.  Rows past the end and channels past C are read again from the last
+// ones: every address is valid and nothing has to be skipped.
+template <typename T, int V, int R>
+__device__ __forceinline__ void load_rows(Pack<T, V> (&d)[R], const Blc &t, int b, int l0, int L, int c) {
+    const T *p = static_cast<const T *>(t.p) + b * t.sb + l0 * t.sl + c;
+    if (l0 + R <= L) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) d[r].load(p + r * t.sl);
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) d[r].load(p + (int64_t)min(r, L - 1 - l0) * t.sl);
+    }
+}
+
 // ------------------------------------------------------------------------------------- forward
-template <typename T, int V, int W, int R, bool GATE>
+template <typename T, int V, int W, int R, bool GATE, bool CUT>
 __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ float2 s_run[W][32 * V];
-    __shared__ float s_in[32 * V];
-    __shared__ int s_tile;
+    __shared__ Scratch<V, W> sm;
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int t = blockIdx.x;
     if (p.chunks > 1) {
-        if (threadIdx.x == 0) s_tile = atomicAdd(p.counter, 1) + 1;
+        if (threadIdx.x == 0) sm.tile = atomicAdd(p.counter, 1) + 1;
         __syncthreads();
-        t = s_tile;
+        t = sm.tile;
     }
     const Tile k = tile_of<V>(p, t, lane);
     const bool live = k.c < p.C;
-    const int l0 = k.chunk * SCAN_ROWS + warp * R;
-    const int rows = live ? min(R, p.L - l0) : 0;
+    const int l0 = k.chunk * SCAN_ROWS + warp * R, rows = min(R, p.L - l0), c = live ? k.c : p.C - V;
 
     Pack<T, V> x[R], f[R], o[GATE ? R : 1];
+    load_rows<T, V, R>(f, p.f, k.b, l0, p.L, c);
+    load_rows<T, V, R>(x, p.x, k.b, l0, p.L, c);
+    if constexpr (GATE) load_rows<T, V, R>(o, p.gate, k.b, l0, p.L, c);
+    const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
+    Vf<V> bias = Vf<V>::all(0.f), z[R];
+    if (p.bias) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) z[r] = sigmoid_neg2(fma(f[r].f(), Vf<V>::all(LOG2E), bias));
+    if (rows < R) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r >= rows) z[r] = Vf<V>::all(0.f);
+    }
     {
-        const T *xp = static_cast<const T *>(p.x.p) + k.b * p.x.sb + l0 * p.x.sl + k.c;
-        const T *fp = static_cast<const T *>(p.f.p) + k.b * p.f.sb + l0 * p.f.sl + k.c;
-        const T *op = GATE ? static_cast<const T *>(p.gate.p) + k.b * p.gate.sb + l0 * p.gate.sl + k.c : nullptr;
+        Vf<V> q = Vf<V>::all(0.f), h = q;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r < rows) {
-                f[r].load(fp + r * p.f.sl, V);
-                x[r].load(xp + r * p.x.sl, V);
-                if (GATE) o[GATE ? r : 0].load(op + r * p.gate.sl, V);
-            } else {
-                f[r].zero();
-                x[r].zero();
-                if (GATE) o[GATE ? r : 0].zero();
+            if (CUT && (cuts >> r & 1)) {
+                q = Vf<V>::all(1.f);
+                h = Vf<V>::all(0.f);
             }
+            h = advance(h, z[r], x[r].f());
+            q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
         }
-    }
-    const uint32_t cuts = reset_mask(p, k.b, l0, R, lane);
-    float z[R][V], q[V], h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const float bias = live && p.bias ? __ldg(p.bias + k.c + v) : 0.f;
-        q[v] = h[v] = 0.f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            z[r][v] = r < rows ? sigmoid_neg(f[r].at(v) + bias) : 0.f;
-            if (cuts >> r & 1) {
-                q[v] = 1.f;
-                h[v] = 0.f;
-            }
-            h[v] = advance(h[v], z[r][v], x[r].at(v));
-            q[v] = fmaf(z[r][v], 1.f - q[v], q[v]);
-        }
-        s_run[warp][lane * V + v] = make_float2(q[v], h[v]);
+        sm.run[warp][lane] = {mul(q, Vf<V>::all(-1.f)), h};
     }
     __syncthreads();
-    // this warp's place in the tile: the run before its rows, and the whole tile's
-    float pq[V], ph[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float cq = 0.f, ch = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w == warp) {
-                pq[v] = cq;
-                ph[v] = ch;
-            }
-            const float2 r = s_run[w][lane * V + v];
-            ch = join(ch, r.x, r.y);
-            cq = r.x == 1.f ? 1.f : fmaf(r.x, 1.f - cq, cq);
-        }
-        q[v] = cq;
-        h[v] = ch;
-    }
+    // the run of the tile's rows before this warp's; warp 0, which has none, joins the whole tile
+    Run<V> run = no_run<V>();
+    const int upto = warp ? warp : W;
+    for (int w = 0; w < upto; ++w) run = join<CUT>(run, sm.run[w][lane]);
     __syncthreads();
-    float in[V];
-    chain<V, W>(
-        p, k, q, h, in, s_run, s_in, warp, lane, live, p.chunks > 1,
-        [&](int i) { return k.word0 + (int64_t)(k.chunk - i) * p.C; },
-        [&](int v) { return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f; });
-    if (p.h_last && warp == 0 && k.chunk == p.chunks - 1 && live) {
+    const Vf<V> in = chain<CUT, V, W>(
+        p, k, run, sm, warp, lane, live, [&](int v) { return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f; },
+        [&](Vf<V> out) {
+            if (p.h_last) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.h_last[(int64_t)k.b * p.C + k.c + v] = join(in[v], q[v], h[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = join(in[v], pq[v], ph[v]);
-    T *yp = static_cast<T *>(p.y.p) + k.b * p.y.sb + l0 * p.y.sl + k.c;
+                for (int v = 0; v < V; ++v) p.h_last[(int64_t)k.b * p.C + k.c + v] = out.at(v);
+            }
+        });
+    Vf<V> h = warp ? join<CUT>(in, run) : in;
+    keep_packed(x);
+    if constexpr (GATE) keep_packed(o);
+    T *yp = static_cast<T *>(p.y.p) + k.b * p.y.sb + l0 * p.y.sl + c;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        float y[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (cuts >> r & 1) h[v] = 0.f;
-            h[v] = advance(h[v], z[r][v], x[r].at(v));
-            y[v] = h[v];
-            if (GATE) {
-                const float g = o[GATE ? r : 0].at(v);
-                y[v] *= g * sigmoid(g);
-            }
+        if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
+        h = advance(h, z[r], x[r].f());
+        Vf<V> y = h;
+        if constexpr (GATE) {
+            const Vf<V> g = o[r].f();
+            y = mul(y, mul(g, sigmoid(g)));
         }
-        if (r < rows) Pack<T, V>::store(yp + r * p.y.sl, y, V);
+        if (live && r < rows) Pack<T, V>::store(yp + r * p.y.sl, y);
     }
 }
 
 // ------------------------------------------------------------------------------------ backward
-template <typename T, int V, int W, int R, bool GATE>
+template <typename T, int V, int W, int R, bool GATE, bool CUT>
 __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ float2 s_fwd[W][32 * V], s_run[W][32 * V];
-    __shared__ float s_in[32 * V];
-    __shared__ int s_tile;
+    __shared__ Scratch<V, W> sm;
+    __shared__ Run<V> s_fwd[W][32];
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int t = blockIdx.x;
     if (p.chunks > 1) {
-        if (threadIdx.x == 0) s_tile = atomicAdd(p.counter, 1) + 1;
+        if (threadIdx.x == 0) sm.tile = atomicAdd(p.counter, 1) + 1;
         __syncthreads();
-        t = s_tile;
+        t = sm.tile;
     }
     const Tile k = tile_of<V>(p, t, lane);
     const bool live = k.c < p.C;
     const int chunk = p.chunks - 1 - k.chunk;  // the last tokens first
-    const int l0 = chunk * SCAN_ROWS + warp * R;
-    const int rows = live ? min(R, p.L - l0) : 0;
+    const int l0 = chunk * SCAN_ROWS + warp * R, rows = min(R, p.L - l0), c = live ? k.c : p.C - V;
 
     Pack<T, V> x[R], f[R], dy[R], o[GATE ? R : 1];
+    load_rows<T, V, R>(f, p.f, k.b, l0, p.L, c);
+    load_rows<T, V, R>(x, p.x, k.b, l0, p.L, c);
+    load_rows<T, V, R>(dy, p.dy, k.b, l0, p.L, c);
+    if constexpr (GATE) load_rows<T, V, R>(o, p.gate, k.b, l0, p.L, c);
+    Vf<V> start = Vf<V>::all(0.f), bias = start;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (chunk > 0)
+            start.set(v, __uint_as_float(p.states[((int64_t)k.b * p.chunks + chunk - 1) * p.C + c + v]));
+        else if (p.h0)
+            start.set(v, p.h0[(int64_t)k.b * p.C + c + v]);
+        if (p.bias) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
+    }
+    const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
+    Vf<V> z[R], sg[GATE ? R : 1];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        z[r] = sigmoid_neg2(fma(f[r].f(), Vf<V>::all(LOG2E), bias));
+        if constexpr (GATE) sg[r] = sigmoid(o[r].f());
+    }
+    // dL/dh_t through y_t; zero past the end, where z is zero too
+    auto into = [&](int r) {
+        Vf<V> s = dy[r].f();
+        if constexpr (GATE) s = mul(s, mul(o[r].f(), sg[r]));
+        if (r >= rows) s = Vf<V>::all(0.f);
+        return s;
+    };
+    if (rows < R) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r >= rows) z[r] = Vf<V>::all(0.f);
+    }
+    // the carry a g of one token
+    auto carry = [&](int r, Vf<V> g) {
+        if (CUT && (cuts >> r & 1)) return Vf<V>::all(0.f);
+        return fma(mul(z[r], Vf<V>::all(-1.f)), g, g);
+    };
     {
-        const T *xp = static_cast<const T *>(p.x.p) + k.b * p.x.sb + l0 * p.x.sl + k.c;
-        const T *fp = static_cast<const T *>(p.f.p) + k.b * p.f.sb + l0 * p.f.sl + k.c;
-        const T *dp = static_cast<const T *>(p.dy.p) + k.b * p.dy.sb + l0 * p.dy.sl + k.c;
-        const T *op = GATE ? static_cast<const T *>(p.gate.p) + k.b * p.gate.sb + l0 * p.gate.sl + k.c : nullptr;
+        Vf<V> q = Vf<V>::all(0.f), h = q, cc = q;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r < rows) {
-                f[r].load(fp + r * p.f.sl, V);
-                x[r].load(xp + r * p.x.sl, V);
-                dy[r].load(dp + r * p.dy.sl, V);
-                if (GATE) o[GATE ? r : 0].load(op + r * p.gate.sl, V);
-            } else {
-                f[r].zero();
-                x[r].zero();
-                dy[r].zero();
-                if (GATE) o[GATE ? r : 0].zero();
+            if (CUT && (cuts >> r & 1)) {
+                q = Vf<V>::all(1.f);
+                h = Vf<V>::all(0.f);
             }
-        }
-    }
-    float start[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-        start[v] = !live       ? 0.f
-                   : chunk > 0 ? __uint_as_float(p.states[k.word0 + (int64_t)(chunk - 1) * p.C + v])
-                   : p.h0      ? p.h0[(int64_t)k.b * p.C + k.c + v]
-                               : 0.f;
-    const uint32_t cuts = reset_mask(p, k.b, l0, R, lane);
-    float bias[V], z[R][V], sg[GATE ? R : 1][V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        bias[v] = live && p.bias ? __ldg(p.bias + k.c + v) : 0.f;
-        float q = 0.f, h = 0.f, c = 0.f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            z[r][v] = r < rows ? sigmoid_neg(f[r].at(v) + bias[v]) : 0.f;
-            if (cuts >> r & 1) {
-                q = 1.f;
-                h = 0.f;
-            }
-            h = advance(h, z[r][v], x[r].at(v));
-            q = fmaf(z[r][v], 1.f - q, q);
+            h = advance(h, z[r], x[r].f());
+            q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
         }
 #pragma unroll
-        for (int r = R - 1; r >= 0; --r) {
-            float s = dy[r].at(v);
-            if (GATE) {
-                const float g = o[GATE ? r : 0].at(v);
-                sg[GATE ? r : 0][v] = sigmoid(g);
-                s *= g * sg[GATE ? r : 0][v];
-            }
-            s += c;
-            c = cuts >> r & 1 ? 0.f : fmaf(-z[r][v], s, s);
-        }
-        s_fwd[warp][lane * V + v] = make_float2(q, h);
-        s_run[warp][lane * V + v] = make_float2(q, c);
+        for (int r = R - 1; r >= 0; --r) cc = carry(r, add(into(r), cc));
+        const Vf<V> n = mul(q, Vf<V>::all(-1.f));
+        keep_packed(x);
+        keep_packed(f);
+        keep_packed(dy);
+        if constexpr (GATE) keep_packed(o);
+        s_fwd[warp][lane] = {n, h};
+        sm.run[warp][lane] = {n, cc};
     }
     __syncthreads();
-    float q[V], g[V], sq[V], sc[V];  // the tile's run from the right; the run of the rows right of this warp's
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float cq = 0.f, cc = 0.f;
-#pragma unroll
-        for (int w = W - 1; w >= 0; --w) {
-            if (w == warp) {
-                sq[v] = cq;
-                sc[v] = cc;
-            }
-            const float2 r = s_run[w][lane * V + v];
-            cc = join(cc, r.x, r.y);
-            cq = r.x == 1.f ? 1.f : fmaf(r.x, 1.f - cq, cq);
-        }
-        q[v] = cq;
-        g[v] = cc;
-        float h = start[v];
-        for (int w = 0; w < warp; ++w) {
-            const float2 r = s_fwd[w][lane * V + v];
-            h = join(h, r.x, r.y);
-        }
-        start[v] = h;
+    // the carries of the rows right of this warp's; the last warp, which has none, joins the tile's
+    Run<V> run = no_run<V>();
+    {
+        const int mine = W - 1 - warp, upto = mine ? mine : W;
+        for (int i = 0; i < upto; ++i) run = join<CUT>(run, sm.run[W - 1 - i][lane]);
+        for (int w = 0; w < warp; ++w) start = join<CUT>(start, s_fwd[w][lane]);
     }
     __syncthreads();
-    float in[V];
-    chain<V, W>(
-        p, k, q, g, in, s_run, s_in, warp, lane, live, p.chunks > 1,
-        [&](int i) { return k.word0 + (int64_t)(k.chunk - i) * p.C; },
-        [&](int v) { return p.dh_last ? p.dh_last[(int64_t)k.b * p.C + k.c + v] : 0.f; });
-    if (p.dh0 && warp == 0 && chunk == 0 && live) {
+    // in walking order the last warp is the first one
+    const Vf<V> in = chain<CUT, V, W>(
+        p, k, run, sm, W - 1 - warp, lane, live,
+        [&](int v) { return p.dh_last ? p.dh_last[(int64_t)k.b * p.C + k.c + v] : 0.f; },
+        [&](Vf<V> out) {
+            if (p.dh0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = join(in[v], q[v], g[v]);
-    }
-    float prev[R][V], c[V], db[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        c[v] = join(in[v], sq[v], sc[v]);
-        db[v] = 0.f;
-        float h = start[v];
+                for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = out.at(v);
+            }
+        });
+    Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), prev[R], db = Vf<V>::all(0.f);
+    {
+        Vf<V> h = start;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (cuts >> r & 1) h = 0.f;
-            prev[r][v] = h;
-            h = advance(h, z[r][v], x[r].at(v));
+            if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
+            prev[r] = h;
+            h = advance(h, z[r], x[r].f());
         }
+        keep_packed(x);
     }
-    T *dxp = static_cast<T *>(p.dx.p) + k.b * p.dx.sb + l0 * p.dx.sl + k.c;
-    T *dfp = static_cast<T *>(p.df.p) + k.b * p.df.sb + l0 * p.df.sl + k.c;
-    T *dop = GATE ? static_cast<T *>(p.dgate.p) + k.b * p.dgate.sb + l0 * p.dgate.sl + k.c : nullptr;
+    T *dxp = static_cast<T *>(p.dx.p) + k.b * p.dx.sb + l0 * p.dx.sl + c;
+    T *dfp = static_cast<T *>(p.df.p) + k.b * p.df.sb + l0 * p.df.sl + c;
+    T *dop = GATE ? static_cast<T *>(p.dgate.p) + k.b * p.dgate.sb + l0 * p.dgate.sl + c : nullptr;
 #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-        float dx[V], df[V], dg[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float zz = z[r][v], hp = prev[r][v], dd = dy[r].at(v);
-            float s = dd;
-            if (GATE) {
-                const float o_ = o[GATE ? r : 0].at(v), sig = sg[GATE ? r : 0][v];
-                s *= o_ * sig;
+        const Vf<V> xr = x[r].f(), g = add(into(r), cc), dx = mul(z[r], g);
+        cc = carry(r, g);
+        // a = exp(u) sigmoid(-u): 1 - z would lose a small a
+        const Vf<V> a = mul(each(fma(f[r].f(), Vf<V>::all(LOG2E), bias), ex2_sat), z[r]);
+        const Vf<V> df = mul(mul(dx, a), fma(xr, Vf<V>::all(-1.f), prev[r]));
+        if (r < rows) db = add(db, df);
+        if (live && r < rows) {
+            Pack<T, V>::store(dxp + r * p.dx.sl, dx);
+            Pack<T, V>::store(dfp + r * p.df.sl, df);
+            if constexpr (GATE) {
                 // silu'(o) = sigmoid(o) (1 + o (1 - sigmoid(o)))
-                dg[v] = dd * advance(hp, zz, x[r].at(v)) * (sig * fmaf(o_, 1.f - sig, 1.f));
+                const Vf<V> one = Vf<V>::all(1.f), rest = fma(sg[r], Vf<V>::all(-1.f), one);
+                const Vf<V> slope = mul(sg[r], fma(o[r].f(), rest, one));
+                Pack<T, V>::store(dop + r * p.dgate.sl, mul(mul(dy[r].f(), advance(prev[r], z[r], xr)), slope));
             }
-            s += c[v];
-            dx[v] = zz * s;
-            // a = exp(u) sigmoid(-u): 1 - z would lose a small a
-            const float a = exp_sat(f[r].at(v) + bias[v]) * zz;
-            df[v] = dx[v] * (hp - x[r].at(v)) * a;
-            if (r < rows) db[v] += df[v];
-            c[v] = cuts >> r & 1 ? 0.f : fmaf(-zz, s, s);
-        }
-        if (r < rows) {
-            Pack<T, V>::store(dxp + r * p.dx.sl, dx, V);
-            Pack<T, V>::store(dfp + r * p.df.sl, df, V);
-            if (GATE) Pack<T, V>::store(dop + r * p.dgate.sl, dg, V);
         }
     }
     if (p.dbias_part) {
-        // s_fwd is free: every warp read it before the last barrier
-#pragma unroll
-        for (int v = 0; v < V; ++v) s_fwd[warp][lane * V + v].x = db[v];
+        s_fwd[warp][lane].h = db;  // free: every warp read it before the last barrier
         __syncthreads();
         if (warp == 0 && live) {
+            Vf<V> s = Vf<V>::all(0.f);
+            for (int w = 0; w < W; ++w) s = add(s, s_fwd[w][lane].h);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float s = 0.f;
-                for (int w = 0; w < W; ++w) s += s_fwd[w][lane * V + v].x;
-                p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = s;
-            }
+            for (int v = 0; v < V; ++v)
+                p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = s.at(v);
         }
     }
 }
@@ -525,7 +597,7 @@ __global__ void __launch_bounds__(512) scan_bias_sum(const float *part, int64_t 
 // --------------------------------------------------------------------------------- one token
 template <typename T, int V>
 __global__ void __launch_bounds__(128) scan_step(const ScanStepParams p) {
-    const int per = (p.C + V - 1) / V;
+    const int per = p.C / V;
     const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
     if (i >= (int64_t)p.N * per) return;
     const int n = (int)(i / per), c = (int)(i - (int64_t)n * per) * V;
@@ -536,22 +608,23 @@ __global__ void __launch_bounds__(128) scan_step(const ScanStepParams p) {
         held = row >= 0 && row < p.pool_rows;
     }
     Pack<T, V> x, f, o;
-    x.load(static_cast<const T *>(p.x.p) + n * p.x.sb + c, V);
-    f.load(static_cast<const T *>(p.f.p) + n * p.f.sb + c, V);
-    if (p.gate.p) o.load(static_cast<const T *>(p.gate.p) + n * p.gate.sb + c, V);
-    float y[V];
+    x.load(static_cast<const T *>(p.x.p) + n * p.x.sb + c);
+    f.load(static_cast<const T *>(p.f.p) + n * p.f.sb + c);
+    if (p.gate.p) o.load(static_cast<const T *>(p.gate.p) + n * p.gate.sb + c);
+    Vf<V> y = Vf<V>::all(0.f);
+    if (held) {
+        Vf<V> h = y, bias = y;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        y[v] = 0.f;
-        if (held) {
-            float h = p.h_in[row * p.C + c + v];
-            const float z = sigmoid_neg(f.at(v) + (p.bias ? __ldg(p.bias + c + v) : 0.f));
-            h = advance(h, z, x.at(v));
-            p.h_out[row * p.C + c + v] = h;
-            y[v] = p.gate.p ? h * (o.at(v) * sigmoid(o.at(v))) : h;
+        for (int v = 0; v < V; ++v) {
+            h.set(v, p.h_in[row * p.C + c + v]);
+            if (p.bias) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
         }
+        h = advance(h, sigmoid_neg2(fma(f.f(), Vf<V>::all(LOG2E), bias)), x.f());
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.h_out[row * p.C + c + v] = h.at(v);
+        y = p.gate.p ? mul(h, mul(o.f(), sigmoid(o.f()))) : h;
     }
-    Pack<T, V>::store(static_cast<T *>(p.y.p) + n * p.y.sb + c, y, V);
+    Pack<T, V>::store(static_cast<T *>(p.y.p) + n * p.y.sb + c, y);
 }
 
 // bf16 pairs need an even channel count and even strides on 4-byte boundaries; one channel a lane
@@ -565,10 +638,14 @@ cudaError_t forward_t(ScanParams &p, cudaStream_t st) {
     p.ctiles = (p.C + 32 * V - 1) / (32 * V);
     const int64_t tiles = (int64_t)p.chunks * p.B * p.ctiles;
     if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
-    if (p.gate.p)
-        scan_forward<T, V, 8, 16, true><<<(unsigned)tiles, 256, 0, st>>>(p);
+    if (p.gate.p && p.reset)
+        scan_forward<T, V, 8, 16, true, true><<<(unsigned)tiles, 256, 0, st>>>(p);
+    else if (p.gate.p)
+        scan_forward<T, V, 8, 16, true, false><<<(unsigned)tiles, 256, 0, st>>>(p);
+    else if (p.reset)
+        scan_forward<T, V, 8, 16, false, true><<<(unsigned)tiles, 256, 0, st>>>(p);
     else
-        scan_forward<T, V, 8, 16, false><<<(unsigned)tiles, 256, 0, st>>>(p);
+        scan_forward<T, V, 8, 16, false, false><<<(unsigned)tiles, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -577,10 +654,14 @@ cudaError_t backward_t(ScanParams &p, cudaStream_t st) {
     p.ctiles = (p.C + 32 * V - 1) / (32 * V);
     const int64_t tiles = (int64_t)p.chunks * p.B * p.ctiles;
     if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
-    if (p.gate.p)
-        scan_backward<T, V, 16, 8, true><<<(unsigned)tiles, 512, 0, st>>>(p);
+    if (p.gate.p && p.reset)
+        scan_backward<T, V, 16, 8, true, true><<<(unsigned)tiles, 512, 0, st>>>(p);
+    else if (p.gate.p)
+        scan_backward<T, V, 16, 8, true, false><<<(unsigned)tiles, 512, 0, st>>>(p);
+    else if (p.reset)
+        scan_backward<T, V, 16, 8, false, true><<<(unsigned)tiles, 512, 0, st>>>(p);
     else
-        scan_backward<T, V, 16, 8, false><<<(unsigned)tiles, 512, 0, st>>>(p);
+        scan_backward<T, V, 16, 8, false, false><<<(unsigned)tiles, 512, 0, st>>>(p);
     return cudaGetLastError();
 }
 
