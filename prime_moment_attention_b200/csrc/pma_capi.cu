@@ -866,7 +866,7 @@ int pma_gated_scan(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_t
     p.y = blc_of(y);
     p.h_last = h_last;
     if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
-    e = launch_gated_scan(p, x->dtype, st);
+    e = launch_gated_scan(p, x->dtype, di.sms, st);
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 

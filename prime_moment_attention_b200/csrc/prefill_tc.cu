@@ -967,6 +967,20 @@ bool make_map_2d_u8(CUtensorMap *m, const void *base, int64_t rows, int64_t cols
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A [B, L, C] array with element strides: boxes of 128 bytes of C x `rows` of L x 1, no swizzle.
+bool make_blc_map(CUtensorMap *m, const void *base, int64_t sb, int64_t sl, int B, int L, int C, int esize, int rows) {
+    EncodeTiled enc = get_encode();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)C, (cuuint64_t)L, (cuuint64_t)B};
+    // an axis of one element gets a harmless stride
+    const cuuint64_t str[2] = {(cuuint64_t)(L > 1 ? sl * esize : 16), (cuuint64_t)(B > 1 ? sb * esize : 16)};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / esize), (cuuint32_t)rows, 1};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return enc(m, esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+               const_cast<void *>(base), dims, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool SO, typename TO, bool PRO, bool PT>
 static cudaError_t launch_t(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
                             const PrefillParams &p0, dim3 grid, cudaStream_t st) {

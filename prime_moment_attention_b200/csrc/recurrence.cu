@@ -201,61 +201,76 @@ __device__ __forceinline__ unsigned long long get64(const unsigned long long *p)
     return v;
 }
 
-// The runs of V channels of a tile before this one, or the states leaving it as runs (-1, state).
-// `must_end`: wait for the states.
-template <int V> __device__ __forceinline__ Run<V> fetch(const ScanParams &p, int64_t at, bool must_end) {
+// The runs of V channels of K earlier tiles, at[0 .. K - 1] in the word arrays, or the states leaving
+// them as runs (-1, state); wait for the state where `must_end`, and skip a negative position.
+template <int V, int K>
+__device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K], const bool (&must_end)[K],
+                                      Run<V> (&out)[K]) {
     unsigned long long t0 = 0;
-    float n[V], h[V];
-    bool got[V];
+    float n[K][V], h[K][V];
+    bool got[K][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) got[v] = false;
-    for (uint32_t it = 1;; ++it) {
-        bool all = true;
-        uint32_t s[V];
-        unsigned long long a[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {  // every load is in flight before the first is looked at
-            s[v] = get32(p.incl + at + v);
-            a[v] = must_end ? ~0ull : get64(p.agg + at + v);
-        }
+    for (int i = 0; i < K; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (got[v]) continue;
-            if (s[v] != EMPTY) {
-                n[v] = -1.f;
-                h[v] = __uint_as_float(s[v]);
-                got[v] = true;
-            } else if (a[v] != ~0ull) {
-                n[v] = __uint_as_float((uint32_t)a[v]);
-                h[v] = __uint_as_float((uint32_t)(a[v] >> 32));
-                got[v] = true;
-            }
-            all = all && got[v];
+            got[i][v] = at[i] < 0;
+            n[i][v] = h[i][v] = 0.f;
         }
+    for (uint32_t it = 1;; ++it) {
+        bool all = true;
+        uint32_t s[K][V];
+        unsigned long long a[K][V];
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {  // every load is in flight before the first is looked at
+                s[i][v] = got[i][v] ? EMPTY : get32(p.incl + at[i] + v);
+                a[i][v] = got[i][v] || must_end[i] ? ~0ull : get64(p.agg + at[i] + v);
+            }
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (got[i][v]) continue;
+                if (s[i][v] != EMPTY) {
+                    n[i][v] = -1.f;
+                    h[i][v] = __uint_as_float(s[i][v]);
+                    got[i][v] = true;
+                } else if (a[i][v] != ~0ull) {
+                    n[i][v] = __uint_as_float((uint32_t)a[i][v]);
+                    h[i][v] = __uint_as_float((uint32_t)(a[i][v] >> 32));
+                    got[i][v] = true;
+                }
+                all = all && got[i][v];
+            }
         if (all) break;
         if ((it & 255) == 0) {
             const unsigned long long now = tc::gtimer();
             if (!t0) t0 = now;
             const bool gone = *reinterpret_cast<volatile int *>(p.counter + 1) != -1;
-            if (gone || now - t0 > p.wait_ns) {
+            if (gone || now - t0 > p.wait_ns) {  // NaN states: the launch's results are void
                 *reinterpret_cast<volatile int *>(p.counter + 1) = FAULT_CODE;
                 tc::report_fault(FAULT_CODE, p.fault);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    n[v] = -1.f;
-                    h[v] = __uint_as_float(0x7fffffffu);
-                }
+                for (int i = 0; i < K; ++i)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        n[i][v] = -1.f;
+                        h[i][v] = __uint_as_float(0x7fffffffu);
+                    }
                 break;
             }
         }
     }
-    Run<V> r = no_run<V>();
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        r.n.set(v, n[v]);
-        r.h.set(v, h[v]);
+    for (int i = 0; i < K; ++i) {
+        out[i] = no_run<V>();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            out[i].n.set(v, n[i][v]);
+            out[i].h.set(v, h[i][v]);
+        }
     }
-    return r;
 }
 
 // Test hook: a wait that nothing ends runs out, and the launch gives up before any other work.
@@ -287,18 +302,20 @@ __device__ __forceinline__ Tile tile_of(const ScanParams &p, int t, int lane) {
     return k;
 }
 
-template <int V, int W> struct Scratch {
-    Run<V> run[W][32];
+// How many tiles back a tile looks: each step of the chain of states covers as many tiles.
+constexpr int LOOK = 16;
+
+template <int V> struct Scratch {
+    Run<V> run[LOOK][32];
     Vf<V> in[32];
-    int tile;
 };
 
-// Publish this tile's run (warp 0 holds it), gather the runs of the W tiles that precede it in
+// Publish this tile's run (warp 0 holds it), gather the runs of the LOOK tiles that precede it in
 // walking order (the last of them as a state) and return the state that enters the tile; publish
-// the one that leaves, which `last` receives (warp 0).
-template <bool CUT, int V, int W, typename First, typename Last>
-__device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const Run<V> &whole, Scratch<V, W> &sm,
-                                       int warp, int lane, bool live, First first, Last last) {
+// the one that leaves, which `last` receives (warp 0).  sync(): a barrier of the W warps.
+template <bool CUT, int V, int W, typename Sync, typename First, typename Last>
+__device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const Run<V> &whole, Scratch<V> &sm,
+                                       int warp, int lane, bool live, Sync sync, First first, Last last) {
     const int64_t slot = k.word0 + (int64_t)k.chunk * p.C;
     Vf<V> in = Vf<V>::all(0.f);
     if (k.chunk == 0) {
@@ -311,11 +328,24 @@ __device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const
 #pragma unroll
             for (int v = 0; v < V; ++v) put64(p.agg + slot + v, whole.n.at(v), whole.h.at(v));
         }
-        const int reach = k.chunk < W ? k.chunk : W;
-        if (warp < reach)
-            sm.run[warp][lane] =
-                live ? fetch<V>(p, slot - (int64_t)(warp + 1) * p.C, warp == reach - 1) : no_run<V>();
-        __syncthreads();
+        const int reach = k.chunk < LOOK ? k.chunk : LOOK;
+        constexpr int K = LOOK / W;
+        if (warp < reach) {
+            int64_t at[K];
+            bool end[K];
+            Run<V> r[K];
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int d = warp + i * W;
+                at[i] = d < reach && live ? slot - (int64_t)(d + 1) * p.C : -1;
+                end[i] = d == reach - 1;
+            }
+            fetch<V, K>(p, at, end, r);
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (warp + i * W < reach) sm.run[warp + i * W][lane] = r[i];
+        }
+        sync();
         if (warp == 0) {
             for (int i = reach - 1; i >= 0; --i) in = join<true>(in, sm.run[i][lane]);
             sm.in[lane] = in;
@@ -330,7 +360,7 @@ __device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const
         if (k.chunk == p.chunks - 1) last(out);
     }
     if (k.chunk) {
-        __syncthreads();
+        sync();
         in = sm.in[lane];
     }
     return in;
@@ -360,14 +390,15 @@ __device__ __forceinline__ void load_rows(Pack<T, V> (&d)[R], const Blc &t, int 
 template <typename T, int V, int W, int R, bool GATE, bool CUT>
 __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ Scratch<V, W> sm;
+    __shared__ Scratch<V> sm;
+    __shared__ int s_tile;
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int t = blockIdx.x;
     if (p.chunks > 1) {
-        if (threadIdx.x == 0) sm.tile = atomicAdd(p.counter, 1) + 1;
+        if (threadIdx.x == 0) s_tile = atomicAdd(p.counter, 1) + 1;
         __syncthreads();
-        t = sm.tile;
+        t = s_tile;
     }
     const Tile k = tile_of<V>(p, t, lane);
     const bool live = k.c < p.C;
@@ -410,7 +441,8 @@ __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const Sca
     for (int w = 0; w < upto; ++w) run = join<CUT>(run, sm.run[w][lane]);
     __syncthreads();
     const Vf<V> in = chain<CUT, V, W>(
-        p, k, run, sm, warp, lane, live, [&](int v) { return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f; },
+        p, k, run, sm, warp, lane, live, [] { __syncthreads(); },
+        [&](int v) { return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f; },
         [&](Vf<V> out) {
             if (p.h_last) {
 #pragma unroll
@@ -438,15 +470,16 @@ __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const Sca
 template <typename T, int V, int W, int R, bool GATE, bool CUT>
 __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ Scratch<V, W> sm;
+    __shared__ Scratch<V> sm;
     __shared__ Run<V> s_fwd[W][32];
+    __shared__ int s_tile;
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int t = blockIdx.x;
     if (p.chunks > 1) {
-        if (threadIdx.x == 0) sm.tile = atomicAdd(p.counter, 1) + 1;
+        if (threadIdx.x == 0) s_tile = atomicAdd(p.counter, 1) + 1;
         __syncthreads();
-        t = sm.tile;
+        t = s_tile;
     }
     const Tile k = tile_of<V>(p, t, lane);
     const bool live = k.c < p.C;
@@ -523,7 +556,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
     __syncthreads();
     // in walking order the last warp is the first one
     const Vf<V> in = chain<CUT, V, W>(
-        p, k, run, sm, W - 1 - warp, lane, live,
+        p, k, run, sm, W - 1 - warp, lane, live, [] { __syncthreads(); },
         [&](int v) { return p.dh_last ? p.dh_last[(int64_t)k.b * p.C + k.c + v] : 0.f; },
         [&](Vf<V> out) {
             if (p.dh0) {
@@ -575,6 +608,209 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
                 p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = s.at(v);
         }
     }
+}
+
+// ------------------------------------------------------------------ forward, tiles moved by TMA
+// Rows of 128 bytes (64 bf16 or 32 float32 channels).  A CTA keeps taking tiles: one thread takes a
+// tile's number and starts its copies, eight warps work on it (16 rows each), and another thread
+// stores the outputs, which lie where x lay, and frees the stage.  Against the kernel above there
+// are no addresses to compute, x and the gate need no registers, and the next tile is on its way
+// while one waits for its state.
+struct ScanMaps {
+    CUtensorMap x, f, gate, y;
+};
+
+template <typename T, bool GATE> struct FwdCfg {
+    static constexpr int W = 8, R = 16, V = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int TILE = SCAN_ROWS * 128, STAGE = (GATE ? 3 : 2) * TILE;
+    static constexpr int STAGES = GATE ? 2 : 3, SMEM = STAGES * STAGE + 128;
+    static constexpr int THREADS = (W + 2) * 32;
+};
+
+__device__ __forceinline__ void tma_load3(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            tc::su32(dst)),
+        "l"(map), "r"(tc::su32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store3(const CUtensorMap *map, const void *src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                 "r"(tc::su32(src)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
+// The lane's word of a 128-byte row.
+template <typename T> struct Word;
+template <> struct Word<float> {
+    static __device__ __forceinline__ Vf<1> get(const uint8_t *p) { return {*reinterpret_cast<const float *>(p)}; }
+    static __device__ __forceinline__ void put(uint8_t *p, Vf<1> v) { *reinterpret_cast<float *>(p) = v.v; }
+};
+template <> struct Word<__nv_bfloat16> {
+    static __device__ __forceinline__ Vf<2> get(const uint8_t *p) {
+        const uint32_t r = *reinterpret_cast<const uint32_t *>(p);
+        return Vf<2>::of(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+    }
+    static __device__ __forceinline__ void put(uint8_t *p, Vf<2> v) {
+        *reinterpret_cast<uint32_t *>(p) = tc::pack2(v.at(0), v.at(1));
+    }
+};
+
+// Barriers of the stages, and the tiles in them (-1: no more).
+template <int STAGES> struct Ring {
+    uint64_t full[STAGES], done[STAGES], empty[STAGES];
+    int tile[STAGES];
+    tc::CtlShared ctl;
+    __device__ __forceinline__ void init(int consumers, int *fault) {
+        for (int i = 0; i < STAGES; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&done[i], consumers);
+            tc::mbar_init(&empty[i], 1);
+        }
+        tc::init_ctl(ctl, fault);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // One thread: take tiles in the counter's order and start their copies.
+    template <typename Copy>
+    __device__ __forceinline__ void produce(const ScanParams &p, int tiles, const tc::Ctl &c, Copy copy) {
+        uint32_t n = 0;
+        for (;; ++n) {
+            const int s = n % STAGES;
+            if (!tc::mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, c, FAULT_CODE + 1)) break;
+            const int t = p.chunks > 1 ? atomicAdd(p.counter, 1) + 1 : (int)(blockIdx.x + n * gridDim.x);
+            tile[s] = t < tiles ? t : -1;
+            if (t >= tiles) {  // the workers wait for every copy before they see this
+                tc::mbar_arrive(&full[s]);
+                return;
+            }
+            copy(s, t);
+        }
+        // gave up: do not leave with copies in flight
+        for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n; ++i) {
+            const unsigned long long w0 = tc::gtimer();
+            while (!tc::mbar_try(&full[i % STAGES], (i / STAGES) & 1) && tc::gtimer() - w0 < tc::WAIT_NS) {
+            }
+        }
+    }
+    // One thread: store finished tiles and free their stages.
+    template <typename Store> __device__ __forceinline__ void retire(const tc::Ctl &c, Store store) {
+        for (uint32_t n = 0;; ++n) {
+            const int s = n % STAGES;
+            if (!tc::mbar_wait(&done[s], (n / STAGES) & 1, c, FAULT_CODE + 2)) break;
+            const int t = tile[s];
+            if (t < 0) break;
+            store(s, t);
+            tc::bulk_commit();
+            tc::bulk_wait_read();
+            tc::mbar_arrive(&empty[s]);
+        }
+        tc::bulk_wait_all();
+    }
+};
+
+template <typename T, bool GATE, bool CUT>
+__global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 2)
+    scan_forward_tma(const __grid_constant__ ScanMaps maps, const ScanParams p, int tiles) {
+    using G = FwdCfg<T, GATE>;
+    constexpr int W = G::W, R = G::R, V = G::V;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u);
+    __shared__ Scratch<V> sm;
+    __shared__ Ring<G::STAGES> ring;
+    if (test_expired(p)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) ring.init(W * 32, p.fault);
+    __syncthreads();
+    const tc::Ctl ctl{&ring.ctl, nullptr};
+
+    if (warp == W) {
+        if (lane == 0)
+            ring.produce(p, tiles, ctl, [&](int s, int t) {
+                const Tile k = tile_of<V>(p, t, 0);
+                uint8_t *d = smem + s * G::STAGE;
+                tc::mbar_expect_tx(&ring.full[s], G::STAGE);
+                tma_load3(d, &maps.x, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
+                tma_load3(d + G::TILE, &maps.f, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
+                if (GATE) tma_load3(d + 2 * G::TILE, &maps.gate, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
+            });
+    } else if (warp == W + 1) {
+        if (lane == 0)
+            ring.retire(ctl, [&](int s, int t) {
+                const Tile k = tile_of<V>(p, t, 0);
+                tma_store3(&maps.y, smem + s * G::STAGE, k.c, k.chunk * SCAN_ROWS, k.b);
+            });
+    } else {
+        auto sync = [] { tc::named_bar(1, W * 32); };
+        for (uint32_t n = 0;; ++n) {
+            const int s = n % G::STAGES;
+            if (!tc::mbar_wait(&ring.full[s], (n / G::STAGES) & 1, ctl, FAULT_CODE + 3)) break;
+            const int t = ring.tile[s];
+            if (t < 0) {
+                tc::mbar_arrive(&ring.done[s]);
+                break;
+            }
+            const Tile k = tile_of<V>(p, t, lane);
+            const bool live = k.c < p.C;
+            const int l0 = k.chunk * SCAN_ROWS + warp * R, rows = p.L - l0;
+            uint8_t *xs = smem + s * G::STAGE + warp * R * 128 + lane * 4;
+            const uint8_t *fs = xs + G::TILE, *os = xs + 2 * G::TILE;
+            const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
+            Vf<V> bias = Vf<V>::all(0.f), z[R];
+            if (p.bias && live) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) bias.set(v, __ldg(p.bias + k.c + v) * LOG2E);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) z[r] = sigmoid_neg2(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias));
+            if (rows < R) {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (r >= rows) z[r] = Vf<V>::all(0.f);
+            }
+            {
+                Vf<V> q = Vf<V>::all(0.f), h = q;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (CUT && (cuts >> r & 1)) {
+                        q = Vf<V>::all(1.f);
+                        h = Vf<V>::all(0.f);
+                    }
+                    h = advance(h, z[r], Word<T>::get(xs + r * 128));
+                    q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
+                }
+                sm.run[warp][lane] = {mul(q, Vf<V>::all(-1.f)), h};
+            }
+            sync();
+            Run<V> run = no_run<V>();
+            const int upto = warp ? warp : W;
+            for (int w = 0; w < upto; ++w) run = join<CUT>(run, sm.run[w][lane]);
+            sync();
+            const Vf<V> in = chain<CUT, V, W>(
+                p, k, run, sm, warp, lane, live, sync,
+                [&](int v) { return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f; },
+                [&](Vf<V> out) {
+                    if (p.h_last) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) p.h_last[(int64_t)k.b * p.C + k.c + v] = out.at(v);
+                    }
+                });
+            Vf<V> h = warp ? join<CUT>(in, run) : in;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
+                h = advance(h, z[r], Word<T>::get(xs + r * 128));
+                Vf<V> y = h;
+                if constexpr (GATE) {
+                    const Vf<V> g = Word<T>::get(os + r * 128);
+                    y = mul(y, mul(g, sigmoid(g)));
+                }
+                Word<T>::put(xs + r * 128, y);  // rows past the end are not stored
+            }
+            tc::mbar_arrive_after_reads(&ring.done[s]);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) tc::report_fault(ring.ctl.abort_flag, p.fault);
 }
 
 // dbias[c] = sum of the tiles' partial sums, in a fixed order: 32 channels a block, 16 warps
@@ -633,6 +869,40 @@ bool pairs(const Blc &t) {
     return !t.p || (reinterpret_cast<uintptr_t>(t.p) % 4 == 0 && t.sb % 2 == 0 && t.sl % 2 == 0);
 }
 
+// TMA rows: 16-byte starts and strides, and strides that are not 0 (a broadcast axis).
+bool boxes(const Blc &t, int B, int L, int es) {
+    return !t.p || (reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && (L == 1 || (t.sl > 0 && t.sl * es % 16 == 0)) &&
+                    (B == 1 || (t.sb > 0 && t.sb * es % 16 == 0)));
+}
+
+template <typename T, bool GATE, bool CUT> cudaError_t forward_tma_v(const ScanMaps &maps, const ScanParams &p, int tiles, int grid, cudaStream_t st) {
+    using G = FwdCfg<T, GATE>;
+    cudaError_t e = set_smem_once<scan_forward_tma<T, GATE, CUT>>(G::SMEM);
+    if (e != cudaSuccess) return e;
+    scan_forward_tma<T, GATE, CUT><<<grid, G::THREADS, G::SMEM, st>>>(maps, p, tiles);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t forward_tma(ScanParams p, int sms, cudaStream_t st) {
+    constexpr int V = sizeof(T) == 2 ? 2 : 1;
+    p.ctiles = (p.C + 32 * V - 1) / (32 * V);
+    const int64_t tiles = (int64_t)p.chunks * p.B * p.ctiles;
+    if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
+    ScanMaps m;
+    if (!tc::make_blc_map(&m.x, p.x.p, p.x.sb, p.x.sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS) ||
+        !tc::make_blc_map(&m.f, p.f.p, p.f.sb, p.f.sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS) ||
+        !tc::make_blc_map(&m.y, p.y.p, p.y.sb, p.y.sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS))
+        return cudaErrorInvalidValue;
+    if (p.gate.p && !tc::make_blc_map(&m.gate, p.gate.p, p.gate.sb, p.gate.sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS))
+        return cudaErrorInvalidValue;
+    const int grid = (int)(tiles < 2 * sms ? tiles : 2 * sms);
+    if (p.gate.p)
+        return p.reset ? forward_tma_v<T, true, true>(m, p, (int)tiles, grid, st)
+                       : forward_tma_v<T, true, false>(m, p, (int)tiles, grid, st);
+    return p.reset ? forward_tma_v<T, false, true>(m, p, (int)tiles, grid, st)
+                   : forward_tma_v<T, false, false>(m, p, (int)tiles, grid, st);
+}
+
 template <typename T, int V>
 cudaError_t forward_t(ScanParams &p, cudaStream_t st) {
     p.ctiles = (p.C + 32 * V - 1) / (32 * V);
@@ -667,7 +937,11 @@ cudaError_t backward_t(ScanParams &p, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_gated_scan(ScanParams p, int dtype, cudaStream_t st) {
+cudaError_t launch_gated_scan(ScanParams p, int dtype, int sms, cudaStream_t st) {
+    const int es = dtype == PMA_F32 ? 4 : 2;
+    if (tc::tensor_maps_available() && p.C * es % 4 == 0 && boxes(p.x, p.B, p.L, es) && boxes(p.f, p.B, p.L, es) &&
+        boxes(p.gate, p.B, p.L, es) && boxes(p.y, p.B, p.L, es))
+        return dtype == PMA_F32 ? forward_tma<float>(p, sms, st) : forward_tma<__nv_bfloat16>(p, sms, st);
     if (dtype == PMA_F32) return forward_t<float, 1>(p, st);
     if (p.C % 2 == 0 && pairs(p.x) && pairs(p.f) && pairs(p.gate) && pairs(p.y))
         return forward_t<__nv_bfloat16, 2>(p, st);

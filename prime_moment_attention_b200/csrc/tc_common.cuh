@@ -361,6 +361,8 @@ __device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 12
 bool tensor_maps_available();
 bool make_tile_map(CUtensorMap *m, const Seq &s, int B, int H, int L, int Dh);
 // [rows, cols] bytes, 128-byte-swizzled boxes of 128 bytes x box_rows (base and stride multiples of 16)
+// [B, L, C] (element strides on B and L): boxes of 128 bytes of C x `rows` of L, not swizzled
+bool make_blc_map(CUtensorMap *m, const void *base, int64_t sb, int64_t sl, int B, int L, int C, int esize, int rows);
 bool make_map_2d_u8(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t stride, int box_rows);
 
 }  // namespace tc

@@ -58,6 +58,9 @@ CASES = [
     (2, 257, 128, "bf16", {"gate": False, "bias": False, "h0": False}), (4, 640, 70, "bf16", {"layout": "time"}),
     (1, 2500, 1, "bf16", {"layout": "packed"}), (2, 2176, 30, "f32", {"h0": False, "layout": "offset"}),
     (1, 20000, 64, "bf16", {"layout": "packed"}),
+    # more tiles than fit the GPU at once, with and without the strides that TMA takes
+    (2, 5000, 1024, "bf16", {"layout": "packed", "reset": True}), (1, 5000, 1024, "f32", {}),
+    (2, 3000, 1001, "bf16", {}),
 ]
 
 
