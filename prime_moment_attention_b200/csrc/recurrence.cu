@@ -183,22 +183,36 @@ __device__ __forceinline__ uint32_t word_of(float v) {
     const uint32_t u = __float_as_uint(v);
     return u == EMPTY ? 0x7fffffffu : u;
 }
-__device__ __forceinline__ void put32(uint32_t *p, float v) {
-    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(word_of(v)) : "memory");
+// V neighbouring words in one access (V divides C, so they are aligned); each word is whole.
+__device__ __forceinline__ void put(uint32_t *p, Vf<1> v) {
+    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(word_of(v.v)) : "memory");
 }
-__device__ __forceinline__ void put64(unsigned long long *p, float n, float h) {
-    const unsigned long long v = ((unsigned long long)word_of(h) << 32) | word_of(n);
-    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+__device__ __forceinline__ void put(uint32_t *p, Vf<2> v) {
+    asm volatile("st.relaxed.gpu.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(word_of(v.at(0))), "r"(word_of(v.at(1)))
+                 : "memory");
 }
-__device__ __forceinline__ uint32_t get32(const uint32_t *p) {
-    uint32_t v;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
+__device__ __forceinline__ unsigned long long word_of(float n, float h) {
+    return ((unsigned long long)word_of(h) << 32) | word_of(n);
 }
-__device__ __forceinline__ unsigned long long get64(const unsigned long long *p) {
-    unsigned long long v;
-    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-    return v;
+__device__ __forceinline__ void put(unsigned long long *p, const Run<1> &r) {
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(word_of(r.n.v, r.h.v)) : "memory");
+}
+__device__ __forceinline__ void put(unsigned long long *p, const Run<2> &r) {
+    asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};" ::"l"(p), "l"(word_of(r.n.at(0), r.h.at(0))),
+                 "l"(word_of(r.n.at(1), r.h.at(1)))
+                 : "memory");
+}
+__device__ __forceinline__ void get(const uint32_t *p, uint32_t (&v)[1]) {
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v[0]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void get(const uint32_t *p, uint32_t (&v)[2]) {
+    asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void get(const unsigned long long *p, unsigned long long (&v)[1]) {
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v[0]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void get(const unsigned long long *p, unsigned long long (&v)[2]) {
+    asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "l"(p) : "memory");
 }
 
 // The runs of V channels of K earlier tiles, at[0 .. K - 1] in the word arrays, or the states leaving
@@ -221,12 +235,19 @@ __device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K
         uint32_t s[K][V];
         unsigned long long a[K][V];
 #pragma unroll
-        for (int i = 0; i < K; ++i)
+        for (int i = 0; i < K; ++i) {  // every load is in flight before the first is looked at
+            bool have = true;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {  // every load is in flight before the first is looked at
-                s[i][v] = got[i][v] ? EMPTY : get32(p.incl + at[i] + v);
-                a[i][v] = got[i][v] || must_end[i] ? ~0ull : get64(p.agg + at[i] + v);
+            for (int v = 0; v < V; ++v) {
+                have = have && got[i][v];
+                s[i][v] = EMPTY;
+                a[i][v] = ~0ull;
             }
+            if (!have) {
+                get(p.incl + at[i], s[i]);
+                if (!must_end[i]) get(p.agg + at[i], a[i]);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < K; ++i)
 #pragma unroll
@@ -324,39 +345,36 @@ __device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const
             for (int v = 0; v < V; ++v) in.set(v, first(v));
         }
     } else {
-        if (warp == 0 && live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) put64(p.agg + slot + v, whole.n.at(v), whole.h.at(v));
-        }
+        if (warp == 0 && live) put(p.agg + slot, whole);
         const int reach = k.chunk < LOOK ? k.chunk : LOOK;
-        constexpr int K = LOOK / W;
-        if (warp < reach) {
+        constexpr int K = LOOK / W < 2 ? 1 : 2;  // tiles a warp asks for at once
+        for (int d0 = warp; d0 < LOOK; d0 += K * W) {
             int64_t at[K];
             bool end[K];
             Run<V> r[K];
 #pragma unroll
             for (int i = 0; i < K; ++i) {
-                const int d = warp + i * W;
-                at[i] = d < reach && live ? slot - (int64_t)(d + 1) * p.C : -1;
+                const int d = d0 + i * W;
+                at[i] = d < reach && live ? slot - (int64_t)(d + 1) * p.C : -1;  // else an empty run
                 end[i] = d == reach - 1;
             }
             fetch<V, K>(p, at, end, r);
 #pragma unroll
-            for (int i = 0; i < K; ++i)
-                if (warp + i * W < reach) sm.run[warp + i * W][lane] = r[i];
+            for (int i = 0; i < K; ++i) sm.run[d0 + i * W][lane] = r[i];
         }
         sync();
         if (warp == 0) {
-            for (int i = reach - 1; i >= 0; --i) in = join<true>(in, sm.run[i][lane]);
+            Run<V> r[LOOK];
+#pragma unroll
+            for (int i = 0; i < LOOK; ++i) r[i] = sm.run[i][lane];
+#pragma unroll
+            for (int i = LOOK - 1; i >= 0; --i) in = join<true>(in, r[i]);
             sm.in[lane] = in;
         }
     }
     if (warp == 0 && live) {
         const Vf<V> out = join<CUT>(in, whole);
-        if (p.chunks > 1) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) put32(p.incl + slot + v, out.at(v));
-        }
+        if (p.chunks > 1) put(p.incl + slot, out);
         if (k.chunk == p.chunks - 1) last(out);
     }
     if (k.chunk) {
@@ -611,20 +629,22 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
 }
 
 // ------------------------------------------------------------------ forward, tiles moved by TMA
-// Rows of 128 bytes (64 bf16 or 32 float32 channels).  A CTA keeps taking tiles: one thread takes a
-// tile's number and starts its copies, eight warps work on it (16 rows each), and another thread
-// stores the outputs, which lie where x lay, and frees the stage.  Against the kernel above there
-// are no addresses to compute, x and the gate need no registers, and the next tile is on its way
-// while one waits for its state.
+// Rows of 128 bytes (64 bf16 or 32 float32 channels).  One CTA an SM keeps taking tiles: a thread
+// takes a tile's number and starts its copies, one of three groups of four warps works on it (32 rows
+// a thread), and another thread stores the outputs, which lie where x lay, and frees the stage.
+// Against the kernel above there are no addresses to compute, x and the gate need no registers, and
+// a tile is on its way while three are at work.
 struct ScanMaps {
     CUtensorMap x, f, gate, y;
 };
 
 template <typename T, bool GATE> struct FwdCfg {
-    static constexpr int W = 8, R = 16, V = sizeof(T) == 2 ? 2 : 1;
-    static constexpr int TILE = SCAN_ROWS * 128, STAGE = (GATE ? 3 : 2) * TILE;
-    static constexpr int STAGES = GATE ? 2 : 3, SMEM = STAGES * STAGE + 128;
-    static constexpr int THREADS = (W + 2) * 32;
+    static constexpr int GROUPS = 3, W = 4, R = SCAN_ROWS / W, V = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int TILE = SCAN_ROWS * 128;
+    // f is done with after a tile's first pass, x and the gate after its last
+    static constexpr int FSTAGES = 3, STAGES = 4, STAGE = (GATE ? 2 : 1) * TILE;
+    static constexpr int SMEM = FSTAGES * TILE + STAGES * STAGE + 128;
+    static constexpr int THREADS = (GROUPS * W + 2) * 32;
 };
 
 __device__ __forceinline__ void tma_load3(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
@@ -656,10 +676,11 @@ template <> struct Word<__nv_bfloat16> {
     }
 };
 
-// Barriers of the stages, and the tiles in them (-1: no more).
-template <int STAGES> struct Ring {
-    uint64_t full[STAGES], done[STAGES], empty[STAGES];
-    int tile[STAGES];
+// Barriers of the stages, and the tiles in them (chunk -1: no more).  The FSTAGES stages of the first
+// pass's input are freed by the workers.
+template <int FSTAGES, int STAGES> struct Ring {
+    uint64_t full[STAGES], done[STAGES], empty[STAGES], f_empty[FSTAGES];
+    Tile tile[STAGES];
     tc::CtlShared ctl;
     __device__ __forceinline__ void init(int consumers, int *fault) {
         for (int i = 0; i < STAGES; ++i) {
@@ -667,23 +688,28 @@ template <int STAGES> struct Ring {
             tc::mbar_init(&done[i], consumers);
             tc::mbar_init(&empty[i], 1);
         }
+        for (int i = 0; i < FSTAGES; ++i) tc::mbar_init(&f_empty[i], consumers);
         tc::init_ctl(ctl, fault);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // One thread: take tiles in the counter's order and start their copies.
-    template <typename Copy>
-    __device__ __forceinline__ void produce(const ScanParams &p, int tiles, const tc::Ctl &c, Copy copy) {
+    template <int V, typename Copy>
+    __device__ __forceinline__ void produce(const ScanParams &p, int tiles, int ends, const tc::Ctl &c, Copy copy) {
         uint32_t n = 0;
         for (;; ++n) {
             const int s = n % STAGES;
             if (!tc::mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, c, FAULT_CODE + 1)) break;
             const int t = p.chunks > 1 ? atomicAdd(p.counter, 1) + 1 : (int)(blockIdx.x + n * gridDim.x);
-            tile[s] = t < tiles ? t : -1;
-            if (t >= tiles) {  // the workers wait for every copy before they see this
+            if (t >= tiles) {  // an end for every group; the workers wait for every copy before they see one
+                tile[s].chunk = -1;
                 tc::mbar_arrive(&full[s]);
-                return;
+                if (--ends == 0) return;
+                continue;
             }
-            copy(s, t);
+            const int fs = n % FSTAGES;
+            if (!tc::mbar_wait(&f_empty[fs], ((n / FSTAGES) & 1) ^ 1, c, FAULT_CODE + 1)) break;
+            tile[s] = tile_of<V>(p, t, 0);
+            copy(s, fs, tile[s]);
         }
         // gave up: do not leave with copies in flight
         for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n; ++i) {
@@ -693,15 +719,17 @@ template <int STAGES> struct Ring {
         }
     }
     // One thread: store finished tiles and free their stages.
-    template <typename Store> __device__ __forceinline__ void retire(const tc::Ctl &c, Store store) {
+    template <typename Store> __device__ __forceinline__ void retire(int ends, const tc::Ctl &c, Store store) {
         for (uint32_t n = 0;; ++n) {
             const int s = n % STAGES;
             if (!tc::mbar_wait(&done[s], (n / STAGES) & 1, c, FAULT_CODE + 2)) break;
-            const int t = tile[s];
-            if (t < 0) break;
-            store(s, t);
-            tc::bulk_commit();
-            tc::bulk_wait_read();
+            if (tile[s].chunk < 0) {
+                if (--ends == 0) break;
+            } else {
+                store(s, tile[s]);
+                tc::bulk_commit();
+                tc::bulk_wait_read();
+            }
             tc::mbar_arrive(&empty[s]);
         }
         tc::bulk_wait_all();
@@ -709,51 +737,51 @@ template <int STAGES> struct Ring {
 };
 
 template <typename T, bool GATE, bool CUT>
-__global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 2)
+__global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
     scan_forward_tma(const __grid_constant__ ScanMaps maps, const ScanParams p, int tiles) {
     using G = FwdCfg<T, GATE>;
     constexpr int W = G::W, R = G::R, V = G::V;
     extern __shared__ uint8_t raw[];
-    uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u);
-    __shared__ Scratch<V> sm;
-    __shared__ Ring<G::STAGES> ring;
+    uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u), *f_tiles = smem + G::STAGES * G::STAGE;
+    __shared__ Scratch<V> scratch[G::GROUPS];
+    __shared__ Ring<G::FSTAGES, G::STAGES> ring;
     if (test_expired(p)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, group = threadIdx.x / (W * 32), warp = (threadIdx.x >> 5) & (W - 1);
     if (threadIdx.x == 0) ring.init(W * 32, p.fault);
     __syncthreads();
     const tc::Ctl ctl{&ring.ctl, nullptr};
 
-    if (warp == W) {
-        if (lane == 0)
-            ring.produce(p, tiles, ctl, [&](int s, int t) {
-                const Tile k = tile_of<V>(p, t, 0);
+    if (group == G::GROUPS) {
+        if (warp == 0 && lane == 0)
+            ring.template produce<V>(p, tiles, G::GROUPS, ctl, [&](int s, int fs, const Tile &k) {
                 uint8_t *d = smem + s * G::STAGE;
-                tc::mbar_expect_tx(&ring.full[s], G::STAGE);
+                tc::mbar_expect_tx(&ring.full[s], G::STAGE + G::TILE);
+                tma_load3(f_tiles + fs * G::TILE, &maps.f, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
                 tma_load3(d, &maps.x, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
-                tma_load3(d + G::TILE, &maps.f, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
-                if (GATE) tma_load3(d + 2 * G::TILE, &maps.gate, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
+                if (GATE) tma_load3(d + G::TILE, &maps.gate, &ring.full[s], k.c, k.chunk * SCAN_ROWS, k.b);
             });
-    } else if (warp == W + 1) {
-        if (lane == 0)
-            ring.retire(ctl, [&](int s, int t) {
-                const Tile k = tile_of<V>(p, t, 0);
+        if (warp == 1 && lane == 0)
+            ring.retire(G::GROUPS, ctl, [&](int s, const Tile &k) {
                 tma_store3(&maps.y, smem + s * G::STAGE, k.c, k.chunk * SCAN_ROWS, k.b);
             });
     } else {
-        auto sync = [] { tc::named_bar(1, W * 32); };
-        for (uint32_t n = 0;; ++n) {
+        Scratch<V> &sm = scratch[group];
+        auto sync = [&] { tc::named_bar(1 + group, W * 32); };
+        for (uint32_t n = group;; n += G::GROUPS) {
             const int s = n % G::STAGES;
             if (!tc::mbar_wait(&ring.full[s], (n / G::STAGES) & 1, ctl, FAULT_CODE + 3)) break;
-            const int t = ring.tile[s];
-            if (t < 0) {
+            Tile k = ring.tile[s];
+            if (k.chunk < 0) {
                 tc::mbar_arrive(&ring.done[s]);
                 break;
             }
-            const Tile k = tile_of<V>(p, t, lane);
+            k.c += lane * V;
+            k.word0 += lane * V;
             const bool live = k.c < p.C;
             const int l0 = k.chunk * SCAN_ROWS + warp * R, rows = p.L - l0;
             uint8_t *xs = smem + s * G::STAGE + warp * R * 128 + lane * 4;
-            const uint8_t *fs = xs + G::TILE, *os = xs + 2 * G::TILE;
+            const uint8_t *os = xs + G::TILE;
+            const uint8_t *fs = f_tiles + (n % G::FSTAGES) * G::TILE + warp * R * 128 + lane * 4;
             const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
             Vf<V> bias = Vf<V>::all(0.f), z[R];
             if (p.bias && live) {
@@ -762,28 +790,36 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 2)
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) z[r] = sigmoid_neg2(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias));
+            tc::mbar_arrive_after_reads(&ring.f_empty[n % G::FSTAGES]);
             if (rows < R) {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     if (r >= rows) z[r] = Vf<V>::all(0.f);
             }
             {
-                Vf<V> q = Vf<V>::all(0.f), h = q;
+                Vf<V> q = Vf<V>::all(0.f), h = q, left = Vf<V>::all(1.f);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (CUT && (cuts >> r & 1)) {
                         q = Vf<V>::all(1.f);
-                        h = Vf<V>::all(0.f);
+                        h = left = Vf<V>::all(0.f);
                     }
-                    h = advance(h, z[r], Word<T>::get(xs + r * 128));
-                    q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
+                    // Q as the sum of z times the product so far: as exact, and a shorter chain
+                    const Vf<V> a = fma(z[r], Vf<V>::all(-1.f), Vf<V>::all(1.f));
+                    h = fma(a, h, mul(z[r], Word<T>::get(xs + r * 128)));
+                    q = fma(z[r], left, q);
+                    left = mul(left, a);
                 }
                 sm.run[warp][lane] = {mul(q, Vf<V>::all(-1.f)), h};
             }
             sync();
             Run<V> run = no_run<V>();
-            const int upto = warp ? warp : W;
-            for (int w = 0; w < upto; ++w) run = join<CUT>(run, sm.run[w][lane]);
+            {
+                const int upto = warp ? warp : W;
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    if (w < upto) run = join<CUT>(run, sm.run[w][lane]);
+            }
             sync();
             const Vf<V> in = chain<CUT, V, W>(
                 p, k, run, sm, warp, lane, live, sync,
@@ -895,7 +931,7 @@ template <typename T> cudaError_t forward_tma(ScanParams p, int sms, cudaStream_
         return cudaErrorInvalidValue;
     if (p.gate.p && !tc::make_blc_map(&m.gate, p.gate.p, p.gate.sb, p.gate.sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS))
         return cudaErrorInvalidValue;
-    const int grid = (int)(tiles < 2 * sms ? tiles : 2 * sms);
+    const int grid = (int)(tiles < sms ? tiles : sms);
     if (p.gate.p)
         return p.reset ? forward_tma_v<T, true, true>(m, p, (int)tiles, grid, st)
                        : forward_tma_v<T, true, false>(m, p, (int)tiles, grid, st);
