@@ -1,5 +1,5 @@
 """Build libpma.so (the C-ABI library of include/pma.h) in place with nvcc for sm_100a, and
-_pma_torch.so, the torch.ops.pma operators over that C ABI (csrc/torch_ops.cpp, g++ against the
+_pma_torch.so, the torch.ops.pma operators over that C ABI (csrc/torch_ops*.cpp, g++ against the
 installed PyTorch).
 
     python -m prime_moment_attention_b200.build        # or build() from Python
@@ -50,25 +50,31 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def build_torch_ops(verbose: bool = True) -> str:
-    """_pma_torch.so: csrc/torch_ops.cpp compiled against the installed PyTorch, linked to libpma.so
+    """_pma_torch.so: csrc/torch_ops.cpp and torch_ops_layers.cpp compiled against the installed PyTorch, linked to libpma.so
     (found next to it at run time through an $ORIGIN rpath)."""
     import torch
     import torch.utils.cpp_extension as ce
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    deps = [src, os.path.join(HERE, "..", "include", "pma.h"), LIB]
+    srcs = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_ops_layers.cpp")]
+    deps = [*srcs, os.path.join(HERE, "..", "include", "pma.h"), LIB]
     if os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(d) for d in deps):
         return TORCH_LIB
     cuda_home = ce.CUDA_HOME or "/usr/local/cuda"
     incs = [f"-I{p}" for p in ce.include_paths("cuda")] + [f"-I{os.path.join(cuda_home, 'include')}"]
     libdirs = ce.library_paths("cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *incs, src,
-           "-o", TORCH_LIB, *[f"-L{d}" for d in libdirs], f"-L{HERE}", "-lpma", "-lc10", "-lc10_cuda", "-ltorch",
-           "-ltorch_cpu", "-ltorch_cuda", "-lcudart", "-Wl,-rpath,$ORIGIN",
-           *[f"-Wl,-rpath,{d}" for d in libdirs]]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"torch ops build failed:\n{r.stderr[-4000:]}")
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"]
+    objs = [os.path.join(OUT, os.path.basename(src) + ".o") for src in srcs]
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"torch ops build failed:\n{r.stderr[-4000:]}")
+
+    with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        list(ex.map(lambda so: run(["g++", *flags, *incs, "-c", so[0], "-o", so[1]]), zip(srcs, objs)))
+    run(["g++", "-shared", *objs, "-o", TORCH_LIB, *[f"-L{d}" for d in libdirs], f"-L{HERE}", "-lpma", "-lc10",
+         "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lcudart", "-Wl,-rpath,$ORIGIN",
+         *[f"-Wl,-rpath,{d}" for d in libdirs]])
     return TORCH_LIB
 
 

@@ -12,11 +12,12 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, torch_ops
 from .ops import _DT, _require_cuda, _stream, check_faults
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
+_fn = None
 
 
 def _blocks(n: int) -> int:
@@ -111,23 +112,14 @@ def matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tenso
 def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] (bf16 or float32, quantised per row and 128 of K inside the call) times w [N, K] -> [..., N]."""
-    dev = _require_cuda(x, wq, ws)
+    global _fn
+    _require_cuda(x, wq, ws)
     check_faults("fp8.linear")
-    if x.dim() == 0:
-        raise ValueError("x must have at least one axis")
-    lead, K = x.shape[:-1], x.shape[-1]
-    x2 = _dense("x", x.reshape(-1, K) if x.dim() != 2 else x)
-    M, N = x2.shape[0], wq.shape[0]
-    wq = _rows("wq", wq, K)
-    ws = _scales("ws", ws, (_blocks(N), _blocks(K)), dev)
-    ws = ws if ws.stride(1) == 1 else ws.contiguous()
-    y = _out(out, M, N, out_dtype, dev)
-    if N and M:
-        L = _lib.load()
-        n = L.pma_fp8_linear_workspace_bytes(M, K)
-        scratch = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.check("pma_fp8_linear", L.pma_fp8_linear(
-            M, N, K, x2.data_ptr(), x2.stride(0), _DT[x2.dtype], wq.data_ptr(), wq.stride(0), ws.data_ptr(),
-            max(ws.stride(0), ws.shape[1]), y.data_ptr(), y.stride(0), _DT[y.dtype], scratch.data_ptr(), n,
-            _stream(dev)))
-    return y if x.dim() == 2 else y.view(*lead, N)
+    if out is None:
+        if _fn is None:
+            torch_ops.load()
+            _fn = torch.ops.pma.fp8_linear.default
+        return _fn(x.detach(), wq, ws, out_dtype)
+    if x.dim() != 2:
+        raise ValueError("x must be a matrix when out is given")
+    return matmul(*quantize(x), wq, ws, out=out)

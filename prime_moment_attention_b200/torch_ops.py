@@ -9,6 +9,9 @@ opaque node whose output shapes come from the fake implementations registered be
     torch.ops.pma.decode_step(q, k, v, decay, state, eps=1.0) -> (y, [new state])
     torch.ops.pma.decode_step_(q, k, v, decay, state, eps=1.0) -> y        (state updated in place)
 
+    torch.ops.pma.gated_scan, gated_scan_step, gated_scan_step_, sample, fp8_linear: the calls behind
+    the recurrence, sampling and fp8 modules, which document their arguments
+
 `decay` is a float32 CUDA tensor of H (or B*H) decays; states are the reference tuple
 (S0, S1, S2, K0, K1, K2) in float32.  Loading fails loudly when _pma_torch.so is missing.
 """
@@ -50,6 +53,26 @@ def load() -> None:
     @torch.library.register_fake("pma::decode_step_")
     def _decode_inplace_fake(q, k, v, decay, state, eps=1.0):
         return q.new_empty(q.shape)
+
+    @torch.library.register_fake("pma::gated_scan")
+    def _gated_scan_fake(x, f, bias=None, gate=None, h0=None, reset=None):
+        return x.new_empty(x.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)
+
+    @torch.library.register_fake("pma::gated_scan_step")
+    def _gated_scan_step_fake(x, f, h, bias=None, gate=None):
+        return x.new_empty(x.shape), h.new_empty(h.shape)
+
+    @torch.library.register_fake("pma::gated_scan_step_")
+    def _gated_scan_step_inplace_fake(x, f, h, bias=None, gate=None, rows=None):
+        return x.new_empty(x.shape)
+
+    @torch.library.register_fake("pma::sample")
+    def _sample_fake(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, t=1.0, k=0, p=1.0, m=0.0):
+        return u.new_empty(u.shape, dtype=torch.int64), u.new_empty(u.shape)
+
+    @torch.library.register_fake("pma::fp8_linear")
+    def _fp8_linear_fake(x, wq, ws, out_dtype):
+        return x.new_empty((*x.shape[:-1], wq.shape[0]), dtype=out_dtype)
 
     _loaded = True
 
