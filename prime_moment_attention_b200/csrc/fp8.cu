@@ -14,6 +14,8 @@
 // a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "fp8.cuh"
 
 #include "tc_common.cuh"
@@ -34,8 +36,12 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
+//
+// The division is only made where it can matter: x (448 / amax) is within 2 ulp of the quotient, which
+// rounds to the same e4m3 value unless it lies that close to the middle of two (or is below 2^-6,
+// where e4m3's spacing is fixed).
 struct Quant {
-    float amax, pre;
+    float amax, pre, fast;
     // amax of 0 (or below 2^-100) counts as 2^-100; a block of huge values is divided by 2^20 first,
     // so that 448 x stays finite
     __device__ __forceinline__ explicit Quant(float a) : amax(fmaxf(a, 7.888609052210118e-31f)), pre(448.0f) {
@@ -43,9 +49,12 @@ struct Quant {
             pre *= 9.5367431640625e-07f;
             amax *= 9.5367431640625e-07f;
         }
+        fast = __fmul_rn(pre, __frcp_rn(amax));
     }
-    __device__ __forceinline__ float operator()(float x) const { return __fdiv_rn(x * pre, amax); }
-    static __device__ __forceinline__ float scale(float a) { return fmaxf(a, 7.888609052210118e-31f) / 448.0f; }
+    __device__ __forceinline__ float exact(float x) const { return __fdiv_rn(x * pre, amax); }
+    static __device__ __forceinline__ float scale(float a) {
+        return a == a ? fmaxf(a, 7.888609052210118e-31f) / 448.0f : a;
+    }
 };
 
 // NaN is kept: a block that holds one gets a NaN scale
@@ -56,17 +65,50 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // Eight consecutive elements of a row, zero past K.
-template <typename T>
-__device__ __forceinline__ void load8(const T *row, int k, int K, bool vec, float (&x)[8]) {
-    if (vec && k + 8 <= K) {
-        const float4 a = load4(row + k), b = load4(row + k + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float *row, int k, int K, bool vec) {
+        if (vec && k + 8 <= K) {
+            const float4 a = load4(row + k), b = load4(row + k + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = k + i < K ? Elem<T>::to_f(row[k + i]) : 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : 0.f;
+        }
     }
-}
+    __device__ __forceinline__ float at(int i) const { return v[i]; }
+    __device__ __forceinline__ float amax() const {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
+        return a;
+    }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint32_t v[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16 *row, int k, int K, bool vec) {
+        if (vec && k + 8 <= K) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + k));
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        } else {
+            const unsigned short *r = reinterpret_cast<const unsigned short *>(row);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = (k + 2 * i < K ? r[k + 2 * i] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)r[k + 2 * i + 1] : 0u) << 16;
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        return __uint_as_float(i & 1 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+    }
+    __device__ __forceinline__ float amax() const {  // two at a time, exact in bf16
+        uint32_t a = v[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(v[i] & 0x7fff7fffu));
+        return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+    }
+};
 __device__ __forceinline__ void store8(uint8_t *row, int k, int K, uint2 v) {
     if (k + 8 <= K) {
         *reinterpret_cast<uint2 *>(row + k) = v;  // rows start on 16 bytes, k is a multiple of 8
@@ -74,35 +116,52 @@ __device__ __forceinline__ void store8(uint8_t *row, int k, int K, uint2 v) {
         for (int i = 0; i < 8 && k + i < K; ++i) row[k + i] = (uint8_t)((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
     }
 }
-__device__ __forceinline__ float amax8(const float (&x)[8]) {
-    float a = 0.f;
+template <typename E> __device__ __forceinline__ uint2 quant8(const E &x, const Quant &q) {
+    float v[8], small = INFINITY;
+    uint32_t off = 0xffffffffu;  // distance of the 20 bits below e4m3's significand from their middle, + 4
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(x[i]));
-    return a;
-}
-__device__ __forceinline__ uint2 quant8(const float (&x)[8], const Quant &q) {
-    return make_uint2(e4m3x2(q(x[0]), q(x[1])) | e4m3x2(q(x[2]), q(x[3])) << 16,
-                      e4m3x2(q(x[4]), q(x[5])) | e4m3x2(q(x[6]), q(x[7])) << 16);
+    for (int i = 0; i < 8; ++i) {
+        v[i] = __fmul_rn(x.at(i), q.fast);
+        off = min(off, __float_as_uint(v[i]) - 0x7fffcu & 0xfffffu);
+        small = fminf(small, fabsf(v[i]));
+    }
+    if (off <= 8u || !(small >= 0.015625f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = q.exact(x.at(i));
+    }
+    return make_uint2(e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16, e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16);
 }
 
-// 16 lanes a block of 128; the grid covers rows x blocks.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows(const T *__restrict__ x, int64_t xs, int M, int K, int blocks,
-                                                    bool vec, uint8_t *__restrict__ q, int64_t qs,
+// Lets the product that follows in the stream start: it waits for this grid before it reads q.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 16 lanes a block of 128; a lane group takes GROUPS neighbouring blocks of a row (its loads in flight
+// together).
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(256) quantize_rows(const T *__restrict__ x, int64_t xs, uint32_t items, int K,
+                                                    uint32_t per_row, bool vec, uint8_t *__restrict__ q, int64_t qs,
                                                     float *__restrict__ scale, int64_t si, int64_t sj) {
-    const int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
-    const int l = threadIdx.x & 15;
-    const bool on = g < (int64_t)M * blocks;
-    const int m = on ? (int)(g / blocks) : 0, j = on ? (int)(g - (int64_t)m * blocks) : 0;
-    const int k = on ? j * FP8_BLOCK + l * 8 : K;
-    float v[8];
-    load8(x + (int64_t)m * xs, k, K, vec, v);
-    float a = amax8(v);
+    launch_dependents();
+    const uint32_t g = blockIdx.x * 16u + (threadIdx.x >> 4);
+    const bool on = g < items;
+    const uint32_t m = on ? g / per_row : 0, j0 = on ? (g - m * per_row) * GROUPS : 0;
+    const int k0 = (int)j0 * FP8_BLOCK + (threadIdx.x & 15) * 8;
+    x += (int64_t)m * xs;
+    q += (int64_t)m * qs;
+    Eight<T> v[GROUPS];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (!on) return;
-    store8(q + (int64_t)m * qs, k, K, quant8(v, Quant(a)));
-    if (l == 0) scale[m * si + j * sj] = a == a ? Quant::scale(a) : a;
+    for (int i = 0; i < GROUPS; ++i) v[i].load(x, on ? k0 + i * FP8_BLOCK : K, K, vec);
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+        float a = v[i].amax();
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const int k = k0 + i * FP8_BLOCK;
+        if (on && (int)(j0 + i) * FP8_BLOCK < K) {
+            store8(q, k, K, quant8(v[i], Quant(a)));
+            if ((threadIdx.x & 15) == 0) scale[(int64_t)m * si + (int64_t)(j0 + i) * sj] = Quant::scale(a);
+        }
+    }
 }
 
 // One CTA a 128 x 128 block of weights: 256 threads, 16 lanes a row.
@@ -117,9 +176,9 @@ __global__ void __launch_bounds__(256) quantize_blocks(const T *__restrict__ w, 
     for (int r = r0; r < FP8_BLOCK; r += 16) {
         const int n = nb * FP8_BLOCK + r;
         if (n >= N) break;
-        float v[8];
-        load8(w + (int64_t)n * ws, k, K, vec, v);
-        a = max_nan(a, amax8(v));
+        Eight<T> v;
+        v.load(w + (int64_t)n * ws, k, K, vec);
+        a = max_nan(a, v.amax());
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -132,11 +191,11 @@ __global__ void __launch_bounds__(256) quantize_blocks(const T *__restrict__ w, 
     for (int r = r0; r < FP8_BLOCK; r += 16) {
         const int n = nb * FP8_BLOCK + r;
         if (n >= N) break;
-        float v[8];
-        load8(w + (int64_t)n * ws, k, K, vec, v);  // from L1 or L2: the block was just read
+        Eight<T> v;
+        v.load(w + (int64_t)n * ws, k, K, vec);  // from L1 or L2: the block was just read
         store8(q + (int64_t)n * qs, k, K, quant8(v, qu));
     }
-    if (threadIdx.x == 0) scale[(int64_t)nb * blocks + j] = a == a ? Quant::scale(a) : a;
+    if (threadIdx.x == 0) scale[(int64_t)nb * blocks + j] = Quant::scale(a);
 }
 
 // ------------------------------------------------------------------------------------- product
@@ -158,6 +217,17 @@ __device__ __forceinline__ void tma_load2(void *dst, const CUtensorMap *map, uin
         "l"(map), "r"(su32(bar)), "r"(c0), "r"(c1)
         : "memory");
 }
+__device__ __forceinline__ void tmem_issue(uint32_t t, uint32_t (&r)[16]) { tmem_ld16_issue(t, r); }
+__device__ __forceinline__ void tmem_issue(uint32_t t, uint32_t (&r)[32]) { tmem_ld32_issue(t, r); }
+// The kernel before this one in the stream is complete and its writes are visible.
+__device__ __forceinline__ void wait_for_x() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void copy4(float *dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(su32(dst)), "l"(src) : "memory");
+}
+// arrives on `bar` when this thread's copies so far have landed
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
 // two float32 products and sums at once
 __device__ __forceinline__ void fma2(unsigned long long &acc, uint32_t lo, uint32_t hi, unsigned long long s) {
     unsigned long long d;
@@ -173,11 +243,36 @@ __device__ __forceinline__ float half_of(unsigned long long v, int i) {
     return __uint_as_float((uint32_t)(i ? v >> 32 : v));
 }
 
+constexpr int OUT_PITCH = 80;  // bytes between rows of 64: 16-byte accesses of 8 lanes hit all banks
+
+// 32 rows of 64 bytes in shared memory to `rows` rows of `cols` elements at y (row stride ys).
+template <typename T>
+__device__ __forceinline__ void store_rows(const uint8_t *s, T *y, int64_t ys, int rows, int cols, int lane) {
+    constexpr int PER = 64 / sizeof(T), E16 = 16 / sizeof(T);
+    if (rows <= 0 || cols <= 0) return;
+    if (cols == PER && reinterpret_cast<uintptr_t>(y) % 16 == 0 && ys % E16 == 0) {
+        const int q = lane & 3;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+            const int r = r0 + (lane >> 2);
+            if (r < rows)
+                *reinterpret_cast<uint4 *>(y + r * ys + q * E16) = *reinterpret_cast<const uint4 *>(s + r * OUT_PITCH + q * 16);
+        }
+    } else {
+        constexpr int RPI = 32 / PER;  // rows a store covers: 1 (bf16) or 2 (float32)
+        const int c = lane % PER;
+        if (c < cols)
+            for (int r = lane / PER; r < rows; r += RPI)
+                y[r * ys + c] = *reinterpret_cast<const T *>(s + r * OUT_PITCH + c * sizeof(T));
+    }
+}
+
 // BN: rows of the second operand in a tile; FEW: w is the 128-row operand.
 template <int BN, bool FEW> struct Cfg {
     static constexpr int EPI = BN == 256 ? 8 : 4;      // epilogue warps: 128 lanes x COLS columns each group of 4
     static constexpr int COLS = BN == 256 ? 128 : BN;  // accumulator columns of a thread
-    static constexpr int WARPS = BN == 256 ? 12 : 6;
+    static constexpr int WARPS = BN == 256 ? 12 : 7;   // and TMA, products, scales
+    static constexpr int SLOT = (BN > 128 ? BN : 128) + 4;  // floats: one K block's scales
     static constexpr int THREADS = WARPS * 32;
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 4;
@@ -186,8 +281,10 @@ template <int BN, bool FEW> struct Cfg {
     static constexpr int SMEM = STAGES * STAGE + 1024;
 };
 
+constexpr int SLOTS = 8;  // K blocks whose scales are on their way or in use
+
 template <int STAGES> struct Bars {
-    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], never;
+    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], sc_full[SLOTS], sc_empty[SLOTS], never;
     uint32_t tmem;
     CtlShared ctl;
 };
@@ -199,6 +296,8 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
     using G = Cfg<BN, FEW>;
     extern __shared__ uint8_t raw[];
     __shared__ Bars<G::STAGES> sm;
+    __shared__ __align__(16) float scales[SLOTS][G::SLOT];
+    __shared__ __align__(16) uint8_t out_s[FEW ? 1 : G::EPI][FEW ? 16 : 32 * OUT_PITCH];
     uint8_t *tiles = smem_align1024(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Ctl ctl{&sm.ctl, nullptr};
@@ -211,6 +310,10 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.acc_full[i], 1);
             mbar_init(&sm.acc_empty[i], G::EPI);
+        }
+        for (int i = 0; i < SLOTS; ++i) {
+            mbar_init(&sm.sc_full[i], 32);
+            mbar_init(&sm.sc_empty[i], G::EPI);
         }
         mbar_init(&sm.never, 1);
         init_ctl(sm.ctl, p.fault);
@@ -252,20 +355,45 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         ia = band * 16 + r - ib * h;
     };
 
+    if (warp >= G::EPI) {
+    // registers to the accumulators: 256 x 224 + 128 x 56 = 384 x 168
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == G::EPI) {
         // ------------------------------------------------------------------ TMA
         if (lane == 0) {
+            // Until the kernel before has written x, load weights only.
+            auto load_w = [&](int s, int j, int ia, int ib) {
+                if (FEW)
+                    tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
+                else
+                    tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
+            };
+            auto load_x = [&](int s, int j, int ia, int ib) {
+                if (FEW)
+                    tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
+                else
+                    tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
+            };
             uint32_t n = 0;
             bool ok = true;
+            const int early = first < all ? min(G::STAGES, j1 - j0) : 0;
+            int ia, ib;
+            tile_at(first, ia, ib);
+            for (int i = 0; i < early; ++i) {
+                mbar_expect_tx(&sm.full[i], G::STAGE);
+                load_w(i, j0 + i, ia, ib);
+            }
+            wait_for_x();
             for (int t = first; ok && t < all; t += step) {
-                int ia, ib;
                 tile_at(t, ia, ib);
                 for (int j = j0; j < j1; ++j, ++n) {
                     const int s = n % G::STAGES;
-                    if (!(ok = mbar_wait(&sm.empty[s], ((n / G::STAGES) & 1) ^ 1, ctl, 131))) break;
-                    mbar_expect_tx(&sm.full[s], G::STAGE);
-                    tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
-                    tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
+                    if (n >= (uint32_t)early) {
+                        if (!(ok = mbar_wait(&sm.empty[s], ((n / G::STAGES) & 1) ^ 1, ctl, 131))) break;
+                        mbar_expect_tx(&sm.full[s], G::STAGE);
+                        load_w(s, j, ia, ib);
+                    }
+                    load_x(s, j, ia, ib);
                 }
             }
             // never leave with copies in flight
@@ -304,8 +432,36 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
                 }
             }
         }
-    } else if (warp < G::EPI) {
-        // ------------------------------------------------------------------ scales, sums, output
+    } else if (warp == G::EPI + 2) {
+        // ------------------------------------------------------------------ scales
+        // of a K block: x's rows of the tile, then w's blocks
+        constexpr int ROWS = FEW ? BN : 128;
+        wait_for_x();
+        uint32_t n = 0;
+        bool ok = true;
+        for (int t = first; ok && t < all; t += step) {
+            int ia, ib;
+            tile_at(t, ia, ib);
+            const int m0 = FEW ? ib * BN : ia * 128, n0 = FEW ? ia : ib * (BN / 128);
+            for (int j = j0; j < j1; ++j, ++n) {
+                const int s = n % SLOTS;
+                if (!(ok = mbar_wait(&sm.sc_empty[s], ((n / SLOTS) & 1) ^ 1, ctl, 135))) break;
+#pragma unroll
+                for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+                    const int r = i * 32 + lane;
+                    if (r < ROWS) copy4(&scales[s][r], p.x.scale + (int64_t)min(m0 + r, p.M - 1) * p.x.si + j * p.x.sj);
+                }
+                if (lane < (FEW ? 1 : BN / 128))
+                    copy4(&scales[s][G::SLOT - 4 + lane],
+                          p.w.scale + (int64_t)min(n0 + lane, (p.N - 1) / 128) * p.w.si + j * p.w.sj);
+                copies_arrive(&sm.sc_full[s]);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    } else {
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ------------------------------------------------------------------ sums, output
         const int row = (warp & 3) * 32 + lane, col0 = (warp >> 2) * G::COLS;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
         uint32_t n = 0;
@@ -314,52 +470,45 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
             int ia, ib;
             tile_at(t, ia, ib);
             const int ra = ia * 128 + row, cb = ib * BN + col0;  // this thread's row and first column
-            // its scales: of the row (x) or of the tile (w), and of the columns
-            const float *sa = FEW ? p.w.scale + (int64_t)ia * p.w.si
-                                  : p.x.scale + (int64_t)min(ra, p.M - 1) * p.x.si;
-            const int64_t saj = FEW ? p.w.sj : p.x.sj;
-            const float *sb = FEW ? p.x.scale : p.w.scale + (int64_t)min(cb / 128, (p.N - 1) / 128) * p.w.si;
-            const int64_t sbj = FEW ? p.x.sj : p.w.sj;
             unsigned long long acc[G::COLS / 2];
 #pragma unroll
             for (int i = 0; i < G::COLS / 2; ++i) acc[i] = 0ull;
-            float s0 = j0 < j1 ? __ldg(sa + j0 * saj) * (FEW ? 1.f : __ldg(sb + j0 * sbj)) : 0.f;
             for (int j = j0; j < j1; ++j, ++n) {
-                const int a = n & 1;
-                const float s = s0;
-                if (j + 1 < j1) s0 = __ldg(sa + (j + 1) * saj) * (FEW ? 1.f : __ldg(sb + (j + 1) * sbj));
+                const int a = n & 1, sl = n % SLOTS;
+                if (!(ok = mbar_wait(&sm.sc_full[sl], (n / SLOTS) & 1, ctl, 136))) break;
+                const float *sx = scales[sl];
+                const float s = FEW ? sx[G::SLOT - 4] : sx[row] * sx[G::SLOT - 4 + col0 / 128];
                 if (!(ok = mbar_wait(&sm.acc_full[a], (n >> 1) & 1, ctl, 134))) break;
                 tc_fence_after();
-                constexpr int CH = G::COLS < 32 ? 16 : 32;
+                // CH columns are read while the CH before them are scaled: a read's latency, not its
+                // bandwidth, is what it costs
+                constexpr int CH = G::COLS == 128 ? 32 : 16;
+                uint32_t d[2][CH];
+                tmem_issue(mine + a * BN, d[0]);
 #pragma unroll
                 for (int c = 0; c < G::COLS; c += CH) {
-                    uint32_t d[CH];
-                    if constexpr (CH == 32)
-                        tmem_ld32_issue(mine + a * BN + c, d);
-                    else
-                        tmem_ld16_issue(mine + a * BN + c, d);
-                    tmem_wait_ld_regs(d);
-                    if (c + CH == G::COLS) {  // all columns are in registers
+                    uint32_t(&v)[CH] = d[(c / CH) & 1];
+                    tmem_wait_ld_regs(v);
+                    if (c + CH < G::COLS) {
+                        tmem_issue(mine + a * BN + c + CH, d[(c / CH & 1) ^ 1]);
+                    } else {  // all columns are in registers
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sm.acc_empty[a]);
                     }
-                    if (FEW) {
+                    const unsigned long long sp = pair(s);
 #pragma unroll
-                        for (int i = 0; i < CH; i += 2) {
-                            const int m0 = cb + c + i, m1 = m0 + 1;
-                            const float x0 = __ldg(sb + (int64_t)min(m0, p.M - 1) * p.x.si + j * sbj);
-                            const float x1 = __ldg(sb + (int64_t)min(m1, p.M - 1) * p.x.si + j * sbj);
-                            unsigned long long sc;
-                            asm("mov.b64 %0, {%1, %2};" : "=l"(sc) : "f"(s * x0), "f"(s * x1));
-                            fma2(acc[(c + i) / 2], d[i], d[i + 1], sc);
+                    for (int i = 0; i < CH; i += 2) {
+                        unsigned long long x2 = sp;
+                        if (FEW) {
+                            x2 = *reinterpret_cast<const unsigned long long *>(sx + c + i);
+                            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x2) : "l"(sp));
                         }
-                    } else {
-                        const unsigned long long sc = pair(s);
-#pragma unroll
-                        for (int i = 0; i < CH; i += 2) fma2(acc[(c + i) / 2], d[i], d[i + 1], sc);
+                        fma2(acc[(c + i) / 2], v[i], v[i + 1], x2);
                     }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.sc_empty[sl]);
             }
             if (!ok) break;
             if (FEW && splits > 1) {
@@ -379,36 +528,40 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
                                 static_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(v);
                         }
                 }
-            } else if (ra < p.M) {
+            } else if (!FEW) {
+                // rows leave through shared memory, 64 bytes of each at a time, so that a store covers
+                // whole sectors whatever y's row stride is
+                uint8_t *mine_s = out_s[warp];
+                const int rows = min(32, p.M - (ra - lane));
                 if (p.y_f32) {
-                    float *o = static_cast<float *>(p.y) + (int64_t)ra * p.ys + cb;
-                    if (cb + G::COLS <= p.N && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
-                        for (int i = 0; i < G::COLS; i += 4)
-                            *reinterpret_cast<float4 *>(o + i) =
-                                make_float4(half_of(acc[i / 2], 0), half_of(acc[i / 2], 1), half_of(acc[i / 2 + 1], 0),
-                                            half_of(acc[i / 2 + 1], 1));
-                    } else {
+                    for (int c = 0; c < G::COLS; c += 16) {
 #pragma unroll
-                        for (int i = 0; i < G::COLS; ++i)
-                            if (cb + i < p.N) o[i] = half_of(acc[i / 2], i & 1);
+                        for (int i = 0; i < 16; i += 4) {
+                            const unsigned long long lo = acc[(c + i) / 2], hi = acc[(c + i) / 2 + 1];
+                            *reinterpret_cast<ulonglong2 *>(mine_s + lane * OUT_PITCH + i * 4) = make_ulonglong2(lo, hi);
+                        }
+                        __syncwarp();
+                        store_rows<float>(mine_s, static_cast<float *>(p.y) + (int64_t)(ra - lane) * p.ys + cb + c, p.ys, rows,
+                                          min(16, p.N - cb - c), lane);
+                        __syncwarp();
                     }
                 } else {
-                    __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.y) + (int64_t)ra * p.ys + cb;
-                    if (cb + G::COLS <= p.N && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
-                        for (int i = 0; i < G::COLS; i += 8) {
+                    for (int c = 0; c < G::COLS; c += 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
                             uint4 v;
                             uint32_t *e = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
                             for (int h = 0; h < 4; ++h)
-                                e[h] = pack2(half_of(acc[i / 2 + h], 0), half_of(acc[i / 2 + h], 1));
-                            *reinterpret_cast<uint4 *>(o + i) = v;
+                                e[h] = pack2(half_of(acc[(c + i) / 2 + h], 0), half_of(acc[(c + i) / 2 + h], 1));
+                            *reinterpret_cast<uint4 *>(mine_s + lane * OUT_PITCH + i * 2) = v;
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < G::COLS; ++i)
-                            if (cb + i < p.N) o[i] = __float2bfloat16_rn(half_of(acc[i / 2], i & 1));
+                        __syncwarp();
+                        store_rows<__nv_bfloat16>(mine_s, static_cast<__nv_bfloat16 *>(p.y) + (int64_t)(ra - lane) * p.ys + cb + c,
+                                                  p.ys, rows, min(32, p.N - cb - c), lane);
+                        __syncwarp();
                     }
                 }
             }
@@ -444,7 +597,7 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
     if (tid == 0) report_fault(sm.ctl.abort_flag, p.fault);
 }
 
-template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, cudaStream_t st) {
+template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, bool after_quantize, cudaStream_t st) {
     using G = Cfg<BN, FEW>;
     const Fp8Rows &a = FEW ? p.w : p.x, &b = FEW ? p.x : p.w;
     const int ra = FEW ? p.N : p.M, rb = FEW ? p.M : p.N;
@@ -465,12 +618,14 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, cudaStre
     cfg.blockDim = dim3(G::THREADS);
     cfg.dynamicSmemBytes = G::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)splits;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = after_quantize ? 2 : 1;  // only after our own kernel, which says when it may start
     e = cudaLaunchKernelEx(&cfg, fp8_matmul_kernel<BN, FEW>, ta, tb, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -480,16 +635,25 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, cudaStre
 cudaError_t launch_fp8_quantize(const void *x, int64_t xs, int dtype, int M, int K, uint8_t *q, int64_t qs,
                                 float *scale, int64_t si, int64_t sj, cudaStream_t st) {
     const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-    const int64_t grid = ((int64_t)M * blocks * 16 + 255) / 256;
-    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    // two blocks a lane group once that still fills the GPU
+    const int groups = (int64_t)M * blocks >= 148 * 128 * 4 && blocks > 1 ? 2 : 1;
+    const uint32_t per_row = (uint32_t)((blocks + groups - 1) / groups);
+    const int64_t items = (int64_t)M * per_row;
+    if (items > 0xfffffff0ll) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)((items + 15) / 16);
     const int step = dtype == PMA_F32 ? 4 : 8;  // 16-byte rows for the vector loads (load4 of bf16 is 8 bytes)
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && xs % step == 0;
+    auto run = [&](auto *p) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        if (groups == 2)
+            quantize_rows<T, 2><<<grid, 256, 0, st>>>(p, xs, (uint32_t)items, K, per_row, vec, q, qs, scale, si, sj);
+        else
+            quantize_rows<T, 1><<<grid, 256, 0, st>>>(p, xs, (uint32_t)items, K, per_row, vec, q, qs, scale, si, sj);
+    };
     if (dtype == PMA_F32)
-        quantize_rows<float><<<(unsigned)grid, 256, 0, st>>>(static_cast<const float *>(x), xs, M, K, blocks, vec, q, qs,
-                                                            scale, si, sj);
+        run(static_cast<const float *>(x));
     else
-        quantize_rows<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(x), xs, M, K,
-                                                                     blocks, vec, q, qs, scale, si, sj);
+        run(static_cast<const __nv_bfloat16 *>(x));
     return cudaGetLastError();
 }
 
@@ -509,15 +673,15 @@ cudaError_t launch_fp8_quantize_weight(const void *w, int64_t ws, int dtype, int
     return cudaGetLastError();
 }
 
-cudaError_t launch_fp8_matmul(Fp8Params p, int sms, cudaStream_t st) {
+cudaError_t launch_fp8_matmul(Fp8Params p, int sms, bool after_quantize, cudaStream_t st) {
     p.blocks = (p.K + FP8_BLOCK - 1) / FP8_BLOCK;
-    if (p.M <= 16) return matmul_t<16, true>(p, sms, st);
-    if (p.M <= 32) return matmul_t<32, true>(p, sms, st);
-    if (p.M <= 64) return matmul_t<64, true>(p, sms, st);
+    if (p.M <= 16) return matmul_t<16, true>(p, sms, after_quantize, st);
+    if (p.M <= 32) return matmul_t<32, true>(p, sms, after_quantize, st);
+    if (p.M <= 64) return matmul_t<64, true>(p, sms, after_quantize, st);
     // 256 columns halve the re-reads of x, once that leaves a tile for every SM
     const int64_t wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256);
-    if (wide >= sms) return matmul_t<256, false>(p, sms, st);
-    return matmul_t<128, false>(p, sms, st);
+    if (wide >= sms) return matmul_t<256, false>(p, sms, after_quantize, st);
+    return matmul_t<128, false>(p, sms, after_quantize, st);
 }
 
 }  // namespace pma

@@ -30,6 +30,7 @@ cudaError_t launch_fp8_quantize(const void *x, int64_t xs, int dtype, int M, int
                                 float *scale, int64_t si, int64_t sj, cudaStream_t st);
 cudaError_t launch_fp8_quantize_weight(const void *w, int64_t ws, int dtype, int N, int K, uint8_t *q, int64_t qs,
                                        float *scale, cudaStream_t st);
-cudaError_t launch_fp8_matmul(Fp8Params p, int sms, cudaStream_t st);
+// after_quantize: the last kernel in the stream is launch_fp8_quantize's, with which it may overlap.
+cudaError_t launch_fp8_matmul(Fp8Params p, int sms, bool after_quantize, cudaStream_t st);
 
 }  // namespace pma

@@ -199,7 +199,7 @@ struct Fp8Ws {
 };
 
 int fp8_product(int M, int N, int K, const Fp8Rows &x, const Fp8Rows &w, void *y, int64_t ys, int ydt, int sms,
-                cudaStream_t st) {
+                bool after_quantize, cudaStream_t st) {
     Fp8Params p{};
     p.M = M;
     p.N = N;
@@ -211,7 +211,7 @@ int fp8_product(int M, int N, int K, const Fp8Rows &x, const Fp8Rows &w, void *y
     p.y_f32 = ydt == PMA_F32;
     p.fault = g_fault_word.load(std::memory_order_acquire);
     p.test_wait_ns = g_test_wait_ns.load(std::memory_order_acquire);
-    const cudaError_t e = launch_fp8_matmul(p, sms, st);
+    const cudaError_t e = launch_fp8_matmul(p, sms, after_quantize, st);
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 
@@ -996,10 +996,10 @@ int pma_fp8_quantize_weight(int N, int K, const void *w, int64_t w_stride, int d
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 
-int pma_fp8_matmul(int M, int N, int K, const void *xq, int64_t xq_stride, const float *x_scale,
-                   int64_t x_scale_stride_m, int64_t x_scale_stride_k, const void *wq, int64_t wq_stride,
-                   const float *w_scale, int64_t w_scale_stride, void *y, int64_t y_stride, int y_dtype,
-                   pma_stream_t stream) {
+static int fp8_matmul_impl(int M, int N, int K, const void *xq, int64_t xq_stride, const float *x_scale,
+                           int64_t x_scale_stride_m, int64_t x_scale_stride_k, const void *wq, int64_t wq_stride,
+                           const float *w_scale, int64_t w_scale_stride, void *y, int64_t y_stride, int y_dtype,
+                           bool after_quantize, pma_stream_t stream) {
     if (M < 0 || N <= 0 || K <= 0 || x_scale_stride_m < 0 || x_scale_stride_k < 0) return PMA_ERR_ARGUMENT;
     if (!supported_dtype(y_dtype)) return PMA_ERR_DTYPE;
     if (M == 0) return PMA_OK;
@@ -1012,7 +1012,15 @@ int pma_fp8_matmul(int M, int N, int K, const void *xq, int64_t xq_stride, const
     if ((rc = device_info(&di))) return rc;
     return fp8_product(M, N, K, {static_cast<const uint8_t *>(xq), xq_stride, x_scale, x_scale_stride_m, x_scale_stride_k},
                        {static_cast<const uint8_t *>(wq), wq_stride, w_scale, w_scale_stride, 1}, y, y_stride, y_dtype,
-                       di.sms, reinterpret_cast<cudaStream_t>(stream));
+                       di.sms, after_quantize, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int pma_fp8_matmul(int M, int N, int K, const void *xq, int64_t xq_stride, const float *x_scale,
+                   int64_t x_scale_stride_m, int64_t x_scale_stride_k, const void *wq, int64_t wq_stride,
+                   const float *w_scale, int64_t w_scale_stride, void *y, int64_t y_stride, int y_dtype,
+                   pma_stream_t stream) {
+    return fp8_matmul_impl(M, N, K, xq, xq_stride, x_scale, x_scale_stride_m, x_scale_stride_k, wq, wq_stride, w_scale,
+                           w_scale_stride, y, y_stride, y_dtype, false, stream);
 }
 
 size_t pma_fp8_linear_workspace_bytes(int M, int K) { return M <= 0 || K <= 0 ? 0 : Fp8Ws::of(M, K).bytes; }
@@ -1027,8 +1035,8 @@ int pma_fp8_linear(int M, int N, int K, const void *x, int64_t x_stride, int x_d
     float *scale = reinterpret_cast<float *>((char *)workspace + w.scale_at);
     const int rc = pma_fp8_quantize(M, K, x, x_stride, x_dtype, workspace, w.stride, scale, 1, M, stream);
     return rc ? rc
-              : pma_fp8_matmul(M, N, K, workspace, w.stride, scale, 1, M, wq, wq_stride, w_scale, w_scale_stride, y,
-                               y_stride, y_dtype, stream);
+              : fp8_matmul_impl(M, N, K, workspace, w.stride, scale, 1, M, wq, wq_stride, w_scale, w_scale_stride, y,
+                                y_stride, y_dtype, true, stream);
 }
 
 int pma_state_combine(int B, int H, int D, const float *lambda, int64_t lambda_stride_b, int64_t len,
