@@ -15,7 +15,7 @@
 //
 // A cluster of 1 to 8 CTAs holds one row in shared memory, read from HBM once.  Nothing is
 // sorted.  A cut of the order is a logit and how many of its equals are kept; it is found by
-// histograms: first over z (1024 bins), then, inside the bin that holds the cut, over the logits'
+// histograms: first over z (512 bins), then, inside the bin that holds the cut, over the logits'
 // ordered bits until a bin is one value.  Only tokens that can be near a cut enter a histogram:
 //     top-k   with G >= k disjoint groups of tokens, the smallest of the groups' maxima is at most
 //             the k-th largest logit (the groups are fixed lanes, so this comes with the maximum)
@@ -32,7 +32,8 @@ namespace pma {
 namespace {
 
 constexpr int NW = 16;       // warps of a CTA
-constexpr int NB = 1024;     // histogram bins
+constexpr int NB = 512;      // histogram bins
+constexpr int LIST = 256;    // candidates a warp keeps
 constexpr int MAXC = 8;      // CTAs of a cluster
 constexpr float ZMIN = -23.0f;  // exp(-23) 2^32 < 1/2: weight 0 below
 constexpr unsigned long long ONE = 1ull << 32;
@@ -54,30 +55,36 @@ struct Shared {
     uint32_t x_cnt[MAXC];
     unsigned long long x_w[MAXC];
     Found found;
+    float list[NW][LIST];              // a warp's logits above the bound
     // per warp
     float w_max[NW], w_bound[NW];
     unsigned long long w_sum[NW];
     uint32_t w_klo[NW], w_khi[NW];
-    unsigned long long f_gt[NW];       // weight of the tokens before the cut in the warp's range
-    uint32_t f_eq[NW];                 // tokens equal to it
+    unsigned long long f_gt[MAXC * NW];  // weight of the tokens before the cut in every warp's range
+    uint32_t f_eq[MAXC * NW];            // tokens equal to it
     int owner;                         // warp of this CTA that holds the goal, or -1
     unsigned long long goal;           // goal left when its range starts
     uint32_t eq_left;                  // equals that may still be kept there
 };
 
+// A vector of VEC logits as loaded, and the largest of it without unpacking (NaN loses).
 template <typename T> struct Row;
 template <> struct Row<float> {
     static constexpr int VEC = 4;
-    static __device__ __forceinline__ void get(const float *s, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4 *>(s);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    using Raw = float4;
+    static __device__ __forceinline__ void get(const Raw &v, float (&x)[4]) { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+    static __device__ __forceinline__ Raw max(const Raw &a, const Raw &b) {
+        return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
     }
+    static __device__ __forceinline__ float max(const Raw &v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+    static __device__ __forceinline__ Raw none() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
     static __device__ __forceinline__ float lowest() { return -INFINITY; }
+    static __device__ __forceinline__ float one(float x) { return x; }
 };
 template <> struct Row<__nv_bfloat16> {
     static constexpr int VEC = 8;
-    static __device__ __forceinline__ void get(const __nv_bfloat16 *s, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(s);
+    using Raw = uint4;
+    static __device__ __forceinline__ void get(const Raw &v, float (&x)[8]) {
         const uint32_t a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -85,7 +92,21 @@ template <> struct Row<__nv_bfloat16> {
             x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
         }
     }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ Raw max(const Raw &a, const Raw &b) {
+        return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
+    }
+    static __device__ __forceinline__ float max(const Raw &v) {
+        const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+        return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
+    static __device__ __forceinline__ Raw none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xff80); }
+    static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 
 // Bits of x in an order that matches <, with -0 as +0.
@@ -113,6 +134,10 @@ __device__ __forceinline__ unsigned long long weight(float e) {
     return w == 0xffffffffu ? ONE : w;
 }
 
+__device__ __forceinline__ void add32(unsigned long long &a, uint32_t w) {
+    asm("mad.wide.u32 %0, %1, 1, %0;" : "+l"(a) : "r"(w));
+}
+
 template <typename T> __device__ __forceinline__ T warp_add(T v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -135,14 +160,69 @@ template <typename T> struct Sampler {
     const T *seg;       // NW * range tokens
     cg::cluster_group cl;
     int nc, rank, warp, lane, range;
+    int listed;      // logits in this warp's list; -1: none made, or they do not fit
+    float list_low;  // it holds those from here on
 
     template <typename F> __device__ __forceinline__ void each(F f) const {
         const T *w = seg + warp * range;
         for (int i = lane * VEC; i < range; i += 32 * VEC) {
             float x[VEC];
-            Row<T>::get(w + i, x);
+            Row<T>::get(*reinterpret_cast<const typename Row<T>::Raw *>(w + i), x);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) f(x[v]);
+        }
+    }
+    // Every logit through f, and those that are at least `low` (and not masked) into this warp's list:
+    // what follows goes by the list, a candidate a lane, instead of through vectors with one in them.
+    template <bool ALL, typename F> __device__ __forceinline__ void list_from(float low, F f) {
+        const T *w = seg + warp * range;
+        int n = 0;
+        for (int i0 = 0; i0 < range; i0 += 32 * VEC) {
+            const int i = i0 + lane * VEC;
+            const typename Row<T>::Raw raw =
+                i < range ? *reinterpret_cast<const typename Row<T>::Raw *>(w + i) : Row<T>::none();
+            float x[VEC];
+            if (ALL) {
+                Row<T>::get(raw, x);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) f(x[v]);
+            }
+            const float m = Row<T>::max(raw);
+            if (__any_sync(0xffffffffu, m >= low && m > -INFINITY)) {
+                if (!ALL) Row<T>::get(raw, x);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const bool in = x[v] >= low && x[v] > -INFINITY;
+                    const uint32_t who = __ballot_sync(0xffffffffu, in);
+                    const int at = n + __popc(who & ((1u << lane) - 1u));
+                    if (in && at < LIST) s.list[warp][at] = x[v];
+                    n += __popc(who);
+                }
+            }
+        }
+        __syncwarp();
+        listed = n <= LIST ? n : -1;
+        list_low = low;
+    }
+    // The logits that are at least `low` and not masked.
+    template <typename F> __device__ __forceinline__ void each_from(float low, F f) const {
+        if (listed >= 0 && low >= list_low) {
+            for (int i = lane; i < listed; i += 32) {
+                const float x = s.list[warp][i];
+                if (x >= low) f(x);
+            }
+            return;
+        }
+        const T *w = seg + warp * range;
+        for (int i = lane * VEC; i < range; i += 32 * VEC) {
+            const typename Row<T>::Raw raw = *reinterpret_cast<const typename Row<T>::Raw *>(w + i);
+            if (Row<T>::max(raw) >= low) {
+                float x[VEC];
+                Row<T>::get(raw, x);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    if (x[v] >= low && x[v] > -INFINITY) f(x[v]);
+            }
         }
     }
 
@@ -265,7 +345,7 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
     const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int range = p.range;
-    Sampler<T> S{s, seg, cl, nc, rank, warp, lane, range};
+    Sampler<T> S{s, seg, cl, nc, rank, warp, lane, range, -1, 0.f};
 
     // ---- the row into shared memory, its maximum, and the top-k bound
     const int first = (rank * NW + warp) * range;  // this warp's tokens of the row
@@ -275,17 +355,30 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
     {
         T *w = seg + warp * range;
         const T *src = row + first;
+        using Raw = typename Row<T>::Raw;
         if (reinterpret_cast<uintptr_t>(row) % 16 == 0) {  // ranges are whole vectors
             const int whole = n / VEC * VEC;
-            for (int i = lane * VEC; i < whole; i += 32 * VEC)
-                *reinterpret_cast<uint4 *>(w + i) = __ldcs(reinterpret_cast<const uint4 *>(src + i));
-            for (int i = whole + lane; i < n; i += 32) w[i] = src[i];
+            Raw top = Row<T>::none();
+#pragma unroll 4
+            for (int i = lane * VEC; i < whole; i += 32 * VEC) {
+                const Raw v = __ldcs(reinterpret_cast<const Raw *>(src + i));
+                *reinterpret_cast<Raw *>(w + i) = v;
+                top = Row<T>::max(top, v);
+            }
+            mx = Row<T>::max(top);
+            for (int i = whole + lane; i < n; i += 32) {
+                w[i] = src[i];
+                mx = fmaxf(mx, Row<T>::one(src[i]));
+            }
         } else {
-            for (int i = lane; i < n; i += 32) w[i] = src[i];
+            for (int i = lane; i < n; i += 32) {
+                const T v = src[i];
+                w[i] = v;
+                mx = fmaxf(mx, Row<T>::one(v));
+            }
         }
         for (int i = n + lane; i < range; i += 32) w[i] = Row<T>::lowest();
         __syncwarp();
-        S.each([&](float x) { mx = fmaxf(mx, x); });  // NaN loses
     }
     const float temp = p.temperature.at(b);
     const bool greedy = !(temp > 0.f);
@@ -336,20 +429,32 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             p.token[b] = -1;
             if (p.logprob) p.logprob[b] = -INFINITY;
         }
-        cl.sync();
         return;
     }
     const Scale sc{mx, greedy ? 1.f : fminf(__frcp_rn(temp), 3.402823466e38f), mx == INFINITY};
 
-    // ---- the weight of all tokens
+    // ---- the weight of all tokens, and with top-k the list of those above its bound
+    const bool only_first = greedy || !(top_p > 0.f) || !(min_p <= 1.f);
+    const bool by_k = !only_first && top_k > 0, by_p = !only_first && top_p < 1.f;
+    float low = by_k && bounded ? bound : -INFINITY;  // tokens below it are behind every cut
+    float fine = 0.f;                                  // bins per unit of z
+    auto set_bins = [&] {
+        // farther tokens share the last bin
+        fine = (float)NB / fminf(fmaxf(-sc.z(low), 1e-6f), -ZMIN);
+    };
+    auto bin_of = [&](float z) { return (int)fminf(-z * fine, (float)(NB - 1)); };
     unsigned long long total = 0;
     {
         uint32_t ones = 0;
-        S.each([&](float x) {
+        auto add = [&](float x) {
             const uint32_t w = weight32(expf(sc.z(x)));  // NaN converts to 0
-            total += w;
+            add32(total, w);
             ones += w == 0xffffffffu;
-        });
+        };
+        if (by_k && bounded)
+            S.template list_from<true>(low, add);
+        else
+            S.each(add);
         total = warp_add(total + ones);
         if (lane == 0) s.w_sum[warp] = total;
         __syncthreads();
@@ -357,46 +462,43 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             total = warp_add(lane < NW ? s.w_sum[lane] : 0ull);
             if (lane < nc) cl.map_shared_rank(&s, lane)->x_sum[rank] = total;
         }
-        cl.sync();
-        total = 0;
-        for (int r = 0; r < nc; ++r) total += s.x_sum[r];
     }
+    auto all_weight = [&] {  // after a cluster barrier
+        unsigned long long t = 0;
+        for (int r = 0; r < nc; ++r) t += s.x_sum[r];
+        return t;
+    };
 
     // ---- the cut
     Cut cut{0, 0xffffffffu, 0};  // keeps every token
-    const bool only_first = greedy || !(top_p > 0.f) || !(min_p <= 1.f);
     if (only_first) {
         cut = Cut{ordered(mx), 1, 0};
-    } else if (top_k || top_p < 1.f) {
-        float low = -INFINITY;  // tokens below it are behind every cut
-        if (top_k) {
-            if (bounded) low = bound;
-        } else {
+    } else if (by_k || by_p) {
+        unsigned long long wk = 0;  // weight of the top-k tokens
+        if (!by_k) {
+            cl.sync();
+            wk = all_weight();
             // weights are rounded up by at most 1/2 each; the margin covers the logarithm's error
-            const float room = (1.f - top_p) * (float)total * (1.f / 4294967296.f) / (float)p.V - 1.f / 8589934592.f;
+            const float room = (1.f - top_p) * (float)wk * (1.f / 4294967296.f) / (float)p.V - 1.f / 8589934592.f;
             if (room > 0.f) {
                 const float zl = logf(room) - 0.02f;
                 if (zl > ZMIN && !sc.inf_top) low = mx + zl / sc.inv - 4e-7f * fabsf(mx);
             }
+            if (low > -INFINITY) S.template list_from<false>(low, [](float) {});
         }
-        float span = -sc.z(low);
-        span = fminf(fmaxf(span, 1e-6f), -ZMIN);  // farther tokens share the last bin
-        const float fine = (float)NB / span;
-        auto bin_of = [&](float z) { return (int)fminf(-z * fine, (float)(NB - 1)); };
+        set_bins();
         S.clear();
-        S.each([&](float x) {
-            if (x >= low && x > -INFINITY) {
-                const float z = sc.z(x);
-                S.count(bin_of(z), weight32(expf(z)));
-            }
+        S.each_from(low, [&](float x) {
+            const float z = sc.z(x);
+            S.count(bin_of(z), weight32(expf(z)));
         });
         S.merge(0);
 
         // Narrow the bin that holds the goal down to one logit.
         auto narrow = [&](bool by_count, uint32_t by_rank, double goal, Found f) {
             uint32_t klo = 0xffffffffu, khi = 0;
-            S.each([&](float x) {
-                if (x >= low && x > -INFINITY && bin_of(sc.z(x)) == f.bin) {
+            S.each_from(low, [&](float x) {
+                if (bin_of(sc.z(x)) == f.bin) {
                     const uint32_t k = ordered(x);
                     klo = min(klo, k);
                     khi = max(khi, k);
@@ -425,13 +527,13 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
                 klo = min(klo, s.x_klo[r]);
                 khi = max(khi, s.x_khi[r]);
             }
-            for (int level = 0; level < 4 && klo < khi; ++level) {  // 10 of 32 bits each
+            for (int level = 0; level < 4 && klo < khi; ++level) {  // 9 of 32 bits each
                 int shift = 0;
                 while ((khi - klo) >> shift >= NB) ++shift;
                 S.clear();
-                S.each([&](float x) {
+                S.each_from(unordered(klo), [&](float x) {
                     const uint32_t k = ordered(x);
-                    if (k >= klo && k <= khi && x == x) S.count((int)((khi - k) >> shift), weight32(expf(sc.z(x))));
+                    if (k <= khi) S.count((int)((khi - k) >> shift), weight32(expf(sc.z(x))));
                 });
                 S.merge(1);
                 f = S.find(1, by_count, by_rank, goal, f.count, f.weight);
@@ -462,17 +564,17 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             return c;
         };
 
-        unsigned long long wk = total;  // weight of the top-k tokens
-        if (top_k) {
+        if (by_k) {
             const Found f = S.find(0, true, (uint32_t)top_k - 1, 0.0, 0, 0);
+            wk = all_weight();
             if (f.bin >= 0) {
                 cut = narrow(true, (uint32_t)top_k - 1, 0.0, f);
                 wk = cut.before + cut.keep * weight(expf(sc.z(unordered(cut.key))));
             }
         }
-        if (top_p < 1.f) {
+        if (by_p) {
             const double goal = (double)top_p * (double)wk;
-            if (top_k) S.totals(0);  // the slices' totals over z again
+            if (by_k) S.totals(0);  // the slices' totals over z again
             const Found f = S.find(0, false, 0, goal, 0, 0);
             if (f.bin >= 0) {
                 const Cut c = narrow(false, 0, goal, f);
@@ -484,26 +586,35 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
     // ---- kept weight by ranges of consecutive tokens
     const float xcut = cut.key == 0 ? -INFINITY : unordered(cut.key);
     const float need = only_first ? 0.f : min_p;
-    unsigned long long gt = 0;
-    uint32_t eq = 0;
-    S.each([&](float x) {
-        if (x >= xcut && x > -INFINITY) {
-            const float e = expf(sc.z(x));
-            if (!(e < need)) {
-                if (x > xcut)
-                    gt += weight(e);
-                else
-                    ++eq;
-            }
+    {
+        unsigned long long gt = 0;
+        uint32_t eq = 0;
+        if (cut.key == 0 && !(need > 0.f)) {
+            gt = s.w_sum[warp];  // every token
+        } else {
+            // tokens that min-p lets through are above its logarithm
+            float from = xcut;
+            if (need > 0.f && !sc.inf_top) from = fmaxf(from, mx + (logf(need) - 0.01f) / sc.inv - 4e-7f * fabsf(mx));
+            S.each_from(from, [&](float x) {
+                const float e = expf(sc.z(x));
+                if (!(e < need)) {
+                    if (x > xcut)
+                        gt += weight(e);
+                    else
+                        ++eq;
+                }
+            });
+            gt = warp_add(gt);
+            eq = warp_add(eq);
         }
-    });
-    gt = warp_add(gt);
-    eq = warp_add(eq);
-    if (lane == 0) {
-        s.f_gt[warp] = gt;
-        s.f_eq[warp] = eq;
+        if (lane < nc) {  // to every CTA: nobody reads another's memory after the barrier
+            Shared *o = cl.map_shared_rank(&s, lane);
+            o->f_gt[rank * NW + warp] = gt;
+            o->f_eq[rank * NW + warp] = eq;
+        }
     }
     cl.sync();
+    total = all_weight();
     const float ecut = expf(sc.z(xcut));
     const unsigned long long wcut = cut.key == 0 ? 0 : weight(ecut);
     if (warp == 0) {
@@ -516,9 +627,8 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
         for (int i = 0; i < MAXC * NW / 32; ++i) {
             const int r = lane * each_lane + i;
             const bool on = i < each_lane && r < ranges;
-            const Shared *o = cl.map_shared_rank(&s, on ? r / NW : rank);
-            eqs[i] = on ? o->f_eq[r % NW] : 0;
-            gts[i] = on ? o->f_gt[r % NW] : 0;
+            eqs[i] = on ? s.f_eq[r] : 0;
+            gts[i] = on ? s.f_gt[r] : 0;
             le += eqs[i];
         }
         uint32_t seen = warp_before(le, lane);
@@ -562,7 +672,7 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             unsigned long long wt[VEC], sum = 0;
             uint32_t eqn = 0;
             if (i < range) {
-                Row<T>::get(w + i, x);
+                Row<T>::get(*reinterpret_cast<const typename Row<T>::Raw *>(w + i), x);
             } else {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) x[v] = -INFINITY;
@@ -605,7 +715,6 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             if (at > goal) break;
         }
     }
-    cl.sync();  // nobody leaves while its shared memory is read
 }
 
 }  // namespace
