@@ -19,7 +19,8 @@
 // ordered bits until a bin is one value.  Only tokens that can be near a cut enter a histogram:
 //     top-k   with G >= k disjoint groups of tokens, the smallest of the groups' maxima is at most
 //             the k-th largest logit (the groups are fixed lanes, so this comes with the maximum)
-//     top-p   the tokens below z weigh less than V exp(z): those with V exp(z) <= (1 - p) W are cut
+//     top-p   the tokens below z weigh less than V exp(z): those with V exp(z) <= (1 - p) W are cut;
+//             the weight below two values of z is measured with W itself
 // The kept weights are then summed by ranges of consecutive tokens, one a warp; the warp whose
 // range holds the goal walks it.
 #include <cooperative_groups.h>
@@ -32,10 +33,12 @@ namespace pma {
 namespace {
 
 constexpr int NW = 16;       // warps of a CTA
-constexpr int NB = 512;      // histogram bins
-constexpr int LIST = 256;    // candidates a warp keeps
+constexpr int NB = NW * 32;  // histogram bins: one a thread
+constexpr int LIST = 192;    // candidates a warp keeps
+constexpr int FEW = 32;      // and how many of them one CTA may take over
 constexpr int MAXC = 8;      // CTAs of a cluster
 constexpr float ZMIN = -23.0f;  // exp(-23) 2^32 < 1/2: weight 0 below
+constexpr float ZCUT0 = -4.5f, ZCUT1 = -9.0f;  // where the tail's weight is measured
 constexpr unsigned long long ONE = 1ull << 32;
 
 struct Found {
@@ -44,21 +47,29 @@ struct Found {
     unsigned long long weight;     // their weight
 };
 
+// A thread's bin of the row's histogram (its CTA's slice of it), and what lies before it in the slice.
+struct Bin {
+    uint32_t count, before;
+    unsigned long long weight, before_weight;
+};
+
 struct Shared {
     uint32_t cnt[NB], lo[NB], hi[NB];  // this CTA's histogram (weights as two 32-bit halves)
-    uint32_t m_cnt[2][NB];             // this CTA's slice of the merged histogram: [0] over z, [1] over bits
-    unsigned long long m_w[2][NB];
     // written by the CTAs of the cluster, one slot each
     float x_max[MAXC], x_bound[MAXC];
-    unsigned long long x_sum[MAXC];
+    unsigned long long x_sum[MAXC], x_below[2][MAXC];
     uint32_t x_klo[MAXC], x_khi[MAXC];
     uint32_t x_cnt[MAXC];
     unsigned long long x_w[MAXC];
     Found found;
-    float list[NW][LIST];              // a warp's logits above the bound
+    int listed[MAXC * NW];             // length of every warp's list (-1: it does not fit)
+    uint16_t list_at[NW][LIST];        // where the listed logits lie in their warp's range
+    uint16_t few_at[MAXC * NW][FEW];   // the row's candidates, where they are few: FEW places a warp
     // per warp
     float w_max[NW], w_bound[NW];
     unsigned long long w_sum[NW];
+    uint32_t b_cnt[NW];                // block scans
+    unsigned long long b_w[NW], b_w2[NW];
     uint32_t w_klo[NW], w_khi[NW];
     unsigned long long f_gt[MAXC * NW];  // weight of the tokens before the cut in every warp's range
     uint32_t f_eq[MAXC * NW];            // tokens equal to it
@@ -118,6 +129,15 @@ __device__ __forceinline__ float unordered(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) - 1u | 0x80000000u));
 }
 
+// Keys: the ordered bits that a logit of this type can have.
+template <typename T> __device__ __forceinline__ uint32_t key_of(float x) {
+    return sizeof(T) == 2 ? ordered(x) >> 16 : ordered(x);
+}
+template <typename T> __device__ __forceinline__ float logit_of(uint32_t k) {
+    // of a negative logit the ordered bits below bf16's are ones
+    return unordered(sizeof(T) == 2 ? k << 16 | (k >> 15 ? 0u : 0xffffu) : k);
+}
+
 // z and weights of one row
 struct Scale {
     float top, inv;
@@ -158,10 +178,13 @@ template <typename T> struct Sampler {
     static constexpr int VEC = Row<T>::VEC;
     Shared &s;
     const T *seg;       // NW * range tokens
+    T *list;            // [NW][LIST] this CTA's candidates, by index
     cg::cluster_group cl;
     int nc, rank, warp, lane, range;
     int listed;      // logits in this warp's list; -1: none made, or they do not fit
     float list_low;  // it holds those from here on
+    uint32_t slice_count;  // this CTA's slice of the last merged histogram
+    unsigned long long slice_weight;
 
     template <typename F> __device__ __forceinline__ void each(F f) const {
         const T *w = seg + warp * range;
@@ -172,9 +195,9 @@ template <typename T> struct Sampler {
             for (int v = 0; v < VEC; ++v) f(x[v]);
         }
     }
-    // Every logit through f, and those that are at least `low` (and not masked) into this warp's list:
+    // Every logit through f, and those that are at least `low` (not -inf) into this warp's list:
     // what follows goes by the list, a candidate a lane, instead of through vectors with one in them.
-    template <bool ALL, typename F> __device__ __forceinline__ void list_from(float low, F f) {
+    template <bool ALL, typename F> __device__ __forceinline__ void list_from(float low, T *few, F f) {
         const T *w = seg + warp * range;
         int n = 0;
         for (int i0 = 0; i0 < range; i0 += 32 * VEC) {
@@ -187,28 +210,52 @@ template <typename T> struct Sampler {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) f(x[v]);
             }
-            const float m = Row<T>::max(raw);
-            if (__any_sync(0xffffffffu, m >= low && m > -INFINITY)) {
+            if (n <= LIST && __any_sync(0xffffffffu, Row<T>::max(raw) >= low)) {
                 if (!ALL) Row<T>::get(raw, x);
+                // lanes hold neighbouring vectors: a candidate's place is behind those of the lanes before
+                int at = n, all = 0;
+                const uint32_t before = (1u << lane) - 1u;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const bool in = x[v] >= low && x[v] > -INFINITY;
-                    const uint32_t who = __ballot_sync(0xffffffffu, in);
-                    const int at = n + __popc(who & ((1u << lane) - 1u));
-                    if (in && at < LIST) s.list[warp][at] = x[v];
-                    n += __popc(who);
+                    const uint32_t who = __ballot_sync(0xffffffffu, x[v] >= low);
+                    at += __popc(who & before);
+                    all += __popc(who);
                 }
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    if (x[v] >= low && at < LIST) {
+                        list[warp * LIST + at] = (T)x[v];
+                        s.list_at[warp][at++] = (uint16_t)(i + v);
+                    }
+                n += all;
             }
         }
         __syncwarp();
         listed = n <= LIST ? n : -1;
         list_low = low;
+        // to the first CTA of the cluster, should all lists be this short
+        if (n <= FEW) {
+            const int q = rank * NW + warp;
+            Shared *o = cl.map_shared_rank(&s, 0);
+            T *x = cl.map_shared_rank(few, 0);
+            x[q * FEW + lane] = lane < n ? list[warp * LIST + lane] : Row<T>::lowest();
+            if (lane < n) o->few_at[q][lane] = s.list_at[warp][lane];
+        }
+        if (lane < nc) cl.map_shared_rank(&s, lane)->listed[rank * NW + warp] = listed;
     }
-    // The logits that are at least `low` and not masked.
+    // A barrier of the row's CTAs.
+    __device__ __forceinline__ void sync() const {
+        if (nc == 1)
+            __syncthreads();
+        else
+            cl.sync();
+    }
+    // The logits that are at least `low` and not masked, from the list where it has them all.
     template <typename F> __device__ __forceinline__ void each_from(float low, F f) const {
         if (listed >= 0 && low >= list_low) {
+#pragma unroll 1
             for (int i = lane; i < listed; i += 32) {
-                const float x = s.list[warp][i];
+                const float x = Row<T>::one(list[warp * LIST + i]);
                 if (x >= low) f(x);
             }
             return;
@@ -243,48 +290,54 @@ template <typename T> struct Sampler {
             if (up) atomicAdd(&s.hi[bin], up);
         }
     }
-    // Sum the CTAs' histograms: this CTA keeps the slice [rank, rank + 1) * NB / nc, and everybody
-    // gets the slices' totals.
-    __device__ __forceinline__ void merge(int which) {
-        cl.sync();
-        const int per = NB / nc;
-        for (int i = threadIdx.x; i < per; i += NW * 32) {
-            uint32_t c = 0;
-            unsigned long long w = 0;
+    // Sum the CTAs' histograms: this CTA takes the slice [rank, rank + 1) * NB / nc of the bins, a bin a
+    // thread, and everybody gets the slices' totals.
+    __device__ __forceinline__ Bin merge() {
+        sync();
+        const int per = NB / nc, t = threadIdx.x;
+        Bin m{0, 0, 0, 0};
+        if (t < per) {
             for (int r = 0; r < nc; ++r) {
                 const Shared *o = cl.map_shared_rank(&s, r);
-                const int at = rank * per + i;
-                c += o->cnt[at];
-                w += ((unsigned long long)o->hi[at] << 32) + o->lo[at];
+                const int at = rank * per + t;
+                m.count += o->cnt[at];
+                m.weight += ((unsigned long long)o->hi[at] << 32) + o->lo[at];
             }
-            s.m_cnt[which][i] = c;
-            s.m_w[which][i] = w;
+        }
+        m.before = warp_before(m.count, lane);
+        m.before_weight = warp_before(m.weight, lane);
+        if (lane == 31) {
+            s.b_cnt[warp] = m.before + m.count;
+            s.b_w[warp] = m.before_weight + m.weight;
         }
         __syncthreads();
-        totals(which);
-    }
-    __device__ __forceinline__ void totals(int which) {
-        const int per = NB / nc;
-        if (warp == 0) {
-            uint32_t c = 0;
-            unsigned long long w = 0;
-            for (int i = lane; i < per; i += 32) {
-                c += s.m_cnt[which][i];
-                w += s.m_w[which][i];
+        uint32_t c = 0;
+        unsigned long long w = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            if (i == warp) {
+                m.before += c;
+                m.before_weight += w;
             }
-            c = warp_add(c);
-            w = warp_add(w);
-            if (lane < nc) {
-                Shared *o = cl.map_shared_rank(&s, lane);
-                o->x_cnt[rank] = c;
-                o->x_w[rank] = w;
-            }
+            c += s.b_cnt[i];
+            w += s.b_w[i];
         }
-        cl.sync();
+        totals(c, w);
+        slice_count = c;
+        slice_weight = w;
+        return m;
     }
-    // The first bin whose tokens reach past `by_rank` tokens (or past the weight `goal`), given what
+    __device__ __forceinline__ void totals(uint32_t c, unsigned long long w) {
+        if (warp == 0 && lane < nc) {
+            Shared *o = cl.map_shared_rank(&s, lane);
+            o->x_cnt[rank] = c;
+            o->x_w[rank] = w;
+        }
+        sync();
+    }
+    // The bin in which the tokens reach past `by_rank` tokens (or past the weight `goal`), given what
     // comes before the first bin.
-    __device__ __forceinline__ Found find(int which, bool by_count, uint32_t by_rank, double goal, uint32_t c0,
+    __device__ __forceinline__ Found find(const Bin &m, bool by_count, uint32_t by_rank, double goal, uint32_t c0,
                                           unsigned long long w0) {
         int owner = -1;
         uint32_t c = c0;
@@ -299,53 +352,39 @@ template <typename T> struct Sampler {
             c = c2;
             w = w2;
         }
-        if (owner == rank && warp == 0) {
-            const int per = NB / nc, each_lane = per / 32;
-            uint32_t lc = 0;
-            unsigned long long lw = 0;
-            for (int i = 0; i < each_lane; ++i) {
-                lc += s.m_cnt[which][lane * each_lane + i];
-                lw += s.m_w[which][lane * each_lane + i];
-            }
-            uint32_t bc = c + warp_before(lc, lane);
-            unsigned long long bw = w + warp_before(lw, lane);
-            const bool past = by_count ? bc + lc > by_rank : !((double)(bw + lw) < goal);
-            const uint32_t who = __ballot_sync(0xffffffffu, past);
-            if (lane == __ffs(who) - 1) {
-                int i = 0;
-                for (; i < each_lane - 1; ++i) {
-                    const uint32_t c2 = bc + s.m_cnt[which][lane * each_lane + i];
-                    const unsigned long long w2 = bw + s.m_w[which][lane * each_lane + i];
-                    if (by_count ? c2 > by_rank : !((double)w2 < goal)) break;
-                    bc = c2;
-                    bw = w2;
-                }
-                const Found f{rank * per + lane * each_lane + i, bc, bw};
+        if (owner == rank && (int)threadIdx.x < NB / nc) {
+            c += m.before;
+            w += m.before_weight;
+            const bool here = by_count ? c <= by_rank && c + m.count > by_rank
+                                       : m.count && (w == 0 || (double)w < goal) && !((double)(w + m.weight) < goal);
+            if (here) {
+                const Found f{(int)(rank * (NB / nc) + threadIdx.x), c, w};
                 for (int r = 0; r < nc; ++r) cl.map_shared_rank(&s, r)->found = f;
             }
         }
-        cl.sync();
+        sync();
         return owner < 0 ? Found{-1, c, w} : s.found;
     }
 };
 
 struct Cut {
-    uint32_t key;    // ordered bits of the last kept logit
+    uint32_t key;    // of the last kept logit; 0: keep all
     uint32_t keep;   // how many of its equals are kept
     unsigned long long before;  // weight before it
 };
 
 template <typename T>
-__global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(NW * 32, 2) sample_kernel(const SampleParams p) {
     constexpr int VEC = Row<T>::VEC;
     extern __shared__ __align__(16) unsigned char raw[];
     Shared &s = *reinterpret_cast<Shared *>(raw);
-    T *seg = reinterpret_cast<T *>(raw + (sizeof(Shared) + 15) / 16 * 16);
-    cg::cluster_group cl = cg::this_cluster();
-    const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    T *few = reinterpret_cast<T *>(raw + (sizeof(Shared) + 15) / 16 * 16), *list = few + MAXC * NW * FEW;
+    T *seg = p.lists ? list + NW * LIST : few;
+    const cg::cluster_group cl = cg::this_cluster();
+    int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int range = p.range;
-    Sampler<T> S{s, seg, cl, nc, rank, warp, lane, range, -1, 0.f};
+    int range = p.range;
+    Sampler<T> S{s, seg, list, cl, nc, rank, warp, lane, range, -1, 0.f, 0, 0};
 
     // ---- the row into shared memory, its maximum, and the top-k bound
     const int first = (rank * NW + warp) * range;  // this warp's tokens of the row
@@ -446,21 +485,51 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
     unsigned long long total = 0;
     {
         uint32_t ones = 0;
+        unsigned long long below[2] = {0, 0};
         auto add = [&](float x) {
             const uint32_t w = weight32(expf(sc.z(x)));  // NaN converts to 0
             add32(total, w);
             ones += w == 0xffffffffu;
         };
-        if (by_k && bounded)
-            S.template list_from<true>(low, add);
-        else
+        if (low > -INFINITY && p.lists) {
+            S.template list_from<true>(low, few, add);
+        } else if (by_p && !by_k) {
+            // also the weight below two values of z, for a bound on the nucleus
+            S.each([&](float x) {
+                const float z = sc.z(x);
+                const uint32_t w = weight32(expf(z));
+                ones += w == 0xffffffffu;
+                if (z >= ZCUT0)
+                    add32(total, w);
+                else if (z >= ZCUT1)
+                    add32(below[0], w);
+                else
+                    add32(below[1], w);
+            });
+            below[0] = warp_add(below[0] + below[1]);
+            below[1] = warp_add(below[1]);
+            if (lane == 0) {
+                s.b_w[warp] = below[0];
+                s.b_w2[warp] = below[1];
+            }
+        } else {
             S.each(add);
-        total = warp_add(total + ones);
+        }
+        total = warp_add(total + ones) + below[0];
         if (lane == 0) s.w_sum[warp] = total;
         __syncthreads();
         if (warp == 0) {
             total = warp_add(lane < NW ? s.w_sum[lane] : 0ull);
-            if (lane < nc) cl.map_shared_rank(&s, lane)->x_sum[rank] = total;
+            if (by_p && !by_k) {
+                below[0] = warp_add(lane < NW ? s.b_w[lane] : 0ull);
+                below[1] = warp_add(lane < NW ? s.b_w2[lane] : 0ull);
+            }
+            if (lane < nc) {
+                Shared *o = cl.map_shared_rank(&s, lane);
+                o->x_sum[rank] = total;
+                o->x_below[0][rank] = below[0];
+                o->x_below[1][rank] = below[1];
+            }
         }
     }
     auto all_weight = [&] {  // after a cluster barrier
@@ -469,10 +538,14 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
         return t;
     };
 
+    bool alone = false;  // only the candidates are left, in one CTA
+    int row_ranges = 0;
+    unsigned long long all_of_row = 0;
+
     // ---- the cut
     Cut cut{0, 0xffffffffu, 0};  // keeps every token
     if (only_first) {
-        cut = Cut{ordered(mx), 1, 0};
+        cut = Cut{key_of<T>(mx), 1, 0};
     } else if (by_k || by_p) {
         unsigned long long wk = 0;  // weight of the top-k tokens
         if (!by_k) {
@@ -480,11 +553,41 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             wk = all_weight();
             // weights are rounded up by at most 1/2 each; the margin covers the logarithm's error
             const float room = (1.f - top_p) * (float)wk * (1.f / 4294967296.f) / (float)p.V - 1.f / 8589934592.f;
-            if (room > 0.f) {
-                const float zl = logf(room) - 0.02f;
-                if (zl > ZMIN && !sc.inf_top) low = mx + zl / sc.inv - 4e-7f * fabsf(mx);
+            float zl = room > 0.f ? logf(room) - 0.02f : ZMIN;
+            // or where the weight above is known to hold the nucleus
+            unsigned long long tail[2] = {0, 0};
+            for (int r = 0; r < nc; ++r) {
+                tail[0] += s.x_below[0][r];
+                tail[1] += s.x_below[1][r];
             }
-            if (low > -INFINITY) S.template list_from<false>(low, [](float) {});
+            const double goal = (double)top_p * (double)wk;
+            if (!((double)(wk - tail[1]) < goal)) zl = fmaxf(zl, ZCUT1 - 0.02f);
+            if (!((double)(wk - tail[0]) < goal)) zl = fmaxf(zl, ZCUT0 - 0.02f);
+            if (zl > ZMIN && !sc.inf_top) low = mx + zl / sc.inv - 4e-7f * fabsf(mx);
+            if (low > -INFINITY && p.lists) S.template list_from<false>(low, few, [](float) {});
+        }
+        if (low > -INFINITY && p.lists) {
+            cl.sync();
+            if (by_k) wk = all_weight();
+            int most = 0, least = 0;
+            for (int i = lane; i < nc * NW; i += 32) {
+                most = max(most, s.listed[i]);
+                least = min(least, s.listed[i]);
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            least = __reduce_min_sync(0xffffffffu, least);
+            if (least == 0 && most <= FEW) {
+                // The first CTA goes on alone, with the candidates as its segment: its own barriers
+                // cost a fraction of a cluster's.
+                if (rank != 0) return;
+                all_of_row = all_weight();
+                row_ranges = nc * NW;
+                S.seg = seg = few;
+                S.nc = nc = 1;
+                S.range = range = row_ranges * FEW / NW;
+                S.listed = -1;
+                alone = true;
+            }
         }
         set_bins();
         S.clear();
@@ -492,14 +595,16 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             const float z = sc.z(x);
             S.count(bin_of(z), weight32(expf(z)));
         });
-        S.merge(0);
+        const Bin over_z = S.merge();
+        const uint32_t z_count = S.slice_count;
+        const unsigned long long z_weight = S.slice_weight;
 
         // Narrow the bin that holds the goal down to one logit.
         auto narrow = [&](bool by_count, uint32_t by_rank, double goal, Found f) {
             uint32_t klo = 0xffffffffu, khi = 0;
             S.each_from(low, [&](float x) {
                 if (bin_of(sc.z(x)) == f.bin) {
-                    const uint32_t k = ordered(x);
+                    const uint32_t k = key_of<T>(x);
                     klo = min(klo, k);
                     khi = max(khi, k);
                 }
@@ -520,7 +625,7 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
                     o->x_khi[rank] = khi;
                 }
             }
-            cl.sync();
+            S.sync();
             klo = 0xffffffffu;
             khi = 0;
             for (int r = 0; r < nc; ++r) {
@@ -531,12 +636,12 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
                 int shift = 0;
                 while ((khi - klo) >> shift >= NB) ++shift;
                 S.clear();
-                S.each_from(unordered(klo), [&](float x) {
-                    const uint32_t k = ordered(x);
+                S.each_from(logit_of<T>(klo), [&](float x) {
+                    const uint32_t k = key_of<T>(x);
                     if (k <= khi) S.count((int)((khi - k) >> shift), weight32(expf(sc.z(x))));
                 });
-                S.merge(1);
-                f = S.find(1, by_count, by_rank, goal, f.count, f.weight);
+                const Bin over_bits = S.merge();
+                f = S.find(over_bits, by_count, by_rank, goal, f.count, f.weight);
                 if (f.bin < 0) break;  // not reached: the goal lies in this range
                 khi -= (uint32_t)f.bin << shift;
                 const uint32_t width = (1u << shift) - 1;
@@ -549,7 +654,7 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
                 c.keep = by_rank + 1 - f.count;
             } else {
                 // the largest m with before + (m - 1) w < goal
-                const unsigned long long w = weight(expf(sc.z(unordered(khi))));
+                const unsigned long long w = weight(expf(sc.z(logit_of<T>(khi))));
                 if (w == 0) {
                     c.keep = 0xffffffffu;
                 } else {
@@ -565,17 +670,17 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
         };
 
         if (by_k) {
-            const Found f = S.find(0, true, (uint32_t)top_k - 1, 0.0, 0, 0);
-            wk = all_weight();
+            const Found f = S.find(over_z, true, (uint32_t)top_k - 1, 0.0, 0, 0);
+            if (!alone) wk = all_weight();
             if (f.bin >= 0) {
                 cut = narrow(true, (uint32_t)top_k - 1, 0.0, f);
-                wk = cut.before + cut.keep * weight(expf(sc.z(unordered(cut.key))));
+                wk = cut.before + cut.keep * weight(expf(sc.z(logit_of<T>(cut.key))));
             }
         }
         if (by_p) {
             const double goal = (double)top_p * (double)wk;
-            if (by_k) S.totals(0);  // the slices' totals over z again
-            const Found f = S.find(0, false, 0, goal, 0, 0);
+            if (by_k) S.totals(z_count, z_weight);  // the slices' totals over z again
+            const Found f = S.find(over_z, false, 0, goal, 0, 0);
             if (f.bin >= 0) {
                 const Cut c = narrow(false, 0, goal, f);
                 if (c.key > cut.key || (c.key == cut.key && c.keep < cut.keep)) cut = c;
@@ -584,12 +689,12 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
     }
 
     // ---- kept weight by ranges of consecutive tokens
-    const float xcut = cut.key == 0 ? -INFINITY : unordered(cut.key);
+    const float xcut = cut.key == 0 ? -INFINITY : logit_of<T>(cut.key);
     const float need = only_first ? 0.f : min_p;
     {
         unsigned long long gt = 0;
         uint32_t eq = 0;
-        if (cut.key == 0 && !(need > 0.f)) {
+        if (cut.key == 0 && !(need > 0.f) && !alone) {
             gt = s.w_sum[warp];  // every token
         } else {
             // tokens that min-p lets through are above its logarithm
@@ -613,8 +718,8 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
             o->f_eq[rank * NW + warp] = eq;
         }
     }
-    cl.sync();
-    total = all_weight();
+    S.sync();
+    total = alone ? all_of_row : all_weight();
     const float ecut = expf(sc.z(xcut));
     const unsigned long long wcut = cut.key == 0 ? 0 : weight(ecut);
     if (warp == 0) {
@@ -705,7 +810,8 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     if (goal >= c && goal - c < wt[v]) {
-                        p.token[b] = first + i + v;
+                        const int q = (warp * range + i + v) / FEW;  // alone: the warp it came from
+                        p.token[b] = alone ? q * p.range + s.few_at[q][(i + v) % FEW] : first + i + v;
                         if (p.logprob) p.logprob[b] = z[v] - logf((float)total * (1.f / 4294967296.f));
                     }
                     c += wt[v];
@@ -721,14 +827,18 @@ __global__ void __launch_bounds__(NW * 32) sample_kernel(const SampleParams p) {
 
 cudaError_t launch_sample(SampleParams p, int dtype, int sms, cudaStream_t st) {
     const int vec = dtype == PMA_F32 ? 4 : 8, esize = dtype == PMA_F32 ? 4 : 2;
-    // CTAs of a row: enough that a segment is at most 64 KB (two or three CTAs fit an SM), more while
+    // CTAs of a row: enough that a segment is at most 64 KB (bf16) or 48 KB (two CTAs fit an SM), more while
     // the batch leaves SMs without one and a warp keeps a vector a lane.
     int nc = 1;
-    while (nc < MAXC && ((int64_t)p.V * esize > (int64_t)nc * 65536 ||
+    while (nc < MAXC && ((int64_t)p.V * esize > (int64_t)nc * (esize == 4 ? 49152 : 65536) ||
                          ((int64_t)p.B * nc < sms && p.V >= nc * 2 * NW * 32 * vec)))
         nc *= 2;
     p.range = ((p.V + nc * NW - 1) / (nc * NW) + vec - 1) / vec * vec;
-    const int smem = (int)((sizeof(Shared) + 15) / 16 * 16) + NW * p.range * esize;
+    int smem = (int)((sizeof(Shared) + 15) / 16 * 16) + NW * p.range * esize;
+    const int lists = (MAXC * NW * FEW + NW * LIST) * esize;
+    // lists where they do not cost the second CTA of an SM
+    p.lists = smem + lists <= (smem <= 112 * 1024 ? 112 : 227) * 1024;
+    if (p.lists) smem += lists;
     cudaError_t e;
     constexpr int most = 227 * 1024;
     if (dtype == PMA_F32)

@@ -22,6 +22,7 @@ struct SampleParams {
     int64_t *token;      // [B]
     float *logprob;      // [B] or nullptr
     int range;           // tokens of a warp's range (set by the launcher)
+    int lists;           // there is shared memory for lists of candidates (set by the launcher)
 };
 
 constexpr int SAMPLE_MAX_V = 360448;  // 8 CTAs of 176 KB of float32 logits
