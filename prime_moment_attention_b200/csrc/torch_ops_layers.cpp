@@ -1,7 +1,8 @@
 // torch_ops_layers.cpp -- torch.ops.pma.* of the gated recurrence, the sampler and the 8-bit linear
 // product, over the C ABI of include/pma.h.
 //
-//   pma::gated_scan(x, f, bias?, gate?, h0?, reset?) -> (y, h)                 differentiable
+//   pma::gated_scan(x, f, bias?, gate?, h0?, reset?) -> (y, h)                 differentiable, through
+//     pma::gated_scan_forward (which returns its workspace too) and pma::gated_scan_backward
 //   pma::gated_scan_step(x, f, h, bias?, gate?) -> (y, new h)
 //   pma::gated_scan_step_(x, f, h(a!), bias?, gate?, rows?) -> y               h (or its rows) updated
 //   pma::sample(logits, u, temperature?, top_k?, top_p?, min_p?, t, k, p, m) -> (tokens, logprobs)
@@ -123,7 +124,9 @@ ScanArgs scan_args(const Tensor &x, const Tensor &f, const OptTensor &bias, cons
     return a;
 }
 
-std::tuple<Tensor, Tensor, Tensor> scan_forward(const ScanArgs &a) {
+std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor &x_in, const Tensor &f_in, const OptTensor &bias,
+                                                const OptTensor &gate, const OptTensor &h0, const OptTensor &reset) {
+    const ScanArgs a = scan_args(x_in, f_in, bias, gate, h0, reset);
     const at::Device dev = a.x.device();
     const c10::cuda::CUDAGuard guard(dev);
     Tensor y = at::empty({a.B, a.L, a.C}, a.x.options());
@@ -138,56 +141,81 @@ std::tuple<Tensor, Tensor, Tensor> scan_forward(const ScanArgs &a) {
     return {y, h, ws};
 }
 
+// Gradients (dx, df, dbias, dgate, dh0); the last three are empty tensors where they are not wanted.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> scan_backward(const Tensor &x_in, const Tensor &f_in,
+                                                                 const OptTensor &bias, const OptTensor &gate,
+                                                                 const OptTensor &h0, const OptTensor &reset,
+                                                                 const Tensor &ws, const OptTensor &dy_in,
+                                                                 const OptTensor &dh_in, bool want_bias, bool want_h0) {
+    const ScanArgs a = scan_args(x_in, f_in, bias, gate, h0, reset);
+    const at::Device dev = a.x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const int B = a.B, L = a.L, C = a.C;
+    if (dy_in) check_like(*dy_in, "dy", {B, L, C}, a.x.scalar_type(), dev);
+    if (dh_in) check_like(*dh_in, "dh", {B, C}, at::kFloat, dev);
+    const Tensor dy = dy_in ? rows_ok(*dy_in) : at::zeros({1, 1, C}, a.x.options()).expand({B, L, C});
+    const OptTensor dh = contiguous(dh_in);
+    const auto f32 = a.x.options().dtype(at::kFloat);
+    Tensor dx = at::empty({B, L, C}, a.x.options()), df = at::empty({B, L, C}, a.x.options());
+    Tensor dg = gate ? at::empty({B, L, C}, a.x.options()) : at::empty({0}, a.x.options());
+    Tensor db = want_bias ? at::empty({C}, f32) : at::empty({0}, f32);
+    Tensor d0 = want_h0 ? at::empty({B, C}, f32) : at::empty({0}, f32);
+    const size_t n = pma_gated_scan_backward_workspace_bytes(B, L, C);
+    Tensor w2 = at::empty({(int64_t)std::max<size_t>(n, 1)}, a.x.options().dtype(at::kByte));
+    const View xv(a.x), fv(a.f), gv(a.gate), dyv(dy), dxv(dx), dfv(df), dgv = gate ? View(dg) : View();
+    check_rc(pma_gated_scan_backward(B, L, C, xv.get(), fv.get(), gv.get(), ptr<float>(a.bias), ptr<float>(a.h0),
+                                     ptr<uint8_t>(a.reset), dyv.get(), ptr<float>(dh), dxv.get(), dfv.get(), dgv.get(),
+                                     want_bias ? db.data_ptr<float>() : nullptr, want_h0 ? d0.data_ptr<float>() : nullptr,
+                                     ws.numel() ? ws.data_ptr() : nullptr, (size_t)ws.numel(), w2.data_ptr(), n,
+                                     stream_of(dev)),
+             "pma_gated_scan_backward");
+    return {dx, df, db, dg, d0};
+}
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor &x, const Tensor &f, const OptTensor &bias, const OptTensor &gate,
+                                      const OptTensor &h0, const OptTensor &reset) {
+    auto [y, h, ws] = scan_forward(x, f, bias, gate, h0, reset);
+    return {y, h};
+}
+
+// The calls below go through the dispatcher, so that tracing sees operators with shape functions.
 struct ScanFunction : torch::autograd::Function<ScanFunction> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &f,
                                                   const OptTensor &bias, const OptTensor &gate, const OptTensor &h0,
                                                   const OptTensor &reset) {
         at::AutoDispatchBelowADInplaceOrView below;
-        const ScanArgs a = scan_args(x, f, bias, gate, h0, reset);
-        auto [y, h, ws] = scan_forward(a);
+        static const auto op = c10::Dispatcher::singleton()
+                                   .findSchemaOrThrow("pma::gated_scan_forward", "")
+                                   .typed<std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const OptTensor &,
+                                                                             const OptTensor &, const OptTensor &,
+                                                                             const OptTensor &)>();
+        auto [y, h, ws] = op.call(x, f, bias, gate, h0, reset);
         auto or_none = [](const OptTensor &t) { return t ? *t : Tensor(); };
-        ctx->save_for_backward({a.x, a.f, or_none(a.bias), or_none(a.gate), or_none(a.h0), or_none(a.reset), ws});
+        ctx->save_for_backward({x, f, or_none(bias), or_none(gate), or_none(h0), or_none(reset), ws});
         ctx->saved_data["want"] = (bias && bias->requires_grad() ? 1 : 0) + (h0 && h0->requires_grad() ? 2 : 0);
         ctx->set_materialize_grads(false);
         return {y, h};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list grads) {
-        TORCH_CHECK(!at::GradMode::is_enabled(), "gated_scan is not twice differentiable");
+        TORCH_CHECK(!at::GradMode::is_enabled() || !(grads[0].defined() && grads[0].requires_grad()),
+                    "gated_scan is not twice differentiable");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &f = saved[1], &ws = saved[6];
         auto opt = [&](int i) { return saved[i].defined() ? OptTensor(saved[i]) : OptTensor(); };
-        const OptTensor bias = opt(2), gate = opt(3), h0 = opt(4), reset = opt(5);
+        auto given = [&](int i) { return grads[i].defined() ? OptTensor(grads[i]) : OptTensor(); };
         const int64_t want = ctx->saved_data["want"].toInt();
-        const at::Device dev = x.device();
-        const c10::cuda::CUDAGuard guard(dev);
-        const int B = (int)x.size(0), L = (int)x.size(1), C = (int)x.size(2);
-        const Tensor dy = grads[0].defined() ? rows_ok(grads[0]) : at::zeros({1, 1, C}, x.options()).expand({B, L, C});
-        const OptTensor dh = grads[1].defined() ? OptTensor(grads[1].contiguous()) : OptTensor();
-        const auto f32 = x.options().dtype(at::kFloat);
-        Tensor dx = at::empty({B, L, C}, x.options()), df = at::empty({B, L, C}, x.options());
-        OptTensor dg, db, d0;
-        if (gate) dg = at::empty({B, L, C}, x.options());
-        if (want & 1) db = at::empty({C}, f32);
-        if (want & 2) d0 = at::empty({B, C}, f32);
-        const size_t n = pma_gated_scan_backward_workspace_bytes(B, L, C);
-        Tensor w2 = at::empty({(int64_t)std::max<size_t>(n, 1)}, x.options().dtype(at::kByte));
-        const View xv(x), fv(f), gv(gate), dyv(dy), dxv(dx), dfv(df), dgv(dg);
-        check_rc(pma_gated_scan_backward(B, L, C, xv.get(), fv.get(), gv.get(), ptr<float>(bias), ptr<float>(h0),
-                                         ptr<uint8_t>(reset), dyv.get(), ptr<float>(dh), dxv.get(), dfv.get(), dgv.get(),
-                                         ptr<float>(db), ptr<float>(d0), ws.numel() ? ws.data_ptr() : nullptr,
-                                         (size_t)ws.numel(), w2.data_ptr(), n, stream_of(dev)),
-                 "pma_gated_scan_backward");
-        auto or_none = [](const OptTensor &t) { return t ? *t : Tensor(); };
-        return {dx, df, or_none(db), or_none(dg), or_none(d0), Tensor()};
+        at::AutoDispatchBelowADInplaceOrView below;
+        static const auto op =
+            c10::Dispatcher::singleton()
+                .findSchemaOrThrow("pma::gated_scan_backward", "")
+                .typed<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(
+                    const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, const OptTensor &,
+                    const OptTensor &, const Tensor &, const OptTensor &, const OptTensor &, bool, bool)>();
+        auto [dx, df, db, dg, d0] = op.call(saved[0], saved[1], opt(2), opt(3), opt(4), opt(5), saved[6], given(0), given(1),
+                                            want & 1, (want & 2) != 0);
+        return {dx, df, want & 1 ? db : Tensor(), saved[3].defined() ? dg : Tensor(), want & 2 ? d0 : Tensor(), Tensor()};
     }
 };
-
-std::tuple<Tensor, Tensor> gated_scan(const Tensor &x, const Tensor &f, const OptTensor &bias, const OptTensor &gate,
-                                      const OptTensor &h0, const OptTensor &reset) {
-    auto [y, h, ws] = scan_forward(scan_args(x, f, bias, gate, h0, reset));
-    return {y, h};
-}
 
 std::tuple<Tensor, Tensor> gated_scan_autograd(const Tensor &x, const Tensor &f, const OptTensor &bias,
                                                const OptTensor &gate, const OptTensor &h0, const OptTensor &reset) {
@@ -198,7 +226,11 @@ std::tuple<Tensor, Tensor> gated_scan_autograd(const Tensor &x, const Tensor &f,
         return {out[0], out[1]};
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    return gated_scan(x, f, bias, gate, h0, reset);
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("pma::gated_scan", "")
+                               .typed<std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const OptTensor &,
+                                                                 const OptTensor &, const OptTensor &, const OptTensor &)>();
+    return op.call(x, f, bias, gate, h0, reset);
 }
 
 Tensor step_into(const Tensor &x_in, const Tensor &f_in, const Tensor &h_in, const Tensor &h_out, const OptTensor &bias_in,
@@ -316,6 +348,10 @@ Tensor fp8_linear(const Tensor &x_in, const Tensor &wq_in, const Tensor &ws_in, 
 TORCH_LIBRARY_FRAGMENT(pma, m) {
     m.def("gated_scan(Tensor x, Tensor f, Tensor? bias=None, Tensor? gate=None, Tensor? h0=None, Tensor? reset=None) -> "
           "(Tensor, Tensor)");
+    m.def("gated_scan_forward(Tensor x, Tensor f, Tensor? bias, Tensor? gate, Tensor? h0, Tensor? reset) -> "
+          "(Tensor, Tensor, Tensor)");
+    m.def("gated_scan_backward(Tensor x, Tensor f, Tensor? bias, Tensor? gate, Tensor? h0, Tensor? reset, Tensor ws, "
+          "Tensor? dy, Tensor? dh, bool want_bias, bool want_h0) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("gated_scan_step(Tensor x, Tensor f, Tensor h, Tensor? bias=None, Tensor? gate=None) -> (Tensor, Tensor)");
     m.def("gated_scan_step_(Tensor x, Tensor f, Tensor(a!) h, Tensor? bias=None, Tensor? gate=None, Tensor? rows=None) "
           "-> Tensor");
@@ -326,6 +362,8 @@ TORCH_LIBRARY_FRAGMENT(pma, m) {
 
 TORCH_LIBRARY_IMPL(pma, CUDA, m) {
     m.impl("gated_scan", &gated_scan);
+    m.impl("gated_scan_forward", &scan_forward);
+    m.impl("gated_scan_backward", &scan_backward);
     m.impl("gated_scan_step", &gated_scan_step);
     m.impl("gated_scan_step_", &gated_scan_step_);
     m.impl("sample", &sample);

@@ -54,6 +54,16 @@ def _scales(name: str, s: torch.Tensor, shape, dev) -> torch.Tensor:
     return s
 
 
+class Fp8Weight:
+    """A weight [N, K] kept in e4m3 with its block scales: call it on x [..., K]."""
+
+    def __init__(self, weight: torch.Tensor):
+        self.q, self.scale = quantize_weight(weight)
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        return linear(x, self.q, self.scale, out_dtype=x.dtype)
+
+
 def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[M, K] bf16 or float32 -> (e4m3 [M, K], scales [M, ceil(K/128)]).  The scales' storage is
     [ceil(K/128), M], the order the product reads them in."""

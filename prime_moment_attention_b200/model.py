@@ -3,13 +3,16 @@
 Mirrors src/prime_moment_attention/model.py (PrimeConfig :20-44, RMSNorm :47-56, PrimeMLP :59-68,
 PrimeBlock :71-117, PrimeForCausalLM :120-244) with the same parameter names and shapes, so a
 state_dict of the reference model loads unchanged; every attention layer is this package's
-PrimeMomentAttention (prologue and core on the CUDA kernels).  Inference only.
+PrimeMomentAttention (prologue and core on the CUDA kernels).  Inference only with those layers.
 
 Beyond the reference's forward / generate, two serving paths:
   * forward(..., last_logits_only=True) computes the LM head for the last position only (what
     generate needs; the reference computes [B, L, vocab] logits);
-  * DecodeGraph: one greedy decode step of the whole model captured in a CUDA graph, the
-    per-layer states updated in place by pma_decode_step (no Python or allocation per step).
+  * DecodeGraph: one greedy or sampled decode step of the whole model captured in a CUDA graph, the
+    per-layer states updated in place by pma_decode_step (no Python or allocation per step), its
+    products in bf16 or on e4m3 weights.
+
+With PrimeConfig(use_recurrence=True) the layers are GatedRecurrence, and the model trains too.
 """
 from __future__ import annotations
 
@@ -21,8 +24,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import fp8 as fp8_ops
 from . import ops
 from .attention import PrimeMomentAttention, _prologue
+from .recurrence import GatedRecurrence
+from .sampling import Sampler
 from .selective import PrimeSelectiveMomentAttention
 
 
@@ -45,6 +51,7 @@ class PrimeConfig:
     use_selective: bool = False
     min_tau: float = 2.0
     max_tau: float = 2000.0
+    use_recurrence: bool = False  # beyond the reference: GatedRecurrence layers, which also train
 
     def __post_init__(self):
         if self.num_kv_heads is None:
@@ -75,7 +82,10 @@ class PrimeMLP(nn.Module):
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return self.down_proj(ops.swiglu(self.gate_proj(x), self.up_proj(x)))
+        gate, up = self.gate_proj(x), self.up_proj(x)
+        if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+            return self.down_proj(F.silu(gate) * up)  # the same values; the kernel has no gradient
+        return self.down_proj(ops.swiglu(gate, up))
 
 
 class PrimeBlock(nn.Module):
@@ -84,7 +94,9 @@ class PrimeBlock(nn.Module):
     def __init__(self, config: PrimeConfig):
         super().__init__()
         self.input_layernorm = RMSNorm(config.hidden_size, eps=config.rms_norm_eps)
-        if config.use_selective:
+        if config.use_recurrence:
+            self.self_attn = GatedRecurrence(config.hidden_size, config.num_heads * config.head_dim)
+        elif config.use_selective:
             self.self_attn = PrimeSelectiveMomentAttention(
                 hidden_size=config.hidden_size, num_heads=config.num_heads, head_dim=config.head_dim,
                 num_kv_heads=config.num_kv_heads, decay=config.decay, use_qk_norm=config.use_qk_norm,
@@ -157,15 +169,24 @@ class PrimeForCausalLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 50, temperature: float = 1.0,
-                 top_k: int = 50, eos_token_id: Optional[int] = None) -> torch.Tensor:
-        """Same sampling rule as model.py:203-242 (greedy when temperature == 0)."""
+                 top_k: int = 50, eos_token_id: Optional[int] = None, top_p: float = 1.0, min_p: float = 0.0,
+                 uniforms: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Same sampling rule as model.py:203-242 (greedy when temperature == 0), drawn by
+        torch.multinomial.  With `uniforms` [max_new_tokens, B], float32 in [0, 1), the tokens come
+        from sampling.sample instead: given numbers, and top_p and min_p as well as top_k."""
         self.eval()
+        if uniforms is None and (top_p < 1.0 or min_p > 0.0):
+            raise ValueError("top_p and min_p need uniforms")
+        sampler = Sampler(temperature, top_k, top_p, min_p)
         out = self.forward(input_ids, return_states=True, last_logits_only=True)
         states, logits = out["states"], out["logits"][:, -1, :]
         generated = input_ids
-        for _ in range(max_new_tokens):
-            logits = torch.nan_to_num(logits, nan=0.0, posinf=50.0, neginf=-50.0)
-            if temperature > 0.0:
+        for step in range(max_new_tokens):
+            if uniforms is None:
+                logits = torch.nan_to_num(logits, nan=0.0, posinf=50.0, neginf=-50.0)
+            if uniforms is not None:
+                nxt = sampler(logits, uniforms[step])[0][:, None]
+            elif temperature > 0.0:
                 lg = logits / max(temperature, 1e-4)
                 if top_k > 0:
                     v, _ = torch.topk(lg, min(top_k, lg.size(-1)))
@@ -183,76 +204,119 @@ class PrimeForCausalLM(nn.Module):
 
 
 class DecodeGraph:
-    """One greedy decode step of `model` for a fixed batch, captured in a CUDA graph.
+    """One decode step of `model` for a fixed batch, captured in a CUDA graph.
 
     The per-layer states are owned here (copied from `states` once) and updated in place by
     pma_decode_step_ex (pma_selective_decode_step for selective layers, whose per-token decay is
-    computed inside the graph); `step()` replays the graph: token ids in `self.tokens` [B, 1] ->
-    next greedy ids in `self.tokens` and the step's logits in `self.logits` [B, vocab].
-    Mirrors the decode loop of generate (model.py:227-240) with temperature 0."""
+    computed inside the graph; pma_gated_scan_step for recurrence layers); `step()` replays the
+    graph: token ids in `self.tokens` [B, 1] -> next ids in `self.tokens` and the step's logits in
+    `self.logits` [B, vocab].  Mirrors the decode loop of generate (model.py:227-240) with
+    temperature 0.
+
+    With a `sampler` (sampling.Sampler) the step samples instead: `step(u)` takes the step's uniform
+    numbers [B] and leaves the tokens' log-probabilities in `self.logprobs`.  With fp8=True the
+    projections and the head run on e4m3 copies of the weights (fp8.Fp8Weight)."""
 
     def __init__(self, model: PrimeForCausalLM, states: List[Tuple[torch.Tensor, ...]], tokens: torch.Tensor,
-                 warmup: int = 2):
+                 warmup: int = 2, sampler: Optional[Sampler] = None, fp8: bool = False):
         self.model = model
         dev = tokens.device
         self.states = [tuple(t.detach().to(torch.float32).contiguous().clone() for t in st) for st in states]
+        self.sampler, self.logprobs = sampler, None
+        self.u = torch.zeros(tokens.numel(), dtype=torch.float32, device=dev) if sampler is not None else None
         # one GEMM for q, k, v and one for gate, up per layer (concatenated copies of the weights,
         # taken now: the graph serves the weights as they are at construction)
-        self.w_qkv, self.w_gu = [], []
+        self.w_qkv, self.w_gu, self.w_o, self.w_down = [], [], [], []
+        keep = fp8_ops.Fp8Weight if fp8 else (lambda w: w)
         for layer in model.layers:
             a, mlp = layer.self_attn, layer.mlp
-            self.w_qkv.append(torch.cat([a.q_proj.weight, a.k_proj.weight, a.v_proj.weight]).detach().contiguous())
-            self.w_gu.append(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]).detach().contiguous())
+            if isinstance(a, GatedRecurrence):
+                w = a.in_proj.weight.detach().clone()
+            else:
+                w = torch.cat([a.q_proj.weight, a.k_proj.weight, a.v_proj.weight]).detach().contiguous()
+            self.w_qkv.append(keep(w))
+            self.w_gu.append(keep(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight]).detach().contiguous()))
+            self.w_o.append(keep(a.o_proj.weight.detach()))
+            self.w_down.append(keep(mlp.down_proj.weight.detach()))
+        self.head = keep(model.lm_head.weight.detach()) if fp8 else None
         self.tokens = tokens.detach().reshape(-1, 1).clone()
         self.logits = None
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(s):
+        with torch.cuda.stream(s), torch.no_grad():
             for _ in range(warmup):  # settles allocator pools and per-module caches before capture
                 self._body(write=False)
         torch.cuda.current_stream(dev).wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with torch.cuda.graph(self.graph), torch.no_grad():
             self._body(write=True)
+
+    @staticmethod
+    def _mm(x: torch.Tensor, w) -> torch.Tensor:
+        return torch.mm(x, w.t()) if isinstance(w, torch.Tensor) else w(x)
+
+    @staticmethod
+    def _add_mm(h: torch.Tensor, x: torch.Tensor, w) -> torch.Tensor:
+        return torch.addmm(h, x, w.t()) if isinstance(w, torch.Tensor) else h + w(x)
 
     def _body(self, write: bool):
         m = self.model
         h = m.embed_tokens(self.tokens)  # [B, 1, hidden]
         h = h[:, 0]  # [B, hidden]
-        for layer, st, w_qkv, w_gu in zip(m.layers, self.states, self.w_qkv, self.w_gu):
+        for layer, st, w_qkv, w_gu, w_o, w_down in zip(m.layers, self.states, self.w_qkv, self.w_gu, self.w_o,
+                                                       self.w_down):
             attn = layer.self_attn
             x = layer.input_layernorm(h)
             B = x.shape[0]
-            H, D, Hk = attn.num_heads, attn.head_dim, attn.num_kv_heads
-            qkv = torch.mm(x, w_qkv.t())  # [B, (H + 2 Hk) D]; q, k, v are strided views of it
-            q = qkv[:, :H * D].view(B, H, D)
-            k = qkv[:, H * D:(H + Hk) * D].view(B, Hk, D)
-            v = qkv[:, (H + Hk) * D:].view(B, Hk, D)
-            pro = _prologue(attn)
-            if pro is None:
-                raise NotImplementedError("DecodeGraph needs QK-norms the kernels fold (nn.LayerNorm over head_dim)")
+            qkv = self._mm(x, w_qkv)  # [B, (H + 2 Hk) D]; q, k, v are strided views of it
             st_step = st if write else tuple(t.clone() for t in st)
-            if isinstance(attn, PrimeSelectiveMomentAttention):
-                # this token's decay exp(-Delta / tau_h), Delta = clamp(softplus(delta_proj(x)), 1e-4, 50),
-                # and k scaled by beta_h, as in the step branch (selective.py:367-396)
-                delta = F.softplus(attn.delta_proj(x)).clamp(min=1e-4, max=50.0)  # [B, H]
-                log_decay = -delta.float() / attn.get_tau(x.device).view(1, H)
-                y, _ = ops.selective_decode_step(q, k, v, log_decay, attn.get_beta(x.device).float(), st_step,
-                                                 eps=attn.eps, inplace=True, prologue=pro)
+            if isinstance(attn, GatedRecurrence):
+                y = attn.step_(qkv, st_step)
             else:
-                decay = getattr(attn, "decay_per_head", None)
-                decay = attn.decay if decay is None else decay
-                y, _ = ops.decode_step(q, k, v, decay, st_step, eps=attn.eps, inplace=True, prologue=pro)
-            h = torch.addmm(h, y.reshape(B, H * D).to(h.dtype), attn.o_proj.weight.t())  # residual + o_proj
-            gu = torch.mm(layer.post_attention_layernorm(h), w_gu.t())
+                y = self._attend(attn, x, qkv, st_step)
+            h = self._add_mm(h, y.reshape(B, -1).to(h.dtype), w_o)  # residual + o_proj
+            gu = self._mm(layer.post_attention_layernorm(h), w_gu)
             inter = gu.shape[1] // 2
-            h = torch.addmm(h, ops.swiglu(gu[:, :inter], gu[:, inter:]), layer.mlp.down_proj.weight.t())
-        logits = m.lm_head(m.norm(h))
-        nxt = torch.argmax(logits, dim=-1, keepdim=True)
+            h = self._add_mm(h, ops.swiglu(gu[:, :inter], gu[:, inter:]), w_down)
+        logits = m.lm_head(m.norm(h)) if self.head is None else self.head(m.norm(h))
+        if self.sampler is None:
+            nxt = torch.argmax(logits, dim=-1, keepdim=True)
+        else:
+            nxt, logprobs = self.sampler(logits, self.u)
+            nxt = nxt[:, None]
+            if write:
+                self.logprobs = logprobs
         if write:
             self.logits = logits
             self.tokens.copy_(nxt)
 
-    def step(self) -> torch.Tensor:
+    @staticmethod
+    def _attend(attn, x: torch.Tensor, qkv: torch.Tensor, st_step) -> torch.Tensor:
+        B = x.shape[0]
+        H, D, Hk = attn.num_heads, attn.head_dim, attn.num_kv_heads
+        q = qkv[:, :H * D].view(B, H, D)
+        k = qkv[:, H * D:(H + Hk) * D].view(B, Hk, D)
+        v = qkv[:, (H + Hk) * D:].view(B, Hk, D)
+        pro = _prologue(attn)
+        if pro is None:
+            raise NotImplementedError("DecodeGraph needs QK-norms the kernels fold (nn.LayerNorm over head_dim)")
+        if isinstance(attn, PrimeSelectiveMomentAttention):
+            # this token's decay exp(-Delta / tau_h), Delta = clamp(softplus(delta_proj(x)), 1e-4, 50),
+            # and k scaled by beta_h, as in the step branch (selective.py:367-396)
+            delta = F.softplus(attn.delta_proj(x)).clamp(min=1e-4, max=50.0)  # [B, H]
+            log_decay = -delta.float() / attn.get_tau(x.device).view(1, H)
+            y, _ = ops.selective_decode_step(q, k, v, log_decay, attn.get_beta(x.device).float(), st_step,
+                                             eps=attn.eps, inplace=True, prologue=pro)
+        else:
+            decay = getattr(attn, "decay_per_head", None)
+            decay = attn.decay if decay is None else decay
+            y, _ = ops.decode_step(q, k, v, decay, st_step, eps=attn.eps, inplace=True, prologue=pro)
+        return y
+
+    def step(self, u: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if (u is None) != (self.sampler is None):
+            raise ValueError("step() takes uniform numbers exactly when the graph samples")
+        if u is not None:
+            self.u.copy_(u)
         self.graph.replay()
         return self.tokens

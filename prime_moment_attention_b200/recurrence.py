@@ -9,12 +9,16 @@ gated_scan is differentiable in x, f, bias, gate and h0.
 
     y, h = gated_scan(x, f, bias, gate, h0, reset)            # prefill or training; h continues it
     y, h = gated_scan_step(x1, f1, h, bias=bias, gate=gate1)  # one token
+
+GatedRecurrence is the layer around it, with the interface of the attention modules.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
+import torch.nn as nn
 
 from . import torch_ops
 from .ops import _require_cuda, check_faults
@@ -57,3 +61,44 @@ def gated_scan_step(x: torch.Tensor, f: torch.Tensor, h: torch.Tensor, bias: Opt
     if rows is not None or inplace:
         return _ops()[2](x, f, h, bias, gate, rows), h
     return _ops()[1](x, f, h, bias, gate)
+
+
+class GatedRecurrence(nn.Module):
+    """Sequence mixer on the gated recurrence, in the place of an attention module: one projection to
+    (x, f, gate), the scan over `width` channels, one projection back.  Trains (the attention modules
+    do not); prefill and decode carry the state (h [B, width] float32,).  The decays start spread
+    over [min_decay, max_decay], evenly in their time constants' logarithm."""
+
+    def __init__(self, hidden_size: int, width: Optional[int] = None, min_decay: float = 0.9,
+                 max_decay: float = 0.9999):
+        super().__init__()
+        if not 0.0 < min_decay <= max_decay < 1.0:
+            raise ValueError("decays must satisfy 0 < min_decay <= max_decay < 1")
+        self.hidden_size = hidden_size
+        self.width = width or hidden_size
+        self.in_proj = nn.Linear(hidden_size, 3 * self.width, bias=False)
+        self.o_proj = nn.Linear(self.width, hidden_size, bias=False)
+        lo, hi = math.log(1.0 - min_decay), math.log(1.0 - max_decay)
+        z = torch.exp(torch.linspace(lo, hi, self.width))  # 1 - decay
+        self.decay_bias = nn.Parameter(torch.log((1.0 - z) / z))
+
+    def forward(self, hidden_states: torch.Tensor, state: Optional[Tuple[torch.Tensor, ...]] = None,
+                return_state: bool = False, reset: Optional[torch.Tensor] = None):
+        """hidden_states [B, L, hidden]; state (h,) of the tokens before; reset [B, L] marks the first
+        tokens of packed documents.  Returns (output, (h,) or None)."""
+        x, f, gate = self.in_proj(hidden_states).split(self.width, dim=-1)
+        h0 = state[0] if state is not None else None
+        bias = self.decay_bias.float()
+        if hidden_states.shape[1] == 1 and reset is None and not torch.is_grad_enabled():
+            if h0 is None:
+                h0 = torch.zeros(x.shape[0], self.width, dtype=torch.float32, device=x.device)
+            y, h = gated_scan_step(x[:, 0], f[:, 0], h0, bias=bias, gate=gate[:, 0])
+            y = y[:, None]
+        else:
+            y, h = gated_scan(x, f, bias, gate, h0, reset)
+        return self.o_proj(y), ((h,) if return_state else None)
+
+    def step_(self, xfg: torch.Tensor, state: Tuple[torch.Tensor, ...]) -> torch.Tensor:
+        """One token from its projections [B, 3 width] with the state updated in place; before o_proj."""
+        x, f, gate = xfg.split(self.width, dim=-1)
+        return gated_scan_step(x, f, state[0], bias=self.decay_bias.float(), gate=gate, inplace=True)[0]

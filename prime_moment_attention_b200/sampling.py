@@ -6,6 +6,7 @@ token in any batch.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Tuple, Union
 
 import torch
@@ -16,6 +17,18 @@ from .ops import _require_cuda
 Setting = Union[int, float, torch.Tensor]
 MAX_VOCAB = 360448
 _fn = None
+
+
+@dataclass
+class Sampler:
+    """Settings of sample(), as numbers or per-row tensors."""
+    temperature: Setting = 1.0
+    top_k: Setting = 0
+    top_p: Setting = 1.0
+    min_p: Setting = 0.0
+
+    def __call__(self, logits: torch.Tensor, u: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return sample(logits, u, self.temperature, self.top_k, self.top_p, self.min_p)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0,

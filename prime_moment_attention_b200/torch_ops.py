@@ -31,6 +31,12 @@ def _state_like(B: int, H: int, D: int, device):
     return [f(B, H, D), f(B, H, D, D), f(B, H, D, D), f(B, H, 1), f(B, H, D), f(B, H, D)]
 
 
+def _scan_bytes(words: int) -> int:
+    """pma_gated_scan_workspace_bytes of `words` states: 256 + states, then runs, each rounded to 256."""
+    runs_at = (256 + 4 * words + 255) // 256 * 256
+    return (runs_at + 8 * words + 255) // 256 * 256
+
+
 def load() -> None:
     """Load the operator library (once) and register the operators' shape functions."""
     global _loaded
@@ -57,6 +63,20 @@ def load() -> None:
     @torch.library.register_fake("pma::gated_scan")
     def _gated_scan_fake(x, f, bias=None, gate=None, h0=None, reset=None):
         return x.new_empty(x.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)
+
+    @torch.library.register_fake("pma::gated_scan_forward")
+    def _gated_scan_forward_fake(x, f, bias, gate, h0, reset):
+        B, L, C = x.shape
+        words = B * ((L + 127) // 128) * C
+        return (x.new_empty(x.shape), x.new_empty((B, C), dtype=torch.float32),
+                x.new_empty((0 if L <= 128 else _scan_bytes(words),), dtype=torch.uint8))
+
+    @torch.library.register_fake("pma::gated_scan_backward")
+    def _gated_scan_backward_fake(x, f, bias, gate, h0, reset, ws, dy, dh, want_bias, want_h0):
+        B, _, C = x.shape
+        f32 = lambda *s: x.new_empty(s, dtype=torch.float32)  # noqa: E731
+        return (x.new_empty(x.shape), x.new_empty(x.shape), f32(C) if want_bias else f32(0),
+                x.new_empty(x.shape if gate is not None else (0,)), f32(B, C) if want_h0 else f32(0))
 
     @torch.library.register_fake("pma::gated_scan_step")
     def _gated_scan_step_fake(x, f, h, bias=None, gate=None):
