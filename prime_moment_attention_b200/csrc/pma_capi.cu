@@ -907,7 +907,7 @@ int pma_gated_scan_backward(int B, int L, int C, const pma_seq_tensor *x, const 
     p.states = w.nwords && w.chunks > 1 ? w.incl(const_cast<void *>(forward_ws)) : nullptr;
     p.dbias_part = dbias ? w.part(workspace) : nullptr;
     if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
-    e = launch_gated_scan_backward(p, x->dtype, dbias, st);
+    e = launch_gated_scan_backward(p, x->dtype, dbias, di.sms, st);
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 

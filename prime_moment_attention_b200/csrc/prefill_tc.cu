@@ -935,6 +935,16 @@ static EncodeTiled get_encode() {
     return fn;
 }
 
+// The encoder is a driver call and needs the device's context current in the calling thread, which a
+// thread that has made no runtime call yet (an autograd worker, say) does not have: bind it and try
+// once more.
+template <typename F> static bool encoded(F encode) {
+    if (encode() == CUDA_SUCCESS) return true;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    return encode() == CUDA_SUCCESS;
+}
+
 bool tensor_maps_available() { return get_encode() != nullptr; }
 
 // [B,H,L,Dh] bf16 with element strides -> 4-D map (d, l, h, b), box 64 x 128 x 1 x 1, 128-byte
@@ -949,9 +959,11 @@ bool make_tile_map(CUtensorMap *m, const Seq &s, int B, int H, int L, int Dh) {
         if (str[i] == 0) str[i] = 16;
     const cuuint32_t box[4] = {64, (cuuint32_t)C, 1, 1};
     const cuuint32_t es[4] = {1, 1, 1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(s.p), dims, str, box, es,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded([&] {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(s.p), dims, str, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 // [rows, cols] bytes with a row stride in bytes: boxes of 128 bytes x box_rows, 128-byte swizzle.
@@ -962,9 +974,11 @@ bool make_map_2d_u8(CUtensorMap *m, const void *base, int64_t rows, int64_t cols
     const cuuint64_t str[1] = {(cuuint64_t)stride};
     const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
     const cuuint32_t es[2] = {1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, str, box, es,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded([&] {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, str, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 // A [B, L, C] array with element strides: boxes of 128 bytes of C x `rows` of L x 1, no swizzle.
@@ -976,9 +990,11 @@ bool make_blc_map(CUtensorMap *m, const void *base, int64_t sb, int64_t sl, int 
     const cuuint64_t str[2] = {(cuuint64_t)(L > 1 ? sl * esize : 16), (cuuint64_t)(B > 1 ? sb * esize : 16)};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / esize), (cuuint32_t)rows, 1};
     const cuuint32_t es[3] = {1, 1, 1};
-    return enc(m, esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-               const_cast<void *>(base), dims, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded([&] {
+        return enc(m, esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                   const_cast<void *>(base), dims, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 template <bool SO, typename TO, bool PRO, bool PT>

@@ -62,7 +62,6 @@ template <> struct Vf<1> {
     float v;
     static __device__ __forceinline__ Vf all(float a) { return {a}; }
     __device__ __forceinline__ float at(int) const { return v; }
-    __device__ __forceinline__ void set(int, float a) { v = a; }
 };
 template <> struct Vf<2> {
     unsigned long long v;
@@ -77,8 +76,15 @@ template <> struct Vf<2> {
         asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
         return i ? b : a;
     }
-    __device__ __forceinline__ void set(int i, float a) { *this = i ? of(at(0), a) : of(a, at(1)); }
 };
+// The values f(0) .. f(V - 1)
+template <int V, typename F> __device__ __forceinline__ Vf<V> gather(F f) {
+    if constexpr (V == 1)
+        return {f(0)};
+    else
+        return Vf<2>::of(f(0), f(1));
+}
+
 __device__ __forceinline__ Vf<1> fma(Vf<1> a, Vf<1> b, Vf<1> c) { return {fmaf(a.v, b.v, c.v)}; }
 __device__ __forceinline__ Vf<1> mul(Vf<1> a, Vf<1> b) { return {a.v * b.v}; }
 __device__ __forceinline__ Vf<1> add(Vf<1> a, Vf<1> b) { return {a.v + b.v}; }
@@ -126,21 +132,13 @@ template <int V> __device__ __forceinline__ Run<V> no_run() { return {Vf<V>::all
 // the state after a run; with CUT, Q = 1 drops the state whatever it was (a reset, or a state handed on)
 template <bool CUT, int V> __device__ __forceinline__ Vf<V> join(Vf<V> h, const Run<V> &r) {
     Vf<V> o = add(h, fma(r.n, h, r.h));
-    if (CUT) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (r.n.at(v) == -1.f) o.set(v, r.h.at(v));
-    }
+    if (CUT) o = gather<V>([&](int v) { return r.n.at(v) == -1.f ? r.h.at(v) : o.at(v); });
     return o;
 }
 // run a, then run b
 template <bool CUT, int V> __device__ __forceinline__ Run<V> join(const Run<V> &a, const Run<V> &b) {
     Run<V> o{fma(b.n, add(a.n, Vf<V>::all(1.f)), a.n), join<CUT>(a.h, b)};
-    if (CUT) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (b.n.at(v) == -1.f) o.n.set(v, -1.f);
-    }
+    if (CUT) o.n = gather<V>([&](int v) { return b.n.at(v) == -1.f ? -1.f : o.n.at(v); });
     return o;
 }
 
@@ -285,12 +283,8 @@ __device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K
     }
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-        out[i] = no_run<V>();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            out[i].n.set(v, n[i][v]);
-            out[i].h.set(v, h[i][v]);
-        }
+        out[i].n = gather<V>([&](int v) { return n[i][v]; });
+        out[i].h = gather<V>([&](int v) { return h[i][v]; });
     }
 }
 
@@ -340,10 +334,7 @@ __device__ __forceinline__ Vf<V> chain(const ScanParams &p, const Tile &k, const
     const int64_t slot = k.word0 + (int64_t)k.chunk * p.C;
     Vf<V> in = Vf<V>::all(0.f);
     if (k.chunk == 0) {
-        if (live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) in.set(v, first(v));
-        }
+        if (live) in = gather<V>(first);
     } else {
         if (warp == 0 && live) put(p.agg + slot, whole);
         const int reach = k.chunk < LOOK ? k.chunk : LOOK;
@@ -427,11 +418,8 @@ __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const Sca
     load_rows<T, V, R>(x, p.x, k.b, l0, p.L, c);
     if constexpr (GATE) load_rows<T, V, R>(o, p.gate, k.b, l0, p.L, c);
     const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
-    Vf<V> bias = Vf<V>::all(0.f), z[R];
-    if (p.bias) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
-    }
+    const Vf<V> bias = gather<V>([&](int v) { return p.bias ? __ldg(p.bias + c + v) * LOG2E : 0.f; });
+    Vf<V> z[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) z[r] = sigmoid_neg2(fma(f[r].f(), Vf<V>::all(LOG2E), bias));
     if (rows < R) {
@@ -509,15 +497,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
     load_rows<T, V, R>(x, p.x, k.b, l0, p.L, c);
     load_rows<T, V, R>(dy, p.dy, k.b, l0, p.L, c);
     if constexpr (GATE) load_rows<T, V, R>(o, p.gate, k.b, l0, p.L, c);
-    Vf<V> start = Vf<V>::all(0.f), bias = start;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (chunk > 0)
-            start.set(v, __uint_as_float(p.states[((int64_t)k.b * p.chunks + chunk - 1) * p.C + c + v]));
-        else if (p.h0)
-            start.set(v, p.h0[(int64_t)k.b * p.C + c + v]);
-        if (p.bias) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
-    }
+    const Vf<V> bias = gather<V>([&](int v) { return p.bias ? __ldg(p.bias + c + v) * LOG2E : 0.f; });
+    Vf<V> start = gather<V>([&](int v) {
+        if (chunk > 0) return __uint_as_float(p.states[((int64_t)k.b * p.chunks + chunk - 1) * p.C + c + v]);
+        return p.h0 ? p.h0[(int64_t)k.b * p.C + c + v] : 0.f;
+    });
     const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
     Vf<V> z[R], sg[GATE ? R : 1];
 #pragma unroll
@@ -677,9 +661,9 @@ template <> struct Word<__nv_bfloat16> {
 };
 
 // Barriers of the stages, and the tiles in them (chunk -1: no more).  The FSTAGES stages of the first
-// pass's input are freed by the workers.
+// pass's input (FSTAGES 0: none apart) are freed by the workers.
 template <int FSTAGES, int STAGES> struct Ring {
-    uint64_t full[STAGES], done[STAGES], empty[STAGES], f_empty[FSTAGES];
+    uint64_t full[STAGES], done[STAGES], empty[STAGES], f_empty[FSTAGES ? FSTAGES : 1];
     Tile tile[STAGES];
     tc::CtlShared ctl;
     __device__ __forceinline__ void init(int consumers, int *fault) {
@@ -706,8 +690,11 @@ template <int FSTAGES, int STAGES> struct Ring {
                 if (--ends == 0) return;
                 continue;
             }
-            const int fs = n % FSTAGES;
-            if (!tc::mbar_wait(&f_empty[fs], ((n / FSTAGES) & 1) ^ 1, c, FAULT_CODE + 1)) break;
+            int fs = 0;
+            if constexpr (FSTAGES > 0) {
+                fs = n % FSTAGES;
+                if (!tc::mbar_wait(&f_empty[fs], ((n / FSTAGES) & 1) ^ 1, c, FAULT_CODE + 1)) break;
+            }
             tile[s] = tile_of<V>(p, t, 0);
             copy(s, fs, tile[s]);
         }
@@ -783,11 +770,8 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
             const uint8_t *os = xs + G::TILE;
             const uint8_t *fs = f_tiles + (n % G::FSTAGES) * G::TILE + warp * R * 128 + lane * 4;
             const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
-            Vf<V> bias = Vf<V>::all(0.f), z[R];
-            if (p.bias && live) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) bias.set(v, __ldg(p.bias + k.c + v) * LOG2E);
-            }
+            const Vf<V> bias = gather<V>([&](int v) { return live && p.bias ? __ldg(p.bias + k.c + v) * LOG2E : 0.f; });
+            Vf<V> z[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) z[r] = sigmoid_neg2(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias));
             tc::mbar_arrive_after_reads(&ring.f_empty[n % G::FSTAGES]);
@@ -849,6 +833,202 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
     if (threadIdx.x == 0) tc::report_fault(ring.ctl.abort_flag, p.fault);
 }
 
+// ------------------------------------------------------------------ backward, tiles moved by TMA
+// As the forward kernel, from the last tile to the first: x, f, dy and the gate in, and the gradients
+// out where x, f and the gate lay.  A thread keeps z of its 16 rows; the states before each row are
+// recomputed four rows at a time from every fourth one, and the gate's sigmoid is taken twice, which
+// costs less than the registers that would hold them.
+struct ScanBackMaps {
+    CUtensorMap x, f, gate, dy, dx, df, dgate;
+};
+
+template <typename T, bool GATE> struct BwdCfg {
+    static constexpr int GROUPS = 2, W = 8, R = SCAN_ROWS / W, V = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int TILE = SCAN_ROWS * 128, STAGE = (GATE ? 4 : 3) * TILE;
+    static constexpr int STAGES = GATE ? 3 : 4, SMEM = STAGES * STAGE + 128;
+    static constexpr int THREADS = (GROUPS * W + 2) * 32;
+};
+
+template <typename T, bool GATE, bool CUT>
+__global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
+    scan_backward_tma(const __grid_constant__ ScanBackMaps maps, const ScanParams p, int tiles) {
+    using G = BwdCfg<T, GATE>;
+    constexpr int W = G::W, R = G::R, V = G::V;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u);
+    __shared__ Scratch<V> scratch[G::GROUPS];
+    __shared__ Run<V> s_fwd[G::GROUPS][W][32];
+    __shared__ Vf<V> s_db[G::GROUPS][W][32];
+    __shared__ Ring<0, G::STAGES> ring;
+    if (test_expired(p)) return;
+    const int lane = threadIdx.x & 31, group = threadIdx.x / (W * 32), warp = (threadIdx.x >> 5) & (W - 1);
+    if (threadIdx.x == 0) ring.init(W * 32, p.fault);
+    __syncthreads();
+    const tc::Ctl ctl{&ring.ctl, nullptr};
+
+    if (group == G::GROUPS) {
+        if (warp == 0 && lane == 0)
+            ring.template produce<V>(p, tiles, G::GROUPS, ctl, [&](int s, int, const Tile &k) {
+                uint8_t *d = smem + s * G::STAGE;
+                const int l = (p.chunks - 1 - k.chunk) * SCAN_ROWS;
+                tc::mbar_expect_tx(&ring.full[s], G::STAGE);
+                tma_load3(d + G::TILE, &maps.f, &ring.full[s], k.c, l, k.b);
+                tma_load3(d, &maps.x, &ring.full[s], k.c, l, k.b);
+                tma_load3(d + 2 * G::TILE, &maps.dy, &ring.full[s], k.c, l, k.b);
+                if (GATE) tma_load3(d + 3 * G::TILE, &maps.gate, &ring.full[s], k.c, l, k.b);
+            });
+        if (warp == 1 && lane == 0)
+            ring.retire(G::GROUPS, ctl, [&](int s, const Tile &k) {
+                const uint8_t *d = smem + s * G::STAGE;
+                const int l = (p.chunks - 1 - k.chunk) * SCAN_ROWS;
+                tma_store3(&maps.dx, d, k.c, l, k.b);
+                tma_store3(&maps.df, d + G::TILE, k.c, l, k.b);
+                if (GATE) tma_store3(&maps.dgate, d + 3 * G::TILE, k.c, l, k.b);
+            });
+    } else {
+        Scratch<V> &sm = scratch[group];
+        auto sync = [&] { tc::named_bar(1 + group, W * 32); };
+        const Vf<V> one = Vf<V>::all(1.f), minus = Vf<V>::all(-1.f), none = Vf<V>::all(0.f);
+        for (uint32_t n = group;; n += G::GROUPS) {
+            const int s = n % G::STAGES;
+            if (!tc::mbar_wait(&ring.full[s], (n / G::STAGES) & 1, ctl, FAULT_CODE + 3)) break;
+            Tile k = ring.tile[s];
+            if (k.chunk < 0) {
+                tc::mbar_arrive(&ring.done[s]);
+                break;
+            }
+            k.c += lane * V;
+            k.word0 += lane * V;
+            const bool live = k.c < p.C;
+            const int chunk = p.chunks - 1 - k.chunk, l0 = chunk * SCAN_ROWS + warp * R, rows = p.L - l0;
+            uint8_t *xs = smem + s * G::STAGE + warp * R * 128 + lane * 4, *fs = xs + G::TILE, *os = xs + 3 * G::TILE;
+            const uint8_t *ds = xs + 2 * G::TILE;
+            const uint32_t cuts = CUT ? reset_mask(p, k.b, l0, R, lane) : 0;
+            const Vf<V> bias = gather<V>([&](int v) { return live && p.bias ? __ldg(p.bias + k.c + v) * LOG2E : 0.f; });
+            Vf<V> start = gather<V>([&](int v) {
+                if (!live) return 0.f;
+                if (chunk > 0) return __uint_as_float(p.states[k.word0 + (int64_t)(chunk - 1) * p.C + v]);
+                return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f;
+            });
+            Vf<V> z[R];
+            // dL/dh_t through y_t; past the end dy was filled with zeros
+            auto into = [&](int r) {
+                Vf<V> v = Word<T>::get(ds + r * 128);
+                if constexpr (GATE) {
+                    const Vf<V> o = Word<T>::get(os + r * 128);
+                    v = mul(v, mul(o, sigmoid(o)));
+                }
+                return v;
+            };
+            auto carry = [&](int r, Vf<V> g) {  // a g of one token
+                if (CUT && (cuts >> r & 1)) return none;
+                return fma(mul(z[r], minus), g, g);
+            };
+            {
+                Vf<V> q = none, h = none, left = one, cc = none;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    z[r] = sigmoid_neg2(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias));
+                    if (r >= rows) z[r] = none;
+                    if (CUT && (cuts >> r & 1)) {
+                        q = one;
+                        h = left = none;
+                    }
+                    const Vf<V> a = fma(z[r], minus, one);
+                    h = fma(a, h, mul(z[r], Word<T>::get(xs + r * 128)));
+                    q = fma(z[r], left, q);
+                    left = mul(left, a);
+                }
+#pragma unroll
+                for (int r = R - 1; r >= 0; --r) cc = carry(r, add(into(r), cc));
+                const Vf<V> nq = mul(q, minus);
+                s_fwd[group][warp][lane] = {nq, h};
+                sm.run[warp][lane] = {nq, cc};
+            }
+            sync();
+            // the carries of the rows right of this warp's; the last warp, which has none, joins the tile's
+            Run<V> run = no_run<V>();
+            {
+                const int mine = W - 1 - warp, upto = mine ? mine : W;
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (i < upto) run = join<CUT>(run, sm.run[W - 1 - i][lane]);
+#pragma unroll
+                for (int w = 0; w < W - 1; ++w)
+                    if (w < warp) start = join<CUT>(start, s_fwd[group][w][lane]);
+            }
+            sync();
+            // in walking order the last warp is the first one
+            const Vf<V> in = chain<CUT, V, W>(
+                p, k, run, sm, W - 1 - warp, lane, live, sync,
+                [&](int v) { return p.dh_last ? p.dh_last[(int64_t)k.b * p.C + k.c + v] : 0.f; },
+                [&](Vf<V> out) {
+                    if (p.dh0) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = out.at(v);
+                    }
+                });
+            Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), db = none, every[R / 4];
+            {
+                Vf<V> h = start;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (r % 4 == 0) every[r / 4] = h;
+                    if (CUT && (cuts >> r & 1)) h = none;
+                    h = advance(h, z[r], Word<T>::get(xs + r * 128));
+                }
+            }
+#pragma unroll
+            for (int r0 = R - 4; r0 >= 0; r0 -= 4) {
+                Vf<V> prev[4], h = every[r0 / 4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (CUT && (cuts >> (r0 + i) & 1)) h = none;
+                    prev[i] = h;
+                    if (i < 3) h = advance(h, z[r0 + i], Word<T>::get(xs + (r0 + i) * 128));
+                }
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    const int r = r0 + i;
+                    const Vf<V> x = Word<T>::get(xs + r * 128), dy = Word<T>::get(ds + r * 128);
+                    Vf<V> g = dy;
+                    if constexpr (GATE) {
+                        const Vf<V> o = Word<T>::get(os + r * 128), sg = sigmoid(o);
+                        g = mul(dy, mul(o, sg));
+                        // silu'(o) = sigmoid(o) (1 + o (1 - sigmoid(o)))
+                        const Vf<V> slope = mul(sg, fma(o, fma(sg, minus, one), one));
+                        Word<T>::put(os + r * 128, mul(mul(dy, advance(prev[i], z[r], x)), slope));
+                    }
+                    g = add(g, cc);
+                    const Vf<V> dx = mul(z[r], g);
+                    cc = carry(r, g);
+                    // a = exp(u) sigmoid(-u): 1 - z would lose a small a
+                    const Vf<V> u = fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias);
+                    const Vf<V> df = mul(mul(dx, mul(each(u, ex2_sat), z[r])), fma(x, minus, prev[i]));
+                    db = add(db, df);
+                    Word<T>::put(xs + r * 128, dx);
+                    Word<T>::put(fs + r * 128, df);
+                }
+            }
+            tc::mbar_arrive_after_reads(&ring.done[s]);
+            if (p.dbias_part) {
+                s_db[group][warp][lane] = db;  // read long before the next tile's
+                sync();
+                if (warp == 0 && live) {
+                    Vf<V> t = none;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) t = add(t, s_db[group][w][lane]);
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = t.at(v);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) tc::report_fault(ring.ctl.abort_flag, p.fault);
+}
+
 // dbias[c] = sum of the tiles' partial sums, in a fixed order: 32 channels a block, 16 warps
 // stride the rows.
 __global__ void __launch_bounds__(512) scan_bias_sum(const float *part, int64_t rows, int C, float *dbias) {
@@ -885,12 +1065,8 @@ __global__ void __launch_bounds__(128) scan_step(const ScanStepParams p) {
     if (p.gate.p) o.load(static_cast<const T *>(p.gate.p) + n * p.gate.sb + c);
     Vf<V> y = Vf<V>::all(0.f);
     if (held) {
-        Vf<V> h = y, bias = y;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h.set(v, p.h_in[row * p.C + c + v]);
-            if (p.bias) bias.set(v, __ldg(p.bias + c + v) * LOG2E);
-        }
+        const Vf<V> bias = gather<V>([&](int v) { return p.bias ? __ldg(p.bias + c + v) * LOG2E : 0.f; });
+        Vf<V> h = gather<V>([&](int v) { return p.h_in[row * p.C + c + v]; });
         h = advance(h, sigmoid_neg2(fma(f.f(), Vf<V>::all(LOG2E), bias)), x.f());
 #pragma unroll
         for (int v = 0; v < V; ++v) p.h_out[row * p.C + c + v] = h.at(v);
@@ -939,6 +1115,34 @@ template <typename T> cudaError_t forward_tma(ScanParams p, int sms, cudaStream_
                    : forward_tma_v<T, false, false>(m, p, (int)tiles, grid, st);
 }
 
+template <typename T, bool GATE, bool CUT>
+cudaError_t backward_tma_v(const ScanBackMaps &maps, const ScanParams &p, int tiles, int grid, cudaStream_t st) {
+    using G = BwdCfg<T, GATE>;
+    cudaError_t e = set_smem_once<scan_backward_tma<T, GATE, CUT>>(G::SMEM);
+    if (e != cudaSuccess) return e;
+    scan_backward_tma<T, GATE, CUT><<<grid, G::THREADS, G::SMEM, st>>>(maps, p, tiles);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t backward_tma(ScanParams p, int sms, cudaStream_t st) {
+    constexpr int V = sizeof(T) == 2 ? 2 : 1;
+    p.ctiles = (p.C + 32 * V - 1) / (32 * V);
+    const int64_t tiles = (int64_t)p.chunks * p.B * p.ctiles;
+    if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
+    ScanBackMaps m;
+    const Blc *from[7] = {&p.x, &p.f, &p.gate, &p.dy, &p.dx, &p.df, &p.dgate};
+    CUtensorMap *to[7] = {&m.x, &m.f, &m.gate, &m.dy, &m.dx, &m.df, &m.dgate};
+    for (int i = 0; i < 7; ++i)
+        if (from[i]->p && !tc::make_blc_map(to[i], from[i]->p, from[i]->sb, from[i]->sl, p.B, p.L, p.C, sizeof(T), SCAN_ROWS))
+            return cudaErrorInvalidValue;
+    const int grid = (int)(tiles < sms ? tiles : sms);
+    if (p.gate.p)
+        return p.reset ? backward_tma_v<T, true, true>(m, p, (int)tiles, grid, st)
+                       : backward_tma_v<T, true, false>(m, p, (int)tiles, grid, st);
+    return p.reset ? backward_tma_v<T, false, true>(m, p, (int)tiles, grid, st)
+                   : backward_tma_v<T, false, false>(m, p, (int)tiles, grid, st);
+}
+
 template <typename T, int V>
 cudaError_t forward_t(ScanParams &p, cudaStream_t st) {
     p.ctiles = (p.C + 32 * V - 1) / (32 * V);
@@ -984,9 +1188,14 @@ cudaError_t launch_gated_scan(ScanParams p, int dtype, int sms, cudaStream_t st)
     return forward_t<__nv_bfloat16, 1>(p, st);
 }
 
-cudaError_t launch_gated_scan_backward(ScanParams p, int dtype, float *dbias, cudaStream_t st) {
+cudaError_t launch_gated_scan_backward(ScanParams p, int dtype, float *dbias, int sms, cudaStream_t st) {
     cudaError_t e;
-    if (dtype == PMA_F32)
+    const int es = dtype == PMA_F32 ? 4 : 2;
+    bool tma = tc::tensor_maps_available() && p.C * es % 4 == 0;
+    for (const Blc *t : {&p.x, &p.f, &p.gate, &p.dy, &p.dx, &p.df, &p.dgate}) tma = tma && boxes(*t, p.B, p.L, es);
+    if (tma)
+        e = dtype == PMA_F32 ? backward_tma<float>(p, sms, st) : backward_tma<__nv_bfloat16>(p, sms, st);
+    else if (dtype == PMA_F32)
         e = backward_t<float, 1>(p, st);
     else if (p.C % 2 == 0 && pairs(p.x) && pairs(p.f) && pairs(p.gate) && pairs(p.dy) && pairs(p.dx) && pairs(p.df) &&
              pairs(p.dgate))

@@ -37,7 +37,7 @@ constexpr int SCAN_ROWS = 128;  // tokens in a tile
 inline int scan_chunks(int L) { return (int)(((int64_t)L + SCAN_ROWS - 1) / SCAN_ROWS); }
 
 cudaError_t launch_gated_scan(ScanParams p, int dtype, int sms, cudaStream_t st);
-cudaError_t launch_gated_scan_backward(ScanParams p, int dtype, float *dbias, cudaStream_t st);
+cudaError_t launch_gated_scan_backward(ScanParams p, int dtype, float *dbias, int sms, cudaStream_t st);
 
 struct ScanStepParams {
     int N, C;

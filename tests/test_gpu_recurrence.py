@@ -195,6 +195,18 @@ def test_extreme_gates_and_values():
     assert torch.isfinite(y[:, 200:]).all() and torch.isfinite(h).all()
 
 
+def test_runs_in_a_thread_without_a_context():
+    """A thread whose first CUDA call is ours (an autograd worker is one)."""
+    import threading
+    a, _, _ = _inputs(1, 100, 64, "f32")
+    want = recurrence.gated_scan(a["x"], a["f"], h0=a["h0"])
+    got = []
+    t = threading.Thread(target=lambda: got.extend(recurrence.gated_scan(a["x"], a["f"], h0=a["h0"])))
+    t.start()
+    t.join()
+    assert len(got) == 2 and all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 def test_runs_on_the_current_stream():
     a, _, _ = _inputs(2, 600, 64, "bf16")
     want = recurrence.gated_scan(a["x"], a["f"], a["bias"], a["gate"], a["h0"])
