@@ -835,9 +835,9 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
 
 // ------------------------------------------------------------------ backward, tiles moved by TMA
 // As the forward kernel, from the last tile to the first: x, f, dy and the gate in, and the gradients
-// out where x, f and the gate lay.  A thread keeps z of its 16 rows; the states before each row are
-// recomputed four rows at a time from every fourth one, and the gate's sigmoid is taken twice, which
-// costs less than the registers that would hold them.
+// out where x, f and the gate lay.  A thread keeps, of its 16 rows, the runs before every fourth one; z,
+// the states and the gate's sigmoid are computed again, four rows at a time, which costs less than the
+// registers that would hold them.
 struct ScanBackMaps {
     CUtensorMap x, f, gate, dy, dx, df, dgate;
 };
@@ -910,7 +910,9 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                 if (chunk > 0) return __uint_as_float(p.states[k.word0 + (int64_t)(chunk - 1) * p.C + v]);
                 return p.h0 ? p.h0[(int64_t)k.b * p.C + k.c + v] : 0.f;
             });
-            Vf<V> z[R];
+            // 2^u of a row, with z of rows past the end zero
+            auto power = [&](int r) { return each(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias), ex2_sat); };
+            auto z_of = [&](int r, Vf<V> e) { return r < rows ? each(add(e, one), rcp) : none; };
             // dL/dh_t through y_t; past the end dy was filled with zeros
             auto into = [&](int r) {
                 Vf<V> v = Word<T>::get(ds + r * 128);
@@ -920,16 +922,17 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                 }
                 return v;
             };
-            auto carry = [&](int r, Vf<V> g) {  // a g of one token
+            auto carry = [&](int r, Vf<V> z, Vf<V> g) {  // a g of one token
                 if (CUT && (cuts >> r & 1)) return none;
-                return fma(mul(z[r], minus), g, g);
+                return fma(mul(z, minus), g, g);
             };
+            Run<V> every[R / 4];  // the run of the rows before every fourth one
             {
-                Vf<V> q = none, h = none, left = one, cc = none;
+                Vf<V> q = none, h = none, left = one, cc = none, z[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    z[r] = sigmoid_neg2(fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias));
-                    if (r >= rows) z[r] = none;
+                    if (r % 4 == 0) every[r / 4] = {mul(q, minus), h};
+                    z[r] = z_of(r, power(r));
                     if (CUT && (cuts >> r & 1)) {
                         q = one;
                         h = left = none;
@@ -940,7 +943,7 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                     left = mul(left, a);
                 }
 #pragma unroll
-                for (int r = R - 1; r >= 0; --r) cc = carry(r, add(into(r), cc));
+                for (int r = R - 1; r >= 0; --r) cc = carry(r, z[r], add(into(r), cc));
                 const Vf<V> nq = mul(q, minus);
                 s_fwd[group][warp][lane] = {nq, h};
                 sm.run[warp][lane] = {nq, cc};
@@ -968,24 +971,17 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                         for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = out.at(v);
                     }
                 });
-            Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), db = none, every[R / 4];
-            {
-                Vf<V> h = start;
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if (r % 4 == 0) every[r / 4] = h;
-                    if (CUT && (cuts >> r & 1)) h = none;
-                    h = advance(h, z[r], Word<T>::get(xs + r * 128));
-                }
-            }
+            Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), db = none;
 #pragma unroll
             for (int r0 = R - 4; r0 >= 0; r0 -= 4) {
-                Vf<V> prev[4], h = every[r0 / 4];
+                Vf<V> prev[4], z[4], e[4], h = r0 ? join<CUT>(start, every[r0 / 4]) : start;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    e[i] = power(r0 + i);
+                    z[i] = z_of(r0 + i, e[i]);
                     if (CUT && (cuts >> (r0 + i) & 1)) h = none;
                     prev[i] = h;
-                    if (i < 3) h = advance(h, z[r0 + i], Word<T>::get(xs + (r0 + i) * 128));
+                    if (i < 3) h = advance(h, z[i], Word<T>::get(xs + (r0 + i) * 128));
                 }
 #pragma unroll
                 for (int i = 3; i >= 0; --i) {
@@ -997,14 +993,13 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                         g = mul(dy, mul(o, sg));
                         // silu'(o) = sigmoid(o) (1 + o (1 - sigmoid(o)))
                         const Vf<V> slope = mul(sg, fma(o, fma(sg, minus, one), one));
-                        Word<T>::put(os + r * 128, mul(mul(dy, advance(prev[i], z[r], x)), slope));
+                        Word<T>::put(os + r * 128, mul(mul(dy, advance(prev[i], z[i], x)), slope));
                     }
                     g = add(g, cc);
-                    const Vf<V> dx = mul(z[r], g);
-                    cc = carry(r, g);
+                    const Vf<V> dx = mul(z[i], g);
+                    cc = carry(r, z[i], g);
                     // a = exp(u) sigmoid(-u): 1 - z would lose a small a
-                    const Vf<V> u = fma(Word<T>::get(fs + r * 128), Vf<V>::all(LOG2E), bias);
-                    const Vf<V> df = mul(mul(dx, mul(each(u, ex2_sat), z[r])), fma(x, minus, prev[i]));
+                    const Vf<V> df = mul(mul(dx, mul(e[i], z[i])), fma(x, minus, prev[i]));
                     db = add(db, df);
                     Word<T>::put(xs + r * 128, dx);
                     Word<T>::put(fs + r * 128, df);
