@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -60,6 +61,7 @@ def build_torch_ops(verbose: bool = True) -> str:
         return TORCH_LIB
     cuda_home = ce.CUDA_HOME or "/usr/local/cuda"
     incs = [f"-I{p}" for p in ce.include_paths("cuda")] + [f"-I{os.path.join(cuda_home, 'include')}"]
+    incs.append(f"-I{sysconfig.get_paths()['include']}")
     libdirs = ce.library_paths("cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"]
@@ -73,7 +75,7 @@ def build_torch_ops(verbose: bool = True) -> str:
     with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
         list(ex.map(lambda so: run(["g++", *flags, *incs, "-c", so[0], "-o", so[1]]), zip(srcs, objs)))
     run(["g++", "-shared", *objs, "-o", TORCH_LIB, *[f"-L{d}" for d in libdirs], f"-L{HERE}", "-lpma", "-lc10",
-         "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lcudart", "-Wl,-rpath,$ORIGIN",
+         "-lc10_cuda", "-ltorch", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lcudart", "-Wl,-rpath,$ORIGIN",
          *[f"-Wl,-rpath,{d}" for d in libdirs]])
     return TORCH_LIB
 

@@ -8,13 +8,22 @@
 //   pma::sample(logits, u, temperature?, top_k?, top_p?, min_p?, t, k, p, m) -> (tokens, logprobs)
 //   pma::fp8_linear(x, wq, ws, out_dtype) -> y
 //
-// A call of one of these costs a few microseconds of host time, against some 20 through ctypes:
-// that is what a small call's time is.  Arguments are checked here; the Python modules
-// (recurrence, sampling, fp8) document them.
+// Arguments are checked here; the Python modules (recurrence, sampling, fp8) document them.
+//
+// The same functions are the Python extension module _pma_torch (this library, imported): a call
+// there skips the dispatcher's argument boxing.  A small call's time is host time: a 64 x 768 step
+// takes 6 us so, 9 through torch.ops, 25 through ctypes.  Calls with anything but plain tensors, or
+// under a dispatch mode, return NotImplemented, and the modules go through torch.ops.
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -371,3 +380,133 @@ TORCH_LIBRARY_IMPL(pma, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(pma, Autograd, m) { m.impl("gated_scan", &gated_scan_autograd); }
+
+// ------------------------------------------------------------------------------ Python extension
+namespace {
+
+// Plain tensors (or None where `optional`) and no dispatch mode: otherwise the dispatcher's business.
+struct Args {
+    PyObject *const *a;
+    bool plain = true;
+    explicit Args(PyObject *const *args) : a(args) { plain = !c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+    const Tensor &tensor(int i) {
+        static const Tensor none;
+        if (!THPVariable_CheckExact(a[i]) && !Py_IS_TYPE(a[i], reinterpret_cast<PyTypeObject *>(ParameterClass))) {
+            plain = false;
+            return none;
+        }
+        return THPVariable_Unpack(a[i]);
+    }
+    OptTensor opt(int i) { return a[i] == Py_None ? OptTensor() : OptTensor(tensor(i)); }
+    double number(int i) {
+        const double v = PyFloat_AsDouble(a[i]);
+        if (v == -1.0 && PyErr_Occurred()) throw python_error();
+        return v;
+    }
+    int64_t whole(int i) {
+        const int64_t v = PyLong_AsLongLong(a[i]);
+        if (v == -1 && PyErr_Occurred()) throw python_error();
+        return v;
+    }
+};
+
+PyObject *wrap(const Tensor &t) { return THPVariable_Wrap(t); }
+PyObject *wrap(const std::tuple<Tensor, Tensor> &t) {
+    THPObjectPtr a(THPVariable_Wrap(std::get<0>(t))), b(THPVariable_Wrap(std::get<1>(t)));
+    return PyTuple_Pack(2, a.get(), b.get());
+}
+PyObject *not_here() { Py_RETURN_NOTIMPLEMENTED; }
+
+bool count_is(Py_ssize_t n, Py_ssize_t want) {
+    if (n == want) return true;
+    PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", want, n);
+    return false;
+}
+
+// gated_scan(x, f, bias, gate, h0, reset)
+PyObject *py_gated_scan(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 6)) return nullptr;
+    Args a(args);
+    const Tensor &x = a.tensor(0), &f = a.tensor(1);
+    const OptTensor bias = a.opt(2), gate = a.opt(3), h0 = a.opt(4), reset = a.opt(5);
+    if (!a.plain) return not_here();
+    auto needs = [](const OptTensor &t) { return t && t->requires_grad(); };
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || f.requires_grad() || needs(bias) || needs(gate) || needs(h0))) {
+        const auto out = ScanFunction::apply(x, f, bias, gate, h0, reset);
+        return wrap(std::make_tuple(out[0], out[1]));
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return wrap(gated_scan(x, f, bias, gate, h0, reset));
+    END_HANDLE_TH_ERRORS
+}
+
+// gated_scan_step(x, f, h, bias, gate) and gated_scan_step_(x, f, h, bias, gate, rows)
+PyObject *py_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 5)) return nullptr;
+    Args a(args);
+    const Tensor &x = a.tensor(0), &f = a.tensor(1), &h = a.tensor(2);
+    const OptTensor bias = a.opt(3), gate = a.opt(4);
+    if (!a.plain) return not_here();
+    at::AutoDispatchBelowADInplaceOrView below;
+    return wrap(gated_scan_step(x, f, h, bias, gate));
+    END_HANDLE_TH_ERRORS
+}
+PyObject *py_step_(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 6)) return nullptr;
+    Args a(args);
+    const Tensor &x = a.tensor(0), &f = a.tensor(1), &h = a.tensor(2);
+    const OptTensor bias = a.opt(3), gate = a.opt(4), rows = a.opt(5);
+    if (!a.plain) return not_here();
+    at::AutoDispatchBelowADInplaceOrView below;
+    return wrap(gated_scan_step_(x, f, h, bias, gate, rows));
+    END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p): each setting a number or a tensor
+PyObject *py_sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 6)) return nullptr;
+    Args a(args);
+    const Tensor &logits = a.tensor(0), &u = a.tensor(1);
+    OptTensor rows[4];
+    double value[4] = {0, 0, 0, 0};
+    int64_t top_k = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (THPVariable_Check(args[2 + i]))
+            rows[i] = a.tensor(2 + i);
+        else if (i == 1)
+            top_k = a.whole(2 + i);
+        else
+            value[i] = a.number(2 + i);
+    }
+    if (!a.plain) return not_here();
+    at::AutoDispatchBelowADInplaceOrView below;
+    return wrap(sample(logits, u, rows[0], rows[1], rows[2], rows[3], value[0], top_k, value[2], value[3]));
+    END_HANDLE_TH_ERRORS
+}
+
+// fp8_linear(x, wq, ws, float32?)
+PyObject *py_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 4)) return nullptr;
+    Args a(args);
+    const Tensor &x = a.tensor(0), &wq = a.tensor(1), &ws = a.tensor(2);
+    if (!a.plain) return not_here();
+    at::AutoDispatchBelowADInplaceOrView below;
+    return wrap(fp8_linear(x, wq, ws, args[3] == Py_True ? at::kFloat : at::kBFloat16));
+    END_HANDLE_TH_ERRORS
+}
+
+#define PMA_FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {PMA_FAST("gated_scan", py_gated_scan), PMA_FAST("gated_scan_step", py_step),
+                         PMA_FAST("gated_scan_step_", py_step_), PMA_FAST("sample", py_sample),
+                         PMA_FAST("fp8_linear", py_fp8_linear), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pma_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject *PyInit__pma_torch(void) { return PyModule_Create(&module); }

@@ -17,7 +17,7 @@ from .ops import _DT, _require_cuda, _stream, check_faults
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
-_fn = None
+_c = None
 
 
 def _blocks(n: int) -> int:
@@ -122,14 +122,20 @@ def matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tenso
 def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] (bf16 or float32, quantised per row and 128 of K inside the call) times w [N, K] -> [..., N]."""
-    global _fn
-    _require_cuda(x, wq, ws)
-    check_faults("fp8.linear")
+    global _c
     if out is None:
-        if _fn is None:
-            torch_ops.load()
-            _fn = torch.ops.pma.fp8_linear.default
-        return _fn(x.detach(), wq, ws, out_dtype)
+        if not torch.compiler.is_compiling() and out_dtype in _DT:
+            if getattr(x, "is_cuda", False):
+                check_faults("fp8.linear")
+            if _c is None:
+                _c = torch_ops.direct()
+            r = _c.fp8_linear(x, wq, ws, out_dtype == torch.float32)
+            if r is not NotImplemented:
+                return r
+        torch_ops.load()
+        _require_cuda(x, wq, ws)
+        return torch.ops.pma.fp8_linear.default(x.detach(), wq, ws, out_dtype)
+    _require_cuda(x, wq, ws)
     if x.dim() != 2:
         raise ValueError("x must be a matrix when out is given")
     return matmul(*quantize(x), wq, ws, out=out)

@@ -24,6 +24,7 @@ from . import torch_ops
 from .ops import _require_cuda, check_faults
 
 _fns = None
+_c = None
 
 
 def _ops():
@@ -36,6 +37,13 @@ def _ops():
     return _fns
 
 
+def _direct():
+    global _c
+    if _c is None:
+        _c = torch_ops.direct()
+    return _c
+
+
 def gated_scan(x: torch.Tensor, f: torch.Tensor, bias: Optional[torch.Tensor] = None,
                gate: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
                reset: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -44,8 +52,13 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, bias: Optional[torch.Tensor] = 
     bias [C] and h0 [B, C] are float32; reset [B, L] (bool or uint8) cuts the state before a token.
     Returns (y [B, L, C] in x's dtype, h_L [B, C] float32).  Differentiable; the backward pass reads
     x, f, gate and one float32 state per channel and 128 tokens.  Gradients repeat bit for bit."""
+    if not torch.compiler.is_compiling():
+        if getattr(x, "is_cuda", False):
+            check_faults("gated_scan")
+        r = _direct().gated_scan(x, f, bias, gate, h0, reset)
+        if r is not NotImplemented:
+            return r
     _require_cuda(x, f)
-    check_faults("gated_scan")
     return _ops()[0](x, f, bias, gate, h0, reset)
 
 
@@ -57,8 +70,14 @@ def gated_scan_step(x: torch.Tensor, f: torch.Tensor, h: torch.Tensor, bias: Opt
     With inplace=True h itself is updated.  With `rows` (int32 [N], distinct) h is a pool [P, C] and
     batch row n advances pool row rows[n] in place; rows outside the pool are skipped (y = 0).
     Inference only."""
+    pool = rows is not None or inplace
+    if not torch.compiler.is_compiling():
+        c = _direct()
+        r = c.gated_scan_step_(x, f, h, bias, gate, rows) if pool else c.gated_scan_step(x, f, h, bias, gate)
+        if r is not NotImplemented:
+            return (r, h) if pool else r
     _require_cuda(x, f, h)
-    if rows is not None or inplace:
+    if pool:
         return _ops()[2](x, f, h, bias, gate, rows), h
     return _ops()[1](x, f, h, bias, gate)
 

@@ -16,7 +16,7 @@ from .ops import _require_cuda
 
 Setting = Union[int, float, torch.Tensor]
 MAX_VOCAB = 360448
-_fn = None
+_c = None
 
 
 @dataclass
@@ -41,11 +41,15 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     min_p times the largest; temperature 0 takes the most likely token.  The logprob is that of the
     token under softmax(logits / temperature) before any cut.  -inf and NaN logits are never taken;
     a row of nothing else gives token -1 and logprob -inf."""
-    global _fn
-    if _fn is None:
-        torch_ops.load()
-        _fn = torch.ops.pma.sample.default
+    global _c
+    if not torch.compiler.is_compiling():
+        if _c is None:
+            _c = torch_ops.direct()
+        r = _c.sample(logits, u, temperature, top_k, top_p, min_p)
+        if r is not NotImplemented:
+            return r
+    torch_ops.load()
     _require_cuda(logits, u)
     rows = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
     t, k, p, m = (v if r is None else 0 for v, r in zip((temperature, top_k, top_p, min_p), rows))
-    return _fn(logits, u, *rows, t, k, p, m)
+    return torch.ops.pma.sample.default(logits, u, *rows, t, k, p, m)

@@ -97,6 +97,14 @@ def load() -> None:
     _loaded = True
 
 
+def direct():
+    """The extension module of the layer operators: the same functions, called without the dispatcher's
+    boxing.  Its functions return NotImplemented for what the dispatcher has to see."""
+    load()
+    from . import _pma_torch
+    return _pma_torch
+
+
 def prefill(q, k, v, decay: torch.Tensor, state=None, eps: float = 1.0, return_state: bool = True):
     """torch.ops.pma.prefill with the library loaded; returns (y, state tuple or None)."""
     load()
