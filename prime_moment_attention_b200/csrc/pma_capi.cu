@@ -144,12 +144,12 @@ struct ScanWs {
     uint32_t *incl(void *ws) const { return reinterpret_cast<uint32_t *>((char *)ws + 256); }
     float *part(void *ws) const { return reinterpret_cast<float *>((char *)ws + part_at); }
     // Every word unwritten (all ones), the counter and the abort flag at -1.
-    cudaError_t arm(ScanParams &p, void *ws, cudaStream_t st) const {
+    cudaError_t arm(ScanParams &p, void *ws, bool needed, cudaStream_t st) const {
         if (chunks <= 1) return cudaSuccess;
         p.counter = reinterpret_cast<int *>(ws);
         p.incl = incl(ws);
         p.agg = reinterpret_cast<unsigned long long *>((char *)ws + runs_at);
-        return cudaMemsetAsync(ws, 0xff, part_at, st);
+        return needed ? cudaMemsetAsync(ws, 0xff, part_at, st) : cudaSuccess;
     }
 };
 
@@ -865,7 +865,8 @@ int pma_gated_scan(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_t
     ScanParams p = scan_params(B, L, C, x, f, gate, bias, h0, reset);
     p.y = blc_of(y);
     p.h_last = h_last;
-    if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
+    const bool words = !scan_by_cluster(B, L, C, x->dtype, di.sms);
+    if ((e = w.arm(p, workspace, words, st)) != cudaSuccess) return cuda_fail(e);
     e = launch_gated_scan(p, x->dtype, di.sms, st);
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
@@ -906,7 +907,8 @@ int pma_gated_scan_backward(int B, int L, int C, const pma_seq_tensor *x, const 
     p.dh0 = dh0;
     p.states = w.nwords && w.chunks > 1 ? w.incl(const_cast<void *>(forward_ws)) : nullptr;
     p.dbias_part = dbias ? w.part(workspace) : nullptr;
-    if ((e = w.arm(p, workspace, st)) != cudaSuccess) return cuda_fail(e);
+    const bool words = !scan_by_cluster(B, L, C, x->dtype, di.sms);
+    if ((e = w.arm(p, workspace, words, st)) != cudaSuccess) return cuda_fail(e);
     e = launch_gated_scan_backward(p, x->dtype, dbias, di.sms, st);
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }

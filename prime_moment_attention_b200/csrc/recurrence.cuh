@@ -36,6 +36,8 @@ struct ScanParams {
 constexpr int SCAN_ROWS = 128;  // tokens in a tile
 inline int scan_chunks(int L) { return (int)(((int64_t)L + SCAN_ROWS - 1) / SCAN_ROWS); }
 
+// One cluster a sequence: the launch needs no words set up.
+bool scan_by_cluster(int B, int L, int C, int dtype, int sms);
 cudaError_t launch_gated_scan(ScanParams p, int dtype, int sms, cudaStream_t st);
 cudaError_t launch_gated_scan_backward(ScanParams p, int dtype, float *dbias, int sms, cudaStream_t st);
 

@@ -381,6 +381,7 @@ __global__ void __launch_bounds__(NW * 32, 2) sample_kernel(const SampleParams p
     T *few = reinterpret_cast<T *>(raw + (sizeof(Shared) + 15) / 16 * 16), *list = few + MAXC * NW * FEW;
     T *seg = p.lists ? list + NW * LIST : few;
     const cg::cluster_group cl = cg::this_cluster();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs
     int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int range = p.range;
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(NW * 32, 2) sample_kernel(const SampleParams p
         }
     }
     __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all of them do: their memory may be written
     if (warp == 0) {
         mx = s.w_max[lane & (NW - 1)];
         float bound = s.w_bound[lane & (NW - 1)];

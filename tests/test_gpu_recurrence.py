@@ -61,6 +61,9 @@ CASES = [
     # more tiles than fit the GPU at once, with and without the strides that TMA takes
     (2, 5000, 1024, "bf16", {"layout": "packed", "reset": True}), (1, 5000, 1024, "f32", {}),
     (2, 3000, 1001, "bf16", {}),
+    # two to eight tiles, as a cluster and otherwise
+    (1, 1024, 64, "bf16", {"reset": True}), (3, 385, 96, "f32", {"gate": False, "reset": True}),
+    (16, 900, 256, "bf16", {"layout": "packed"}), (1, 1025, 64, "bf16", {}),
 ]
 
 
