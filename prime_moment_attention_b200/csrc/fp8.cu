@@ -7,7 +7,9 @@
 // two tensor-memory accumulators, and the epilogue warps read it back, scale it and add it in
 // float32 registers while the tensor core fills the other.  One warp moves tiles by TMA (128-byte
 // swizzle; the tensor map's extents fill ragged edges with zeros, which are zeros in e4m3), one
-// issues the products.
+// issues the products, one copies the scales.  What bounds it is the epilogue: a K block's 128 x 256
+// sums take some 1000 cycles to read, scale and add, against 540 for the products (8192^3: 500 us,
+// 2.2 PFLOP/s).
 //
 // The operand with 128 rows a tile (the tensor core's M) is x for many tokens and w for few: then a
 // tile is 128 weight rows by all the tokens (16 to 128), the weights stream once, and K is split over
@@ -210,6 +212,39 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         "l"(a), "l"(b), "r"(id), "r"(acc)
         : "memory");
 }
+// The same over the CTAs of a pair: 256 rows of A, 128 of each CTA, and 256 of B, 128 of each; every
+// CTA's tensor memory gets its 128 rows of the result.  Issued by the pair's first CTA.
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+// arrives on the barrier at this place in both CTAs once the products so far are complete
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(su32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// the address of this place in the pair's first CTA
+__device__ __forceinline__ uint32_t in_first(const void *p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(su32(p)));
+    return r;
+}
+__device__ __forceinline__ void arrive_in_first(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
+}
+// into this CTA's shared memory, counted on a barrier of the pair's first CTA
+__device__ __forceinline__ void tma_load2_pair(void *dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(su32(dst)),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
 __device__ __forceinline__ void tma_load2(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -267,15 +302,19 @@ __device__ __forceinline__ void store_rows(const uint8_t *s, T *y, int64_t ys, i
     }
 }
 
-// BN: rows of the second operand in a tile; FEW: w is the 128-row operand.
+// BN: rows of the second operand in a tile; FEW: w is the 128-row operand.  BN = 256 runs on pairs of
+// CTAs: a tile of 256 x 256, each CTA with half of both operands in shared memory, which halves what it
+// stages and reads for a product.
 template <int BN, bool FEW> struct Cfg {
+    static constexpr bool PAIR = BN == 256;
+    static constexpr int ROWS = PAIR ? 256 : 128;      // of the first operand in a tile
     static constexpr int EPI = BN == 256 ? 8 : 4;      // epilogue warps: 128 lanes x COLS columns each group of 4
     static constexpr int COLS = BN == 256 ? 128 : BN;  // accumulator columns of a thread
     static constexpr int WARPS = BN == 256 ? 12 : 7;   // and TMA, products, scales
     static constexpr int SLOT = (BN > 128 ? BN : 128) + 4;  // floats: one K block's scales
     static constexpr int THREADS = WARPS * 32;
-    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 4;
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = (PAIR ? BN / 2 : BN) * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN >= 128 ? 6 : 4;
     static constexpr int TCOLS = 2 * BN < 32 ? 32 : 2 * BN;
     // K split: partial sums [BN][128] float32 take the place of the tiles
     static constexpr int SMEM = STAGES * STAGE + 1024;
@@ -309,7 +348,7 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.acc_full[i], 1);
-            mbar_init(&sm.acc_empty[i], G::EPI);
+            mbar_init(&sm.acc_empty[i], G::PAIR ? 2 * G::EPI : G::EPI);  // used in the pair's first CTA
         }
         for (int i = 0; i < SLOTS; ++i) {
             mbar_init(&sm.sc_full[i], 32);
@@ -320,15 +359,26 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
-                     "r"(G::TCOLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (G::PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
+                         "r"(G::TCOLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
+                         "r"(G::TCOLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (G::PAIR)
+        cg::this_cluster().sync();  // both CTAs' barriers are set up
+    else
+        __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
+    const int half = G::PAIR ? (int)cg::this_cluster().block_rank() : 0;
     bool skip = false;
     if (p.test_wait_ns) {  // test hook: a wait expires before any copy or product is issued
         if (tid == 0) expire_test_wait(&sm.never, ctl, p.test_wait_ns, 130);
@@ -338,6 +388,10 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
 
     // Tiles of this CTA (FEW: one, with a share of the K blocks; else every gridDim.x-th).
     int split = 0, splits = 1, first = blockIdx.x, step = gridDim.x;
+    if (G::PAIR) {
+        first = blockIdx.x / 2;
+        step = gridDim.x / 2;
+    }
     if (FEW) {
         const cg::cluster_group cl = cg::this_cluster();
         split = (int)cl.block_rank();
@@ -356,109 +410,129 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
     };
 
     if (warp >= G::EPI) {
-    // registers to the accumulators: 256 x 224 + 128 x 56 = 384 x 168
-    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == G::EPI) {
-        // ------------------------------------------------------------------ TMA
-        if (lane == 0) {
-            // Until the kernel before has written x, load weights only.
-            auto load_w = [&](int s, int j, int ia, int ib) {
-                if (FEW)
-                    tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
-                else
-                    tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
-            };
-            auto load_x = [&](int s, int j, int ia, int ib) {
-                if (FEW)
-                    tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
-                else
-                    tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
-            };
-            uint32_t n = 0;
-            bool ok = true;
-            const int early = first < all ? min(G::STAGES, j1 - j0) : 0;
-            int ia, ib;
-            tile_at(first, ia, ib);
-            for (int i = 0; i < early; ++i) {
-                mbar_expect_tx(&sm.full[i], G::STAGE);
-                load_w(i, j0 + i, ia, ib);
-            }
-            wait_for_x();
-            for (int t = first; ok && t < all; t += step) {
-                tile_at(t, ia, ib);
-                for (int j = j0; j < j1; ++j, ++n) {
-                    const int s = n % G::STAGES;
-                    if (n >= (uint32_t)early) {
-                        if (!(ok = mbar_wait(&sm.empty[s], ((n / G::STAGES) & 1) ^ 1, ctl, 131))) break;
-                        mbar_expect_tx(&sm.full[s], G::STAGE);
-                        load_w(s, j, ia, ib);
+        // registers to the accumulators: 256 x 224 + 128 x 56 = 384 x 168
+        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == G::EPI) {
+            // ------------------------------------------------------------------ TMA
+            if (lane == 0) {
+                // Until the kernel before has written x, load weights only.
+                auto load_w = [&](int s, int j, int ia, int ib) {
+                    if constexpr (G::PAIR)
+                        tma_load2_pair(tiles + s * G::STAGE + G::A_BYTES, &tb, in_first(&sm.full[s]), j * 128, ib * BN + half * 128);
+                    else if (FEW)
+                        tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
+                    else
+                        tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
+                };
+                auto load_x = [&](int s, int j, int ia, int ib) {
+                    if constexpr (G::PAIR)
+                        tma_load2_pair(tiles + s * G::STAGE, &ta, in_first(&sm.full[s]), j * 128, ia * 256 + half * 128);
+                    else if (FEW)
+                        tma_load2(tiles + s * G::STAGE + G::A_BYTES, &tb, &sm.full[s], j * 128, ib * BN);
+                    else
+                        tma_load2(tiles + s * G::STAGE, &ta, &sm.full[s], j * 128, ia * 128);
+                };
+                uint32_t n = 0;
+                bool ok = true;
+                const int early = first < all ? min(G::STAGES, j1 - j0) : 0;
+                int ia, ib;
+                tile_at(first, ia, ib);
+                auto expect = [&](int s) {
+                    if (half == 0) mbar_expect_tx(&sm.full[s], G::PAIR ? 2 * G::STAGE : G::STAGE);
+                };
+                for (int i = 0; i < early; ++i) {
+                    expect(i);
+                    load_w(i, j0 + i, ia, ib);
+                }
+                wait_for_x();
+                for (int t = first; ok && t < all; t += step) {
+                    tile_at(t, ia, ib);
+                    for (int j = j0; j < j1; ++j, ++n) {
+                        const int s = n % G::STAGES;
+                        if (n >= (uint32_t)early) {
+                            if (!(ok = mbar_wait(&sm.empty[s], ((n / G::STAGES) & 1) ^ 1, ctl, 131))) break;
+                            expect(s);
+                            load_w(s, j, ia, ib);
+                        }
+                        load_x(s, j, ia, ib);
                     }
-                    load_x(s, j, ia, ib);
+                }
+                // never leave with copies in flight (a pair's are waited for by its first CTA, whose barriers
+                // count them; the second leaves after it, and where it gave up, after a while)
+                if (half && !ok)
+                    for (const unsigned long long w0 = gtimer(); gtimer() - w0 < 10000000ull;) {
+                    }
+                for (uint32_t i = half ? n : n > G::STAGES ? n - G::STAGES : 0; i < n; ++i) {
+                    const unsigned long long w0 = gtimer();
+                    while (!mbar_try(&sm.full[i % G::STAGES], (i / G::STAGES) & 1) && gtimer() - w0 < WAIT_NS) {
+                    }
                 }
             }
-            // never leave with copies in flight
-            for (uint32_t i = n > G::STAGES ? n - G::STAGES : 0; i < n; ++i) {
-                const unsigned long long w0 = gtimer();
-                while (!mbar_try(&sm.full[i % G::STAGES], (i / G::STAGES) & 1) && gtimer() - w0 < WAIT_NS) {
+        } else if (warp == G::EPI + 1) {
+            // ------------------------------------------------------------------ products
+            if (lane == 0 && half == 0) {
+                constexpr uint32_t ID = idesc_e4m3(G::ROWS, BN);
+                constexpr uint64_t HI = desc_hi(16, 1024, 2);  // K-major rows of 128 bytes, 128-byte swizzle
+                const uint32_t base = su32(tiles) >> 4;
+                uint32_t n = 0;
+                bool ok = true;
+                for (int t = first; ok && t < all; t += step)
+                    for (int j = j0; j < j1; ++j, ++n) {
+                        const int s = n % G::STAGES, a = n & 1;
+                        if (!(ok = mbar_wait(&sm.acc_empty[a], ((n >> 1) & 1) ^ 1, ctl, 132))) break;
+                        if (!(ok = mbar_wait(&sm.full[s], (n / G::STAGES) & 1, ctl, 133))) break;
+                        tc_fence_after();
+                        const uint64_t da = (uint64_t)(base + s * (G::STAGE >> 4)) | HI;
+                        const uint64_t db = (uint64_t)(base + s * (G::STAGE >> 4) + (G::A_BYTES >> 4)) | HI;
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // 32 of K: 32 bytes along the swizzled rows
+                            if constexpr (G::PAIR)
+                                mma_e4m3_pair(tmem + a * BN, da + 2 * k, db + 2 * k, ID, k > 0);
+                            else
+                                mma_e4m3(tmem + a * BN, da + 2 * k, db + 2 * k, ID, k > 0);
+                        }
+                        if constexpr (G::PAIR) {
+                            commit_pair(&sm.empty[s]);
+                            commit_pair(&sm.acc_full[a]);
+                        } else {
+                            commit(&sm.empty[s]);
+                            commit(&sm.acc_full[a]);
+                        }
+                    }
+                // every product issued is complete before tensor memory is freed
+                for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) {
+                    const unsigned long long w0 = gtimer();
+                    while (!mbar_try(&sm.acc_full[i & 1], (i >> 1) & 1) && gtimer() - w0 < WAIT_NS) {
+                    }
                 }
             }
-        }
-    } else if (warp == G::EPI + 1) {
-        // ------------------------------------------------------------------ products
-        if (lane == 0) {
-            constexpr uint32_t ID = idesc_e4m3(128, BN);
-            constexpr uint64_t HI = desc_hi(16, 1024, 2);  // K-major rows of 128 bytes, 128-byte swizzle
-            const uint32_t base = su32(tiles) >> 4;
+        } else if (warp == G::EPI + 2) {
+            // ------------------------------------------------------------------ scales
+            // of a K block: x's rows of the tile, then w's blocks
+            constexpr int ROWS = FEW ? BN : 128;
+            wait_for_x();
             uint32_t n = 0;
             bool ok = true;
-            for (int t = first; ok && t < all; t += step)
+            for (int t = first; ok && t < all; t += step) {
+                int ia, ib;
+                tile_at(t, ia, ib);
+                const int m0 = FEW ? ib * BN : ia * G::ROWS + half * 128, n0 = FEW ? ia : ib * (BN / 128);
                 for (int j = j0; j < j1; ++j, ++n) {
-                    const int s = n % G::STAGES, a = n & 1;
-                    if (!(ok = mbar_wait(&sm.acc_empty[a], ((n >> 1) & 1) ^ 1, ctl, 132))) break;
-                    if (!(ok = mbar_wait(&sm.full[s], (n / G::STAGES) & 1, ctl, 133))) break;
-                    tc_fence_after();
-                    const uint64_t da = (uint64_t)(base + s * (G::STAGE >> 4)) | HI;
-                    const uint64_t db = (uint64_t)(base + s * (G::STAGE >> 4) + (G::A_BYTES >> 4)) | HI;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)  // 32 of K: 32 bytes along the swizzled rows
-                        mma_e4m3(tmem + a * BN, da + 2 * k, db + 2 * k, ID, k > 0);
-                    commit(&sm.empty[s]);
-                    commit(&sm.acc_full[a]);
-                }
-            // every product issued is complete before tensor memory is freed
-            for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) {
-                const unsigned long long w0 = gtimer();
-                while (!mbar_try(&sm.acc_full[i & 1], (i >> 1) & 1) && gtimer() - w0 < WAIT_NS) {
+                    const int s = n % SLOTS;
+                    if (!(ok = mbar_wait(&sm.sc_empty[s], ((n / SLOTS) & 1) ^ 1, ctl, 135))) break;
+    #pragma unroll
+                    for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+                        const int r = i * 32 + lane;
+                        if (r < ROWS) copy4(&scales[s][r], p.x.scale + (int64_t)min(m0 + r, p.M - 1) * p.x.si + j * p.x.sj);
+                    }
+                    if (lane < (FEW ? 1 : BN / 128))
+                        copy4(&scales[s][G::SLOT - 4 + lane],
+                              p.w.scale + (int64_t)min(n0 + lane, (p.N - 1) / 128) * p.w.si + j * p.w.sj);
+                    copies_arrive(&sm.sc_full[s]);
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-    } else if (warp == G::EPI + 2) {
-        // ------------------------------------------------------------------ scales
-        // of a K block: x's rows of the tile, then w's blocks
-        constexpr int ROWS = FEW ? BN : 128;
-        wait_for_x();
-        uint32_t n = 0;
-        bool ok = true;
-        for (int t = first; ok && t < all; t += step) {
-            int ia, ib;
-            tile_at(t, ia, ib);
-            const int m0 = FEW ? ib * BN : ia * 128, n0 = FEW ? ia : ib * (BN / 128);
-            for (int j = j0; j < j1; ++j, ++n) {
-                const int s = n % SLOTS;
-                if (!(ok = mbar_wait(&sm.sc_empty[s], ((n / SLOTS) & 1) ^ 1, ctl, 135))) break;
-#pragma unroll
-                for (int i = 0; i < (ROWS + 31) / 32; ++i) {
-                    const int r = i * 32 + lane;
-                    if (r < ROWS) copy4(&scales[s][r], p.x.scale + (int64_t)min(m0 + r, p.M - 1) * p.x.si + j * p.x.sj);
-                }
-                if (lane < (FEW ? 1 : BN / 128))
-                    copy4(&scales[s][G::SLOT - 4 + lane],
-                          p.w.scale + (int64_t)min(n0 + lane, (p.N - 1) / 128) * p.w.si + j * p.w.sj);
-                copies_arrive(&sm.sc_full[s]);
-            }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    }
     } else {
         if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ------------------------------------------------------------------ sums, output
@@ -469,42 +543,56 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         for (int t = first; ok && t < all; t += step) {
             int ia, ib;
             tile_at(t, ia, ib);
-            const int ra = ia * 128 + row, cb = ib * BN + col0;  // this thread's row and first column
+            const int ra = ia * G::ROWS + half * 128 + row, cb = ib * BN + col0;  // this thread's row and first column
             unsigned long long acc[G::COLS / 2];
 #pragma unroll
             for (int i = 0; i < G::COLS / 2; ++i) acc[i] = 0ull;
-            for (int j = j0; j < j1; ++j, ++n) {
+            // CH columns are read while the CH before them are scaled, across K blocks too: a read's
+            // latency, not its bandwidth, is what it costs
+            constexpr int CH = G::COLS == 128 ? 32 : 16, NC = G::COLS / CH;
+            uint32_t d[2][CH];
+            auto open = [&](uint32_t(&to)[CH]) {  // the next K block's products, its first columns on their way
+                ok = mbar_wait(&sm.acc_full[n & 1], (n >> 1) & 1, ctl, 134);
+                tc_fence_after();
+                if (ok) tmem_issue(mine + (n & 1) * BN, to);
+            };
+            if (!FEW && j0 < j1) open(d[0]);
+            for (int j = j0; ok && j < j1; ++j) {
                 const int a = n & 1, sl = n % SLOTS;
                 if (!(ok = mbar_wait(&sm.sc_full[sl], (n / SLOTS) & 1, ctl, 136))) break;
                 const float *sx = scales[sl];
                 const float s = FEW ? sx[G::SLOT - 4] : sx[row] * sx[G::SLOT - 4 + col0 / 128];
-                if (!(ok = mbar_wait(&sm.acc_full[a], (n >> 1) & 1, ctl, 134))) break;
-                tc_fence_after();
-                // CH columns are read while the CH before them are scaled: a read's latency, not its
-                // bandwidth, is what it costs
-                constexpr int CH = G::COLS == 128 ? 32 : 16;
-                uint32_t d[2][CH];
-                tmem_issue(mine + a * BN, d[0]);
+                const unsigned long long sp = pair(s);
+                if (FEW) {  // not ahead: registers for two CTAs an SM matter more
+                    open(d[0]);
+                    if (!ok) break;
+                }
+                ++n;
 #pragma unroll
-                for (int c = 0; c < G::COLS; c += CH) {
-                    uint32_t(&v)[CH] = d[(c / CH) & 1];
+                for (int c = 0; c < NC; ++c) {
+                    uint32_t(&v)[CH] = d[NC % 2 ? 0 : c & 1];
                     tmem_wait_ld_regs(v);
-                    if (c + CH < G::COLS) {
-                        tmem_issue(mine + a * BN + c + CH, d[(c / CH & 1) ^ 1]);
+                    if (c + 1 < NC) {
+                        tmem_issue(mine + a * BN + (c + 1) * CH, d[(c + 1) & 1]);
                     } else {  // all columns are in registers
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sm.acc_empty[a]);
+                        if (lane == 0) {
+                            if constexpr (G::PAIR)
+                                arrive_in_first(&sm.acc_empty[a]);
+                            else
+                                mbar_arrive(&sm.acc_empty[a]);
+                        }
+                        if (!FEW && j + 1 < j1) open(d[0]);
                     }
-                    const unsigned long long sp = pair(s);
 #pragma unroll
                     for (int i = 0; i < CH; i += 2) {
                         unsigned long long x2 = sp;
                         if (FEW) {
-                            x2 = *reinterpret_cast<const unsigned long long *>(sx + c + i);
+                            x2 = *reinterpret_cast<const unsigned long long *>(sx + c * CH + i);
                             asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x2) : "l"(sp));
                         }
-                        fma2(acc[(c + i) / 2], v[i], v[i + 1], x2);
+                        fma2(acc[(c * CH + i) / 2], v[i], v[i + 1], x2);
                     }
                 }
                 __syncwarp();
@@ -590,10 +678,17 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         cl.sync();
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (G::PAIR)
+        cg::this_cluster().sync();  // nothing of the other CTA reaches this one's memory any more
+    else
+        __syncthreads();
     tc_fence_after();
-    if (warp == 0)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TCOLS) : "memory");
+    if (warp == 0) {
+        if constexpr (G::PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TCOLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TCOLS) : "memory");
+    }
     if (tid == 0) report_fault(sm.ctl.abort_flag, p.fault);
 }
 
@@ -602,9 +697,9 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, bool aft
     const Fp8Rows &a = FEW ? p.w : p.x, &b = FEW ? p.x : p.w;
     const int ra = FEW ? p.N : p.M, rb = FEW ? p.M : p.N;
     CUtensorMap ta, tb;
-    if (!make_map_2d_u8(&ta, a.q, ra, p.K, a.stride, 128) || !make_map_2d_u8(&tb, b.q, rb, p.K, b.stride, BN))
+    if (!make_map_2d_u8(&ta, a.q, ra, p.K, a.stride, 128) || !make_map_2d_u8(&tb, b.q, rb, p.K, b.stride, G::PAIR ? BN / 2 : BN))
         return cudaErrorInvalidValue;
-    p.tiles_a = (ra + 127) / 128;
+    p.tiles_a = (ra + G::ROWS - 1) / G::ROWS;
     p.tiles_b = (rb + BN - 1) / BN;
     const int64_t tiles = (int64_t)p.tiles_a * p.tiles_b;
     if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
@@ -614,13 +709,14 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, bool aft
     if (FEW)  // K over a cluster while SMs would idle and a CTA keeps two K blocks
         while (splits < 8 && tiles * splits * 2 <= sms && p.blocks >= splits * 4) splits *= 2;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(FEW ? tiles * splits : (tiles < sms ? tiles : sms)));
+    const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+    cfg.gridDim = dim3((unsigned)(FEW ? tiles * splits : G::PAIR ? 2 * pairs : (tiles < sms ? tiles : sms)));
     cfg.blockDim = dim3(G::THREADS);
     cfg.dynamicSmemBytes = G::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)splits;
+    at[0].val.clusterDim.x = G::PAIR ? 2 : (unsigned)splits;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
@@ -678,9 +774,9 @@ cudaError_t launch_fp8_matmul(Fp8Params p, int sms, bool after_quantize, cudaStr
     if (p.M <= 16) return matmul_t<16, true>(p, sms, after_quantize, st);
     if (p.M <= 32) return matmul_t<32, true>(p, sms, after_quantize, st);
     if (p.M <= 64) return matmul_t<64, true>(p, sms, after_quantize, st);
-    // 256 columns halve the re-reads of x, once that leaves a tile for every SM
-    const int64_t wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256);
-    if (wide >= sms) return matmul_t<256, false>(p, sms, after_quantize, st);
+    // tiles of 256 x 256 on pairs of CTAs, once that leaves a tile for every pair
+    const int64_t wide = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+    if (wide >= sms / 2) return matmul_t<256, false>(p, sms, after_quantize, st);
     return matmul_t<128, false>(p, sms, after_quantize, st);
 }
 
