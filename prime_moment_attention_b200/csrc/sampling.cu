@@ -178,11 +178,12 @@ template <typename T> struct Sampler {
     static constexpr int VEC = Row<T>::VEC;
     Shared &s;
     const T *seg;       // NW * range tokens
-    T *list;            // [NW][LIST] this CTA's candidates, by index
+    T *list;            // [NW][list_stride] this CTA's candidates, by index
     cg::cluster_group cl;
     int nc, rank, warp, lane, range;
     int listed;      // logits in this warp's list; -1: none made, or they do not fit
     float list_low;  // it holds those from here on
+    int list_stride;
     uint32_t slice_count;  // this CTA's slice of the last merged histogram
     unsigned long long slice_weight;
 
@@ -253,10 +254,11 @@ template <typename T> struct Sampler {
     // The logits that are at least `low` and not masked, from the list where it has them all.
     template <typename F> __device__ __forceinline__ void each_from(float low, F f) const {
         if (listed >= 0 && low >= list_low) {
+            const T *w = list + warp * list_stride;
 #pragma unroll 1
             for (int i = lane; i < listed; i += 32) {
-                const float x = Row<T>::one(list[warp * LIST + i]);
-                if (x >= low) f(x);
+                const float x = Row<T>::one(w[i]);
+                if (x >= low && x > -INFINITY) f(x);
             }
             return;
         }
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(NW * 32, 2) sample_kernel(const SampleParams p
     int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int range = p.range;
-    Sampler<T> S{s, seg, list, cl, nc, rank, warp, lane, range, -1, 0.f, 0, 0};
+    Sampler<T> S{s, seg, list, cl, nc, rank, warp, lane, range, -1, 0.f, LIST, 0, 0};
 
     // ---- the row into shared memory, its maximum, and the top-k bound
     const int first = (rank * NW + warp) * range;  // this warp's tokens of the row
@@ -587,7 +589,9 @@ __global__ void __launch_bounds__(NW * 32, 2) sample_kernel(const SampleParams p
                 S.seg = seg = few;
                 S.nc = nc = 1;
                 S.range = range = row_ranges * FEW / NW;
-                S.listed = -1;
+                S.list = few;
+                S.list_stride = S.listed = range;
+                S.list_low = -INFINITY;
                 alone = true;
             }
         }
