@@ -28,9 +28,10 @@
  *     pma_set_fault_word (and the test hook pma_test_expire_waits); and the
  *     static scratch buffer of pma_prefill_no_alloc with its per-device,
  *     per-context cache of the buffer's address.
- *   - Kernels that wait (the tensor-core prefills) bound every wait; a wait that
- *     expires stops the launch early with unwritten outputs and records a nonzero
- *     code in the workspace status word and in the registered fault word.
+ *   - Kernels that wait (the tensor-core prefills, the recurrence's tiles, the 8-bit
+ *     product) bound every wait; a wait that expires stops the launch early with
+ *     unwritten (of the recurrence: void) outputs and records a nonzero code in the
+ *     registered fault word, the prefills also in the workspace status word.
  *   - Sequence tensors (q, k, v, y) are [B, H, L, D] with arbitrary element
  *     strides on B, H, L and a contiguous D axis, so both the reference's
  *     [B,H,L,D] tensors and its transposed views of [B,L,H,D] projections
