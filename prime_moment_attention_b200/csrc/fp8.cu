@@ -13,7 +13,8 @@
 //
 // The operand with 128 rows a tile (the tensor core's M) is x for many tokens and w for few: then a
 // tile is 128 weight rows by all the tokens (16 to 128), the weights stream once, and K is split over
-// a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order.
+// a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order.  64 x 32000 x 768:
+// 10.9 us, against 3.8 for its bytes: latency of set-up, six K blocks and the stores.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -137,6 +138,8 @@ template <typename E> __device__ __forceinline__ uint2 quant8(const E &x, const 
 // Lets the product that follows in the stream start: it waits for this grid before it reads q.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Bound by instructions, some 13 an element: 8192 x 8192 bf16 in 62 us, 3.3 TB/s (with a division an
+// element 71).
 // 16 lanes a block of 128; a lane group takes GROUPS neighbouring blocks of a row (its loads in flight
 // together).
 template <typename T, int GROUPS>

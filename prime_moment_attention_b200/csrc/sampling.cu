@@ -22,7 +22,12 @@
 //     top-p   the tokens below z weigh less than V exp(z): those with V exp(z) <= (1 - p) W are cut;
 //             the weight below two values of z is measured with W itself
 // The kept weights are then summed by ranges of consecutive tokens, one a warp; the warp whose
-// range holds the goal walks it.
+// range holds the goal walks it.  Where the candidates of a row are few, the cluster's first CTA goes on
+// with them alone.
+//
+// Bound by instructions (some 25 a logit for its weight) in a large batch: 256 x 131072 bf16 take 63 us
+// without filters, 104 with top-p 0.95, of 10.3 that the bytes need; by the latency of its phases in a
+// small one: a row of 32000 with top-k 50 takes 15.5 us.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"

@@ -54,6 +54,13 @@ void check_cuda(const Tensor &t, const char *name) {
     TORCH_CHECK(t.is_cuda(), "pma: ", name, " must be a CUDA tensor (no CPU fallback)");
 }
 
+// The operators without a gradient say so instead of dropping it.
+void check_no_grad(const char *fn, std::initializer_list<const Tensor *> ts) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor *t : ts)
+        TORCH_CHECK(!t->requires_grad(), fn, " is inference-only: run under torch.no_grad() or torch.inference_mode()");
+}
+
 void check_like(const Tensor &t, const char *name, at::IntArrayRef shape, at::ScalarType dtype, const at::Device &dev) {
     TORCH_CHECK_VALUE(t.sizes() == shape && t.scalar_type() == dtype && t.device() == dev, name, " must be a ", dtype,
                       " tensor of shape ", shape, " on ", dev, "; got ", t.scalar_type(), " ", t.sizes(), " on ",
@@ -261,6 +268,7 @@ Tensor step_into(const Tensor &x_in, const Tensor &f_in, const Tensor &h_in, con
 std::tuple<Tensor, Tensor> gated_scan_step(const Tensor &x, const Tensor &f, const Tensor &h, const OptTensor &bias,
                                            const OptTensor &gate) {
     check_common(x, f, bias, gate, 2);
+    check_no_grad("gated_scan_step", {&x, &f, &h});
     check_like(h, "h", x.sizes(), at::kFloat, x.device());
     const Tensor in = h.contiguous();
     Tensor out = at::empty_like(in);
@@ -271,6 +279,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor &x, const Tensor &f, con
 Tensor gated_scan_step_(const Tensor &x, const Tensor &f, const Tensor &h, const OptTensor &bias, const OptTensor &gate,
                         const OptTensor &rows) {
     check_common(x, f, bias, gate, 2);
+    check_no_grad("gated_scan_step", {&x, &f, &h});
     if (rows) {
         check_like(*rows, "rows", {x.size(0)}, at::kInt, x.device());
         TORCH_CHECK_VALUE(h.dim() == 2, "h must be [pool rows, channels]");
@@ -317,6 +326,7 @@ Tensor fp8_linear(const Tensor &x_in, const Tensor &wq_in, const Tensor &ws_in, 
     check_cuda(x_in, "x");
     check_cuda(wq_in, "wq");
     check_cuda(ws_in, "ws");
+    check_no_grad("fp8_linear", {&x_in});
     TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.size(-1) > 0, "x must have at least one column; got ", x_in.sizes());
     const at::Device dev = x_in.device();
     const int dtype = dtype_of(x_in);

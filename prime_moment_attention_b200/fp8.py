@@ -134,7 +134,7 @@ def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out_dtype: torch
                 return r
         torch_ops.load()
         _require_cuda(x, wq, ws)
-        return torch.ops.pma.fp8_linear.default(x.detach(), wq, ws, out_dtype)
+        return torch.ops.pma.fp8_linear.default(x, wq, ws, out_dtype)
     _require_cuda(x, wq, ws)
     if x.dim() != 2:
         raise ValueError("x must be a matrix when out is given")

@@ -39,7 +39,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     (float32; int32 for top_k).  Tokens are ordered by (logit descending, index ascending) and cut
     by top_k, then by the smallest prefix that holds top_p of what is left, then by probability
     min_p times the largest; temperature 0 takes the most likely token.  The logprob is that of the
-    token under softmax(logits / temperature) before any cut.  -inf and NaN logits are never taken;
+    token under softmax(logits / temperature) before any cut; it carries no gradient.  -inf and NaN logits are never taken;
     a row of nothing else gives token -1 and logprob -inf."""
     global _c
     if not torch.compiler.is_compiling():

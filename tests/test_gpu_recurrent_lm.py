@@ -157,6 +157,18 @@ def test_compile_sees_the_operators(L):
         assert torch.equal(want, torch.compile(f, backend="aot_eager", fullgraph=True)(x, b))
 
 
+def test_calls_without_a_gradient_refuse_to_drop_it():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    h = torch.zeros(4, 64, device="cuda")
+    q, s = fp8.quantize_weight(torch.randn(32, 64, device="cuda"))
+    for call in (lambda: fp8.linear(x, q, s), lambda: recurrence.gated_scan_step(x, x, h),
+                 lambda: recurrence.gated_scan_step(x, x, h, inplace=True)):
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 def test_second_derivatives_are_refused():
     x = torch.randn(1, 10, 8, device="cuda", requires_grad=True)
     y, _ = recurrence.gated_scan(x, x)
