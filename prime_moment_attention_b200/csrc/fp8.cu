@@ -13,7 +13,8 @@
 //
 // The operand with 128 rows a tile (the tensor core's M) is x for many tokens and w for few: then a
 // tile is 128 weight rows by all the tokens (16 to 128), the weights stream once, and K is split over
-// a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order.  64 x 32000 x 768:
+// a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order (so it is for few
+// tiles of many tokens and a long K).  64 x 32000 x 768:
 // 10.9 us, against 3.8 for its bytes: latency of set-up, six K blocks and the stores.
 #include <cooperative_groups.h>
 
@@ -389,18 +390,20 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
         skip = ctl.aborted();
     }
 
-    // Tiles of this CTA (FEW: one, with a share of the K blocks; else every gridDim.x-th).
+    // Tiles of this CTA: one, with a share of the K blocks, or every gridDim.x-th.
     int split = 0, splits = 1, first = blockIdx.x, step = gridDim.x;
     if (G::PAIR) {
         first = blockIdx.x / 2;
         step = gridDim.x / 2;
     }
-    if (FEW) {
+    if (!G::PAIR) {
         const cg::cluster_group cl = cg::this_cluster();
         split = (int)cl.block_rank();
         splits = (int)cl.num_blocks();
-        first = blockIdx.x / splits;
-        step = p.tiles_a * p.tiles_b;
+        if (FEW || splits > 1) {
+            first = blockIdx.x / splits;
+            step = p.tiles_a * p.tiles_b;
+        }
     }
     const int all = skip ? 0 : p.tiles_a * p.tiles_b;
     const int j0 = (int)((int64_t)p.blocks * split / splits), j1 = (int)((int64_t)p.blocks * (split + 1) / splits);
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
                 if (lane == 0) mbar_arrive(&sm.sc_empty[sl]);
             }
             if (!ok) break;
-            if (FEW && splits > 1) {
+            if (!G::PAIR && splits > 1) {
                 float *part = reinterpret_cast<float *>(tiles);
 #pragma unroll
                 for (int i = 0; i < G::COLS; ++i) part[i * 128 + row] = half_of(acc[i / 2], i & 1);
@@ -658,20 +661,23 @@ __global__ void __launch_bounds__(Cfg<BN, FEW>::THREADS, FEW ? 2 : 1)
             }
         }
     }
-    if (FEW && splits > 1) {
+    if (!G::PAIR && splits > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();  // every CTA's partial sums are in its shared memory
         if (!skip && !ctl.aborted() && tid < 128) {
             int ia, ib;
             tile_at(first, ia, ib);
-            const int nrow = ia * 128 + tid;
-            for (int i = split; i < BN; i += splits) {
-                const int m = ib * BN + i;
-                if (m >= p.M || nrow >= p.N) break;
+            const int r = ia * 128 + tid;  // of the 128-row operand
+            // this CTA's columns: neighbouring ones where a thread's row is a row of y
+            const int each = BN / splits, c0 = FEW ? split : split * each, dc = FEW ? splits : 1;
+            const int rows = FEW ? p.N : p.M, cols = FEW ? p.M : p.N;
+            for (int n = 0; n < each; ++n) {
+                const int i = c0 + n * dc, c = ib * BN + i;
+                if (c >= cols || r >= rows) break;
                 float v = 0.f;
-                for (int r = 0; r < splits; ++r)
-                    v += cl.map_shared_rank(reinterpret_cast<float *>(tiles), r)[i * 128 + tid];
-                const int64_t at = (int64_t)m * p.ys + nrow;
+                for (int q = 0; q < splits; ++q)
+                    v += cl.map_shared_rank(reinterpret_cast<float *>(tiles), q)[i * 128 + tid];
+                const int64_t at = FEW ? (int64_t)c * p.ys + r : (int64_t)r * p.ys + c;
                 if (p.y_f32)
                     static_cast<float *>(p.y)[at] = v;
                 else
@@ -709,11 +715,11 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, bool aft
     cudaError_t e = set_smem_once<fp8_matmul_kernel<BN, FEW>>(G::SMEM);
     if (e != cudaSuccess) return e;
     int splits = 1;
-    if (FEW)  // K over a cluster while SMs would idle and a CTA keeps two K blocks
+    if (!G::PAIR)  // K over a cluster while SMs would idle and a CTA keeps two K blocks
         while (splits < 8 && tiles * splits * 2 <= sms && p.blocks >= splits * 4) splits *= 2;
     cudaLaunchConfig_t cfg{};
     const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-    cfg.gridDim = dim3((unsigned)(FEW ? tiles * splits : G::PAIR ? 2 * pairs : (tiles < sms ? tiles : sms)));
+    cfg.gridDim = dim3((unsigned)(FEW || splits > 1 ? tiles * splits : G::PAIR ? 2 * pairs : (tiles < sms ? tiles : sms)));
     cfg.blockDim = dim3(G::THREADS);
     cfg.dynamicSmemBytes = G::SMEM;
     cfg.stream = st;
@@ -777,9 +783,13 @@ cudaError_t launch_fp8_matmul(Fp8Params p, int sms, bool after_quantize, cudaStr
     if (p.M <= 16) return matmul_t<16, true>(p, sms, after_quantize, st);
     if (p.M <= 32) return matmul_t<32, true>(p, sms, after_quantize, st);
     if (p.M <= 64) return matmul_t<64, true>(p, sms, after_quantize, st);
-    // tiles of 256 x 256 on pairs of CTAs, once that leaves a tile for every pair
-    const int64_t wide = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
-    if (wide >= sms / 2) return matmul_t<256, false>(p, sms, after_quantize, st);
+    // 256 x 256 on pairs of CTAs where its rounds of tiles take less: a round takes some 1.45 times as long
+    // as one of 128 x 128 tiles, of half the work an SM (8192^3: 14 in 511 us, 28 in 706)
+    const int64_t pairs = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int64_t singles = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128);
+    const int64_t slots = sms / 2;
+    if (20 * ((singles + sms - 1) / sms) >= 29 * ((pairs + slots - 1) / slots))
+        return matmul_t<256, false>(p, sms, after_quantize, st);
     return matmul_t<128, false>(p, sms, after_quantize, st);
 }
 

@@ -82,7 +82,8 @@ def test_quantisation_is_bit_exact(M, K, dtype):
 
 SIZES = [(1, 1, 1), (1, 768, 2048), (2, 130, 128), (16, 128, 4096), (17, 100, 300), (32, 1000, 640), (50, 3000, 768),
          (64, 32000, 768), (65, 129, 257), (128, 128, 128), (129, 257, 1000), (200, 64, 5000), (777, 1530, 1000),
-         (1024, 2048, 768), (2500, 2300, 512), (4096, 2560, 384), (8, 64, 8192)]
+         (1024, 2048, 768), (2500, 2300, 512), (4096, 2560, 384), (8, 64, 8192),
+         (256, 128, 4928), (130, 1000, 2111), (700, 300, 1100)]
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
