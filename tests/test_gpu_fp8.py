@@ -142,3 +142,31 @@ def test_expired_wait_is_reported():
         assert e.value.code == 130
         fp8.linear(x[:m], wq, ws)
         ops.check_faults(synchronize=True)
+
+
+def test_expired_wait_on_pairs_is_reported():
+    x, w = _data(2560, 2304, 256, torch.bfloat16)
+    wq, ws = fp8.quantize_weight(w)
+    ops.check_faults(synchronize=True)
+    _lib.load().pma_test_expire_waits(1_000_000)
+    try:
+        fp8.linear(x, wq, ws)
+    finally:
+        _lib.load().pma_test_expire_waits(0)
+    torch.cuda.synchronize()
+    with pytest.raises(ops.KernelFault) as e:
+        fp8.linear(x, wq, ws)
+    assert e.value.code == 130
+    fp8.linear(x, wq, ws)
+    ops.check_faults(synchronize=True)
+
+
+def test_offsets_past_32_bits():
+    """x of more than 2^31 elements and y of more than 2^32 bytes: the last rows as a call of their own
+    gives them."""
+    M, K, N = 270000, 8192, 8192
+    x = torch.empty(M, K, dtype=torch.bfloat16, device="cuda").normal_()
+    wq, ws = fp8.quantize_weight(torch.randn(N, K, device="cuda"))
+    y = fp8.linear(x, wq, ws)
+    tail = slice(M - 256, M)  # other tiles than the long call's: equal to the order of the sums
+    torch.testing.assert_close(y[tail].float(), fp8.linear(x[tail], wq, ws).float(), rtol=2.0 ** -7, atol=1e-2)

@@ -236,3 +236,25 @@ def test_expired_wait_is_reported():
     assert e.value.code == 120
     recurrence.gated_scan(a["x"], a["f"])
     ops.check_faults(synchronize=True)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements a tensor, forward and backward: the last tokens against a call on them
+    alone that starts from the state before them (and, for the gradient, ends as the long one does)."""
+    B, L, C = 1, 2200000, 1024
+    cut = L - 1000 - (L - 1000) % 128
+    x, f = (torch.empty(B, L, C, dtype=torch.bfloat16, device="cuda").normal_() for _ in range(2))
+    x.requires_grad_()
+    bias = torch.full((C,), 3.0, device="cuda")
+    y, h = recurrence.gated_scan(x, f, bias)
+    dy = torch.ones(1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(B, L, C)
+    (dx,) = torch.autograd.grad([y], [x], [dy])
+    with torch.no_grad():
+        _, before = recurrence.gated_scan(x[:, :cut], f[:, :cut], bias)
+    tail = x[:, cut:].detach().requires_grad_()
+    y2, h2 = recurrence.gated_scan(tail, f[:, cut:], bias, h0=before)
+    (dx2,) = torch.autograd.grad([y2], [tail], [torch.ones_like(y2)])
+    # states within the bar of the module's docstring (values are below 6), rounded to bf16
+    torch.testing.assert_close(h2, h, rtol=0, atol=2e-4)
+    torch.testing.assert_close(y2.float(), y[:, cut:].float(), rtol=2.0 ** -8, atol=2e-4)
+    torch.testing.assert_close(dx2.float(), dx[:, cut:].float(), rtol=2.0 ** -8, atol=2e-4)

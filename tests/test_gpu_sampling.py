@@ -178,3 +178,14 @@ def test_greedy_in_a_graph():
 def test_empty_batch():
     tok, lp = sampling.sample(torch.zeros(0, 10).cuda(), torch.zeros(0).cuda())
     assert tok.shape == (0,) and lp.shape == (0,)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: the last rows as a call of their own gives them."""
+    B, V = 17000, 131072
+    x = torch.empty(B, V, dtype=torch.bfloat16, device="cuda").normal_().mul_(3)
+    u = torch.rand(B, device="cuda")
+    tok, lp = sampling.sample(x, u, top_k=50, top_p=0.9)
+    for b in (0, 16383, 16384, 16999):
+        one = sampling.sample(x[b:b + 1], u[b:b + 1], top_k=50, top_p=0.9)
+        assert one[0] == tok[b] and one[1] == lp[b]
