@@ -170,3 +170,23 @@ def test_offsets_past_32_bits():
     y = fp8.linear(x, wq, ws)
     tail = slice(M - 256, M)  # other tiles than the long call's: equal to the order of the sums
     torch.testing.assert_close(y[tail].float(), fp8.linear(x[tail], wq, ws).float(), rtol=2.0 ** -7, atol=1e-2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("exponent", [-100, -7, 0, 90])
+def test_every_quotient_of_bf16_values(dtype, exponent):
+    """Each pair of an 8-bit significand and an 8-bit largest one, x from amax down to where it rounds to
+    zero, both signs: the bytes of the quotient in 64 bits. (Float32 on the way to e4m3 is harmless: a
+    quotient that is not midway between two e4m3 values is 2^-13 of its size from there.)"""
+    a = torch.arange(128, 256, dtype=torch.float64)[:, None, None, None]
+    down = torch.arange(0, 22, dtype=torch.float64)[None, :, None, None]
+    sign = torch.tensor([1.0, -1.0], dtype=torch.float64)[None, None, :, None]
+    mant = torch.cat([torch.arange(128, 255), torch.arange(129, 256)]).to(torch.float64)
+    x = torch.minimum(mant * 2.0 ** -down, a) * sign                       # (128, 22, 2, 254)
+    lead = a.expand(128, 22, 2, 1)
+    x = torch.cat([lead, x[..., :127], lead, x[..., 127:]], -1).reshape(-1, 256) * 2.0 ** (exponent - 7)
+    amax = (a * 2.0 ** (exponent - 7)).expand(128, 22, 2, 1).reshape(-1, 1)
+    want = (448 * x / amax).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    xq, xs = fp8.quantize(x.to(dtype).cuda())
+    assert torch.equal(xq.view(torch.uint8).cpu(), want)
+    torch.testing.assert_close(xs[:, 0].double().cpu(), amax[:, 0] / 448, rtol=2.0 ** -23, atol=0)
