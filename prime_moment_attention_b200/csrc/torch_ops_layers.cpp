@@ -351,12 +351,14 @@ Tensor fp8_linear(const Tensor &x_in, const Tensor &wq_in, const Tensor &ws_in, 
         wq = at::empty({N, (K + 15) / 16 * 16}, wq_in.options()).narrow(1, 0, K);
         wq.copy_(wq_in);
     }
-    const Tensor ws = kb > 1 && ws_in.stride(1) != 1 ? ws_in.contiguous() : ws_in;
+    // the kernel takes a row stride of at least kb: a broadcast or overlapping view becomes an array of its own
+    const bool as_is = (kb == 1 || ws_in.stride(1) == 1) && (nb == 1 || ws_in.stride(0) >= kb);
+    const Tensor ws = as_is ? ws_in : ws_in.contiguous();
     const int Mi = int_of(M, "rows"), Ni = int_of(N, "outputs"), Ki = int_of(K, "columns");
     const size_t n = pma_fp8_linear_workspace_bytes(Mi, Ki);
     Tensor scratch = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
     check_rc(pma_fp8_linear(Mi, Ni, Ki, x.data_ptr(), x.stride(0), dtype, wq.data_ptr(), wq.stride(0),
-                            ws.data_ptr<float>(), std::max<int64_t>(ws.stride(0), kb), y.data_ptr(), N, dtype_of(y),
+                            ws.data_ptr<float>(), nb == 1 ? kb : ws.stride(0), y.data_ptr(), N, dtype_of(y),
                             scratch.data_ptr(), n, stream_of(dev)),
              "pma_fp8_linear");
     return y;

@@ -109,12 +109,15 @@ def matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tenso
     xq, wq = _rows("xq", xq, K), _rows("wq", wq, K)
     xs = _scales("xs", xs, (M, _blocks(K)), dev)
     ws = _scales("ws", ws, (_blocks(N), _blocks(K)), dev)
-    ws = ws if ws.stride(1) == 1 else ws.contiguous()
+    # the kernel takes a row stride of at least K's blocks: a broadcast or overlapping view becomes an array of its own
+    nb, kb = ws.shape
+    if not ((kb == 1 or ws.stride(1) == 1) and (nb <= 1 or ws.stride(0) >= kb)):
+        ws = ws.contiguous()
     y = _out(out, M, N, out_dtype, dev)
     if N and M:
         _lib.check("pma_fp8_matmul", _lib.load().pma_fp8_matmul(
             M, N, K, xq.data_ptr(), xq.stride(0), xs.data_ptr(), xs.stride(0), xs.stride(1), wq.data_ptr(),
-            wq.stride(0), ws.data_ptr(), max(ws.stride(0), ws.shape[1]), y.data_ptr(), y.stride(0), _DT[y.dtype],
+            wq.stride(0), ws.data_ptr(), kb if nb <= 1 else ws.stride(0), y.data_ptr(), y.stride(0), _DT[y.dtype],
             _stream(dev)))
     return y
 

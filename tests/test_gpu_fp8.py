@@ -190,3 +190,23 @@ def test_every_quotient_of_bf16_values(dtype, exponent):
     xq, xs = fp8.quantize(x.to(dtype).cuda())
     assert torch.equal(xq.view(torch.uint8).cpu(), want)
     torch.testing.assert_close(xs[:, 0].double().cpu(), amax[:, 0] / 448, rtol=2.0 ** -23, atol=0)
+
+
+@pytest.mark.parametrize("M,N,K", [(70, 300, 500), (8, 300, 500), (300, 520, 100), (3, 300, 100), (2600, 2304, 256), (5, 100, 300)])
+def test_scales_of_any_strides(M, N, K):
+    """Scales that are a broadcast (one row for all, one number for all), overlapping, transposed or strided views give
+    what the same numbers give as an array of their own."""
+    x, w = _data(M, N, K, torch.bfloat16)
+    (xq, xs), (wq, _) = fp8.quantize(x), fp8.quantize_weight(w)
+    nb, kb = -(-N // 128), -(-K // 128)
+    g = torch.Generator().manual_seed(5)
+    v = (torch.rand(4 * nb * kb, generator=g) + 0.5).cuda()
+    views = [v[:kb].expand(nb, kb), v[:nb, None].expand(nb, kb), v[:1].expand(nb, kb), v.as_strided((nb, kb), (1, 1)),
+             v.as_strided((nb, kb), (1, nb)), v.as_strided((nb, kb), (2 * kb, 2)), v.as_strided((nb, kb), (kb + 1, 1))]
+    for ws in views:
+        dense = ws.clone(memory_format=torch.contiguous_format)
+        assert torch.equal(fp8.matmul(xq, xs, wq, ws), fp8.matmul(xq, xs, wq, dense))
+        assert torch.equal(fp8.linear(x, wq, ws), fp8.linear(x, wq, dense))
+        _check_product(fp8.linear(x, wq, ws, out_dtype=torch.float32), xq, xs, wq, dense)
+    for one in (xs[:1].expand(M, kb), xs[:, :1].expand(M, kb)):  # and those of x
+        _check_product(fp8.matmul(xq, one, wq, dense), xq, one, wq, dense)
