@@ -8,16 +8,18 @@
 //
 // The time axis is split: a tile is 128 tokens of 32 (or 64) channels, its warps hold consecutive
 // rows and its lanes the channels.  A run of tokens is an affine map of the state that enters it,
-//   h -> h + (H - Q h),   Q = 1 - prod a_t,   H = its result from a zero state,
-// kept as Q rather than as the product: for slow decays 1 - prod a_t is what matters and the
-// product itself would round it away.  A token joins a run by Q <- Q + z (1 - Q), H <- a H + z x.
-// Every input is read once: a tile holds its rows in registers, publishes its (Q, H) as one 64-bit
+//   h -> P h + H = h + (H - Q h),   P = prod a_t,   Q = 1 - P,   H = its result from a zero state,
+// kept as Q where P > 1/2 and as P elsewhere: for slow decays 1 - prod a_t is what matters and the
+// product would round it away; of a state that the run forgets only P h is left, and h + (H - Q h)
+// would keep an ulp of h.  A token joins a run by Q <- Q + z P, P <- a P, H <- a H + z x.
+// Every input is read once: a tile holds its rows in registers, publishes its run as one 64-bit
 // word per channel, gathers the words of the tiles before it back to one that has published the
 // state leaving it, and then writes its outputs.  Words start as all ones (a NaN that no result
 // carries) and are written once, so a word is its own flag and no fence is needed.  A state is
-// always the same chain of joins, tile after tile, however far back a tile looked: results do not
-// depend on timing.  Tiles are handed out in the order of a counter, so a tile only waits for
-// tiles that are already running; every wait is bounded.
+// always the same chain of joins, tile after tile, whether a tile found the state that leaves a
+// neighbour or joined the neighbour's run itself: results do not depend on timing.  A state that is
+// not finite stays so up to a reset.  Tiles are handed out in the order of a counter, so a tile only
+// waits for tiles that are already running; every wait is bounded.
 //
 // Backward, from the right, with the carry c_t = a_t g_t:
 //   g_t = dy_t silu(gate_t) + c_{t+1},   dx = z g,   df = g (h_{t-1} - x) a z,
@@ -128,22 +130,54 @@ template <int V> __device__ __forceinline__ Vf<V> advance(Vf<V> h, Vf<V> z, Vf<V
     return fma(fma(z, Vf<V>::all(-1.f), Vf<V>::all(1.f)), h, mul(z, x));
 }
 
-// A run of tokens: n = -Q and H
+// A run of tokens: H, and in n what it leaves of the state that enters: P > 0 where it is at most 1/2,
+// else -Q (0: an empty run); DROP where the state is dropped whatever it was, NaN and infinities
+// included (a reset, or a state handed on as a run).
+constexpr float DROP = -1.f;
 template <int V> struct Run {
     Vf<V> n, h;
 };
-template <int V> __device__ __forceinline__ Run<V> no_run() { return {Vf<V>::all(0.f), Vf<V>::all(0.f)}; }
-// the state after a run; with CUT, Q = 1 drops the state whatever it was (a reset, or a state handed on)
+// The state after a run.  CUT: the run may drop it; the result of other runs is the same with and without.
 template <bool CUT, int V> __device__ __forceinline__ Vf<V> join(Vf<V> h, const Run<V> &r) {
-    Vf<V> o = add(h, fma(r.n, h, r.h));
-    if (CUT) o = gather<V>([&](int v) { return r.n.at(v) == -1.f ? r.h.at(v) : o.at(v); });
-    return o;
+    const Vf<V> t = fma(r.n, h, r.h), o = add(h, t);
+    return gather<V>([&](int v) {
+        const float n = r.n.at(v), some = n > 0.f ? t.at(v) : o.at(v);
+        return CUT && n == DROP ? r.h.at(v) : some;
+    });
 }
-// run a, then run b
-template <bool CUT, int V> __device__ __forceinline__ Run<V> join(const Run<V> &a, const Run<V> &b) {
-    Run<V> o{fma(b.n, add(a.n, Vf<V>::all(1.f)), a.n), join<CUT>(a.h, b)};
-    if (CUT) o.n = gather<V>([&](int v) { return b.n.at(v) == -1.f ? -1.f : o.n.at(v); });
-    return o;
+// P > 0 or -Q <= 0.  A product that underflows is no drop: 2^-149 of what is not finite is not finite either.
+template <int V> __device__ __forceinline__ Run<V> coded(Vf<V> p, Vf<V> q, Vf<V> h) {
+    return {gather<V>([&](int v) { return p.at(v) <= 0.5f ? fmaxf(p.at(v), __uint_as_float(1u)) : -q.at(v); }), h};
+}
+// A run inside a tile: P to twice the precision, p + e, so that its joins are products and sums alone.
+// Resets are the same for all channels: a part that has one replaces what it joins (the callers' business).
+template <int V> struct Part {
+    Vf<V> p, e, h;
+};
+template <int V> __device__ __forceinline__ Vf<V> minus(Vf<V> a, Vf<V> b) { return fma(b, Vf<V>::all(-1.f), a); }
+template <int V> __device__ __forceinline__ Part<V> part_of(Vf<V> p, Vf<V> q, Vf<V> h) {
+    const Vf<V> one = Vf<V>::all(1.f), hi = minus(one, q), lo = minus(minus(one, hi), q);
+    return {gather<V>([&](int v) { return p.at(v) <= 0.5f ? p.at(v) : hi.at(v); }),
+            gather<V>([&](int v) { return p.at(v) <= 0.5f ? 0.f : lo.at(v); }), h};
+}
+template <int V> __device__ __forceinline__ Part<V> no_part() {
+    return {Vf<V>::all(1.f), Vf<V>::all(0.f), Vf<V>::all(0.f)};
+}
+template <int V> __device__ __forceinline__ Vf<V> join_part(Vf<V> h, const Part<V> &b) { return fma(b.p, h, fma(b.e, h, b.h)); }
+template <int V> __device__ __forceinline__ Part<V> join_part(const Part<V> &a, const Part<V> &b) {
+    const Vf<V> p = mul(a.p, b.p), r = fma(a.p, b.p, mul(p, Vf<V>::all(-1.f)));
+    return {p, fma(a.p, b.e, fma(a.e, b.p, r)), join_part(a.h, b)};
+}
+template <int V> __device__ __forceinline__ Run<V> run_of(const Part<V> &a, bool dropped) {
+    const Vf<V> q = minus(minus(Vf<V>::all(1.f), a.p), a.e);
+    Run<V> r = coded(add(a.p, a.e), each(q, [](float v) { return fmaxf(v, 0.f); }), a.h);
+    if (dropped) r.n = Vf<V>::all(DROP);
+    return r;
+}
+
+// The parts of a tile that have a reset, as a mask
+template <int W> __device__ __forceinline__ uint32_t which_cut(const bool (&cut)[W], int lane) {
+    return __ballot_sync(0xffffffffu, lane < W && cut[lane & (W - 1)]);
 }
 
 // V consecutive channels of one row as one load or store
@@ -218,7 +252,7 @@ __device__ __forceinline__ void get(const unsigned long long *p, unsigned long l
 }
 
 // The runs of V channels of K earlier tiles, at[0 .. K - 1] in the word arrays, or the states leaving
-// them as runs (-1, state); wait for the state where `must_end`, and skip a negative position.
+// them as runs (DROP, state); wait for the state where `must_end`, and skip a negative position.
 template <int V, int K>
 __device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K], const bool (&must_end)[K],
                                       Run<V> (&out)[K]) {
@@ -256,7 +290,7 @@ __device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K
             for (int v = 0; v < V; ++v) {
                 if (got[i][v]) continue;
                 if (s[i][v] != EMPTY) {
-                    n[i][v] = -1.f;
+                    n[i][v] = DROP;
                     h[i][v] = __uint_as_float(s[i][v]);
                     got[i][v] = true;
                 } else if (a[i][v] != ~0ull) {
@@ -278,7 +312,7 @@ __device__ __forceinline__ void fetch(const ScanParams &p, const int64_t (&at)[K
                 for (int i = 0; i < K; ++i)
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        n[i][v] = -1.f;
+                        n[i][v] = DROP;
                         h[i][v] = __uint_as_float(0x7fffffffu);
                     }
                 break;
@@ -429,8 +463,9 @@ __device__ __forceinline__ void load_rows(Pack<T, V> (&d)[R], const Blc &t, int 
 template <typename T, int V, int W, int R, bool GATE, bool CUT, bool CLUSTER>
 __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ Scratch<V> sm;
-    __shared__ Scratch<CLUSTER ? V : 1> peers;  // the other tiles' runs
+    __shared__ Scratch<V> sm;  // the other tiles' runs
+    __shared__ Part<V> parts[W][32];
+    __shared__ bool s_cut[W];
     __shared__ int s_tile;
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -462,27 +497,30 @@ __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const Sca
             if (r >= rows) z[r] = Vf<V>::all(0.f);
     }
     {
-        Vf<V> q = Vf<V>::all(0.f), h = q;
+        Vf<V> q = Vf<V>::all(0.f), h = q, left = Vf<V>::all(1.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (CUT && (cuts >> r & 1)) {
-                q = Vf<V>::all(1.f);
-                h = Vf<V>::all(0.f);
-            }
+            if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
             h = advance(h, z[r], x[r].f());
-            q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
+            q = fma(z[r], left, q);
+            left = mul(left, fma(z[r], Vf<V>::all(-1.f), Vf<V>::all(1.f)));
         }
-        sm.run[warp][lane] = {mul(q, Vf<V>::all(-1.f)), h};
+        parts[warp][lane] = part_of(left, q, h);
+        if (CUT) s_cut[warp] = cuts != 0;
     }
     __syncthreads();
     // the run of the tile's rows before this warp's; warp 0, which has none, joins the whole tile
-    Run<V> run = no_run<V>();
+    Part<V> part = no_part<V>();
     const int upto = warp ? warp : W;
-    for (int w = 0; w < upto; ++w) run = join<CUT>(run, sm.run[w][lane]);
-    __syncthreads();
+    const uint32_t cut = CUT ? which_cut<W>(s_cut, lane) & ((1u << upto) - 1u) : 0;
+    for (int w = 0; w < upto; ++w) {
+        part = join_part(part, parts[w][lane]);
+        if (CUT && (cut >> w & 1)) part.h = parts[w][lane].h;
+    }
+    const Run<V> run = run_of(part, cut);
     const auto join_tiles = [&](auto first, auto last) {
         if constexpr (CLUSTER)
-            return chain_cluster<CUT, V>(p, k, run, peers, warp, lane, live, first, last);
+            return chain_cluster<CUT, V>(p, k, run, sm, warp, lane, live, first, last);
         else
             return chain<CUT, V, W>(p, k, run, sm, warp, lane, live, [] { __syncthreads(); }, first, last);
     };
@@ -515,9 +553,10 @@ __global__ void __launch_bounds__(W * 32, 512 / (W * 32)) scan_forward(const Sca
 template <typename T, int V, int W, int R, bool GATE, bool CUT, bool CLUSTER>
 __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
     static_assert(W * R == SCAN_ROWS, "tile");
-    __shared__ Scratch<V> sm;
-    __shared__ Scratch<CLUSTER ? V : 1> peers;  // the other tiles' runs
-    __shared__ Run<V> s_fwd[W][32];
+    __shared__ Scratch<V> sm;  // the other tiles' runs
+    __shared__ Part<V> parts[W][32];
+    __shared__ Vf<V> carries[W][32];  // the parts' H in the carries' direction
+    __shared__ bool s_cut[W];
     __shared__ int s_tile;
     if (test_expired(p)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -570,39 +609,44 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
         return fma(mul(z[r], Vf<V>::all(-1.f)), g, g);
     };
     {
-        Vf<V> q = Vf<V>::all(0.f), h = q, cc = q;
+        Vf<V> q = Vf<V>::all(0.f), h = q, cc = q, left = Vf<V>::all(1.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (CUT && (cuts >> r & 1)) {
-                q = Vf<V>::all(1.f);
-                h = Vf<V>::all(0.f);
-            }
+            if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
             h = advance(h, z[r], x[r].f());
-            q = fma(z[r], fma(q, Vf<V>::all(-1.f), Vf<V>::all(1.f)), q);
+            q = fma(z[r], left, q);
+            left = mul(left, fma(z[r], Vf<V>::all(-1.f), Vf<V>::all(1.f)));
         }
 #pragma unroll
         for (int r = R - 1; r >= 0; --r) cc = carry(r, add(into(r), cc));
-        const Vf<V> n = mul(q, Vf<V>::all(-1.f));
         keep_packed(x);
         keep_packed(f);
         keep_packed(dy);
         if constexpr (GATE) keep_packed(o);
-        s_fwd[warp][lane] = {n, h};
-        sm.run[warp][lane] = {n, cc};
+        parts[warp][lane] = part_of(left, q, h);
+        carries[warp][lane] = cc;
+        if (CUT) s_cut[warp] = cuts != 0;
     }
     __syncthreads();
     // the carries of the rows right of this warp's; the last warp, which has none, joins the tile's
-    Run<V> run = no_run<V>();
+    Part<V> part = no_part<V>();
+    uint32_t cut = CUT ? which_cut<W>(s_cut, lane) : 0;
     {
         const int mine = W - 1 - warp, upto = mine ? mine : W;
-        for (int i = 0; i < upto; ++i) run = join<CUT>(run, sm.run[W - 1 - i][lane]);
-        for (int w = 0; w < warp; ++w) start = join<CUT>(start, s_fwd[w][lane]);
+        for (int i = 0; i < upto; ++i) {
+            const int w = W - 1 - i;
+            part = join_part(part, Part<V>{parts[w][lane].p, parts[w][lane].e, carries[w][lane]});
+            if (CUT && (cut >> w & 1)) part.h = carries[w][lane];
+        }
+        for (int w = 0; w < warp; ++w) start = CUT && (cut >> w & 1) ? parts[w][lane].h : join_part(start, parts[w][lane]);
+        cut >>= W - upto;  // those that were joined
     }
+    const Run<V> run = run_of(part, cut);
     __syncthreads();
     // in walking order the last warp is the first one
     const auto join_tiles = [&](auto first, auto last) {
         if constexpr (CLUSTER)
-            return chain_cluster<CUT, V>(p, k, run, peers, W - 1 - warp, lane, live, first, last);
+            return chain_cluster<CUT, V>(p, k, run, sm, W - 1 - warp, lane, live, first, last);
         else
             return chain<CUT, V, W>(p, k, run, sm, W - 1 - warp, lane, live, [] { __syncthreads(); }, first, last);
     };
@@ -614,7 +658,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
                 for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = out.at(v);
             }
         });
-    Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), prev[R], db = Vf<V>::all(0.f);
+    Vf<V> cc = warp == W - 1 ? in : cut ? part.h : join_part(in, part), prev[R], db = Vf<V>::all(0.f);
     {
         Vf<V> h = start;
 #pragma unroll
@@ -648,11 +692,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
         }
     }
     if (p.dbias_part) {
-        s_fwd[warp][lane].h = db;  // free: every warp read it before the last barrier
+        carries[warp][lane] = db;  // free: every warp read it before the last barrier
         __syncthreads();
         if (warp == 0 && live) {
             Vf<V> s = Vf<V>::all(0.f);
-            for (int w = 0; w < W; ++w) s = add(s, s_fwd[w][lane].h);
+            for (int w = 0; w < W; ++w) s = add(s, carries[w][lane]);
 #pragma unroll
             for (int v = 0; v < V; ++v)
                 p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = s.at(v);
@@ -781,6 +825,8 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u), *f_tiles = smem + G::STAGES * G::STAGE;
     __shared__ Scratch<V> scratch[G::GROUPS];
+    __shared__ Part<V> s_parts[G::GROUPS][W][32];
+    __shared__ bool s_cut[G::GROUPS][W];
     __shared__ Ring<G::FSTAGES, G::STAGES> ring;
     if (test_expired(p)) return;
     const int lane = threadIdx.x & 31, group = threadIdx.x / (W * 32), warp = (threadIdx.x >> 5) & (W - 1);
@@ -803,6 +849,7 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
             });
     } else {
         Scratch<V> &sm = scratch[group];
+        Part<V>(&parts)[W][32] = s_parts[group];
         auto sync = [&] { tc::named_bar(1 + group, W * 32); };
         for (uint32_t n = group;; n += G::GROUPS) {
             const int s = n % G::STAGES;
@@ -834,26 +881,25 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
                 Vf<V> q = Vf<V>::all(0.f), h = q, left = Vf<V>::all(1.f);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    if (CUT && (cuts >> r & 1)) {
-                        q = Vf<V>::all(1.f);
-                        h = left = Vf<V>::all(0.f);
-                    }
-                    // Q as the sum of z times the product so far: as exact, and a shorter chain
+                    if (CUT && (cuts >> r & 1)) h = Vf<V>::all(0.f);
                     const Vf<V> a = fma(z[r], Vf<V>::all(-1.f), Vf<V>::all(1.f));
                     h = fma(a, h, mul(z[r], Word<T>::get(xs + r * 128)));
                     q = fma(z[r], left, q);
                     left = mul(left, a);
                 }
-                sm.run[warp][lane] = {mul(q, Vf<V>::all(-1.f)), h};
+                parts[warp][lane] = part_of(left, q, h);
+                if (CUT) s_cut[group][warp] = cuts != 0;
             }
             sync();
-            Run<V> run = no_run<V>();
-            {
-                const int upto = warp ? warp : W;
-#pragma unroll
-                for (int w = 0; w < W; ++w)
-                    if (w < upto) run = join<CUT>(run, sm.run[w][lane]);
+            Part<V> part = no_part<V>();
+            const int upto = warp ? warp : W;
+            const uint32_t cut = CUT ? which_cut<W>(s_cut[group], lane) & ((1u << upto) - 1u) : 0;
+#pragma unroll 1
+            for (int w = 0; w < upto; ++w) {
+                part = join_part(part, parts[w][lane]);
+                if (CUT && (cut >> w & 1)) part.h = parts[w][lane].h;
             }
+            const Run<V> run = run_of(part, cut);
             sync();
             const Vf<V> in = chain<CUT, V, W>(
                 p, k, run, sm, warp, lane, live, sync,
@@ -908,8 +954,9 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t *smem = raw + ((128u - (tc::su32(raw) & 127u)) & 127u);
     __shared__ Scratch<V> scratch[G::GROUPS];
-    __shared__ Run<V> s_fwd[G::GROUPS][W][32];
-    __shared__ Vf<V> s_db[G::GROUPS][W][32];
+    __shared__ Part<V> s_parts[G::GROUPS][W][32];
+    __shared__ Vf<V> s_carries[G::GROUPS][W][32];  // the parts' H in the carries' direction
+    __shared__ bool s_cut[G::GROUPS][W];
     __shared__ Ring<0, G::STAGES> ring;
     if (test_expired(p)) return;
     const int lane = threadIdx.x & 31, group = threadIdx.x / (W * 32), warp = (threadIdx.x >> 5) & (W - 1);
@@ -938,8 +985,10 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
             });
     } else {
         Scratch<V> &sm = scratch[group];
+        Part<V>(&parts)[W][32] = s_parts[group];
+        Vf<V>(&carries)[W][32] = s_carries[group];
         auto sync = [&] { tc::named_bar(1 + group, W * 32); };
-        const Vf<V> one = Vf<V>::all(1.f), minus = Vf<V>::all(-1.f), none = Vf<V>::all(0.f);
+        const Vf<V> one = Vf<V>::all(1.f), neg = Vf<V>::all(-1.f), none = Vf<V>::all(0.f);
         for (uint32_t n = group;; n += G::GROUPS) {
             const int s = n % G::STAGES;
             if (!tc::mbar_wait(&ring.full[s], (n / G::STAGES) & 1, ctl, FAULT_CODE + 3)) break;
@@ -975,42 +1024,44 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
             };
             auto carry = [&](int r, Vf<V> z, Vf<V> g) {  // a g of one token
                 if (CUT && (cuts >> r & 1)) return none;
-                return fma(mul(z, minus), g, g);
+                return fma(mul(z, neg), g, g);
             };
             Run<V> every[R / 4];  // the run of the rows before every fourth one
             {
                 Vf<V> q = none, h = none, left = one, cc = none, z[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    if (r % 4 == 0) every[r / 4] = {mul(q, minus), h};
+                    if (r % 4 == 0) every[r / 4] = coded(left, q, h);
                     z[r] = z_of(r, power(r));
-                    if (CUT && (cuts >> r & 1)) {
-                        q = one;
-                        h = left = none;
-                    }
-                    const Vf<V> a = fma(z[r], minus, one);
+                    if (CUT && (cuts >> r & 1)) h = none;
+                    const Vf<V> a = fma(z[r], neg, one);
                     h = fma(a, h, mul(z[r], Word<T>::get(xs + r * 128)));
                     q = fma(z[r], left, q);
                     left = mul(left, a);
                 }
 #pragma unroll
                 for (int r = R - 1; r >= 0; --r) cc = carry(r, z[r], add(into(r), cc));
-                const Vf<V> nq = mul(q, minus);
-                s_fwd[group][warp][lane] = {nq, h};
-                sm.run[warp][lane] = {nq, cc};
+                parts[warp][lane] = part_of(left, q, h);
+                carries[warp][lane] = cc;
+                if (CUT) s_cut[group][warp] = cuts != 0;
             }
             sync();
             // the carries of the rows right of this warp's; the last warp, which has none, joins the tile's
-            Run<V> run = no_run<V>();
+            Part<V> part = no_part<V>();
+            const int mine = W - 1 - warp, upto = mine ? mine : W;
+            auto carried = [&](int w) { return Part<V>{parts[w][lane].p, parts[w][lane].e, carries[w][lane]}; };
+            uint32_t cut = CUT ? which_cut<W>(s_cut[group], lane) : 0;
             {
-                const int mine = W - 1 - warp, upto = mine ? mine : W;
-#pragma unroll
-                for (int i = 0; i < W; ++i)
-                    if (i < upto) run = join<CUT>(run, sm.run[W - 1 - i][lane]);
-#pragma unroll
-                for (int w = 0; w < W - 1; ++w)
-                    if (w < warp) start = join<CUT>(start, s_fwd[group][w][lane]);
+#pragma unroll 1
+                for (int i = 0; i < upto; ++i) {
+                    part = join_part(part, carried(W - 1 - i));
+                    if (CUT && (cut >> (W - 1 - i) & 1)) part.h = carries[W - 1 - i][lane];
+                }
+#pragma unroll 1
+                for (int w = 0; w < warp; ++w) start = CUT && (cut >> w & 1) ? parts[w][lane].h : join_part(start, parts[w][lane]);
+                cut >>= W - upto;  // those that were joined to `part`
             }
+            const Run<V> run = run_of(part, cut);
             sync();
             // in walking order the last warp is the first one
             const Vf<V> in = chain<CUT, V, W>(
@@ -1022,10 +1073,11 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                         for (int v = 0; v < V; ++v) p.dh0[(int64_t)k.b * p.C + k.c + v] = out.at(v);
                     }
                 });
-            Vf<V> cc = warp == W - 1 ? in : join<CUT>(in, run), db = none;
+            Vf<V> cc = warp == W - 1 ? in : cut ? part.h : join_part(in, part), db = none;
 #pragma unroll
             for (int r0 = R - 4; r0 >= 0; r0 -= 4) {
-                Vf<V> prev[4], z[4], e[4], h = r0 ? join<CUT>(start, every[r0 / 4]) : start;
+                Vf<V> prev[4], z[4], e[4], h = start;
+                if (r0) h = CUT && (cuts & ((1u << r0) - 1u)) ? every[r0 / 4].h : join<false>(start, every[r0 / 4]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     e[i] = power(r0 + i);
@@ -1043,14 +1095,14 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
                         const Vf<V> o = Word<T>::get(os + r * 128), sg = sigmoid(o);
                         g = mul(dy, mul(o, sg));
                         // silu'(o) = sigmoid(o) (1 + o (1 - sigmoid(o)))
-                        const Vf<V> slope = mul(sg, fma(o, fma(sg, minus, one), one));
+                        const Vf<V> slope = mul(sg, fma(o, fma(sg, neg, one), one));
                         Word<T>::put(os + r * 128, mul(mul(dy, advance(prev[i], z[i], x)), slope));
                     }
                     g = add(g, cc);
                     const Vf<V> dx = mul(z[i], g);
                     cc = carry(r, z[i], g);
                     // a = exp(u) sigmoid(-u): 1 - z would lose a small a
-                    const Vf<V> df = mul(mul(dx, mul(e[i], z[i])), fma(x, minus, prev[i]));
+                    const Vf<V> df = mul(mul(dx, mul(e[i], z[i])), fma(x, neg, prev[i]));
                     db = add(db, df);
                     Word<T>::put(xs + r * 128, dx);
                     Word<T>::put(fs + r * 128, df);
@@ -1058,12 +1110,14 @@ __global__ void __launch_bounds__(BwdCfg<T, GATE>::THREADS, 1)
             }
             tc::mbar_arrive_after_reads(&ring.done[s]);
             if (p.dbias_part) {
-                s_db[group][warp][lane] = db;  // read long before the next tile's
+                // the look-back's place: it is read before the chain's last barrier, and next written
+                // after two of the next tile's
+                sm.run[warp][lane].h = db;
                 sync();
                 if (warp == 0 && live) {
                     Vf<V> t = none;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) t = add(t, s_db[group][w][lane]);
+                    for (int w = 0; w < W; ++w) t = add(t, sm.run[w][lane].h);
 #pragma unroll
                     for (int v = 0; v < V; ++v)
                         p.dbias_part[((int64_t)k.b * p.chunks + chunk) * p.C + k.c + v] = t.at(v);

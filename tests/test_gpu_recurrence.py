@@ -258,3 +258,74 @@ def test_offsets_past_32_bits():
     torch.testing.assert_close(h2, h, rtol=0, atol=2e-4)
     torch.testing.assert_close(y2.float(), y[:, cut:].float(), rtol=2.0 ** -8, atol=2e-4)
     torch.testing.assert_close(dx2.float(), dx[:, cut:].float(), rtol=2.0 ** -8, atol=2e-4)
+
+
+# float32 rows of a width that TMA takes, and of one that it does not; bf16 pairs and single channels
+REPEATS = [(2, 9000, 64, "bf16"), (2, 9000, 66, "bf16"), (2, 9000, 33, "bf16"), (2, 9000, 64, "f32"), (2, 9000, 33, "f32"),
+           (1, 40000, 256, "bf16"), (2, 900, 64, "bf16"), (2, 900, 33, "f32")]
+
+
+@pytest.mark.parametrize("B,L,C,dtype", REPEATS)
+@pytest.mark.parametrize("bias", [0.0, 2.2])
+def test_results_repeat_without_resets(B, L, C, dtype, bias):
+    """Whether a tile finds a neighbour's state or its run must not show: bit for bit the same, also where a tile forgets
+    all that entered it, with a large state, and with a NaN early on."""
+    a, dy, dh = _inputs(B, L, C, dtype, bias=False, spread=1.0)
+    a["bias"] = torch.full((C,), bias).cuda()
+    a["h0"] = a["h0"] * 1e6
+    a["x"][0, 200, 0] = float("nan")
+    dh = dh * 1e6
+    names = ("x", "f", "bias", "gate", "h0")
+    for k in names:
+        a[k] = a[k].detach().requires_grad_()
+    first = None
+    for _ in range(12):
+        y, h = recurrence.gated_scan(*(a[k] for k in names))
+        got = [y, h, *torch.autograd.grad([y, h], [a[k] for k in names], [dy, dh])]
+        bits = [t.detach().nan_to_num(nan=-12345.0) for t in got]
+        first = first or bits
+        assert all(torch.equal(p, q) for p, q in zip(first, bits))
+
+
+# tiles by TMA, without it, and as a cluster; float32 states throughout
+LARGE = [(1, 2560, 64, "f32"), (1, 2560, 33, "f32"), (1, 2560, 64, "bf16"), (1, 1000, 64, "f32"), (1, 1000, 33, "bf16")]
+
+
+@pytest.mark.parametrize("reset", [False, True])
+@pytest.mark.parametrize("B,L,C,dtype", LARGE)
+def test_a_large_state_is_forgotten(B, L, C, dtype, reset):
+    """h0 = 1e8 (and dh = 1e8 from the right) under a = 1/2 and x = 1: as in a token-by-token loop the error
+    follows the state as it decays.  A row changes it by at most 2^-22 of its size (a within 2^-23, two
+    roundings) and 1e8 is below 1 after 27 rows: 7e-6 of |h_t| + 1, a third of the bar of 2e-5."""
+    x, f = torch.ones(B, L, C, dtype=DT[dtype]).cuda(), torch.zeros(B, L, C, dtype=DT[dtype]).cuda()
+    h0, dh = torch.full((B, C), 1e8).cuda(), torch.full((B, C), 1e8).cuda()
+    cut = None
+    if reset:  # the variant with resets, none of them here
+        cut = torch.zeros(B, L, dtype=torch.bool).cuda()
+    dy = torch.ones_like(x)
+    want = oracle(x, f, None, None, h0, cut, dy, dh)
+    x.requires_grad_(), f.requires_grad_(), h0.requires_grad_()
+    y, h = recurrence.gated_scan(x, f, h0=h0, reset=cut)
+    dx, d0 = torch.autograd.grad([y, h], [x, h0], [dy, dh])
+    half = 2.0 ** -8 if dtype == "bf16" else 0.0
+    for got, w, r in ((y, want["y"], half), (h, want["h"], 0.0), (dx, want["dx"], half), (d0, want["dh0"], 0.0)):
+        got = got.detach().double().cpu().numpy()
+        assert (np.abs(got - w) <= (2e-5 + r) * (np.abs(w) + 1.0)).all()
+
+
+@pytest.mark.parametrize("reset", [False, True])
+@pytest.mark.parametrize("B,L,C,dtype", LARGE)
+def test_a_nan_stays_until_a_reset(B, L, C, dtype, reset):
+    """Decays of all sizes: a NaN at token 150 reaches every later token of its channel, up to a reset at
+    token 700 where there is one, and no earlier token and no other channel."""
+    a, _, _ = _inputs(B, L, C, dtype, gate=False, bias=False, spread=3.0)
+    a["x"][0, 150, 3] = float("nan")
+    cut = None
+    if reset:
+        cut = torch.zeros(B, L, dtype=torch.bool).cuda()
+        cut[0, 700] = True
+    y, h = recurrence.gated_scan(a["x"], a["f"], h0=a["h0"], reset=cut)
+    nan = torch.zeros(L, C, dtype=torch.bool)
+    nan[150:700 if reset else L, 3] = True
+    assert torch.equal(torch.isnan(y[0]).cpu(), nan)
+    assert torch.equal(torch.isnan(h[0]).cpu(), nan[-1])
