@@ -214,8 +214,8 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list grads) {
-        TORCH_CHECK(!at::GradMode::is_enabled() || !(grads[0].defined() && grads[0].requires_grad()),
-                    "gated_scan is not twice differentiable");
+        // create_graph: the gradients depend on the inputs, whatever the incoming ones depend on
+        TORCH_CHECK(!at::GradMode::is_enabled(), "gated_scan is not twice differentiable");
         const auto saved = ctx->get_saved_variables();
         auto opt = [&](int i) { return saved[i].defined() ? OptTensor(saved[i]) : OptTensor(); };
         auto given = [&](int i) { return grads[i].defined() ? OptTensor(grads[i]) : OptTensor(); };

@@ -174,3 +174,15 @@ def test_second_derivatives_are_refused():
     y, _ = recurrence.gated_scan(x, x)
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad((y ** 2).sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("of", ["sum of y", "sum of h", "both", "square of y"])
+def test_second_derivatives_are_refused_whatever_the_first_depends_on(of):
+    """The gradient that enters may be a constant or belong to the last state alone: the gradients that
+    leave depend on the inputs all the same, and carry no graph."""
+    x = torch.randn(1, 300, 8, device="cuda", requires_grad=True)
+    y, h = recurrence.gated_scan(x, x)
+    loss = {"sum of y": y.sum(), "sum of h": (h ** 2).sum(), "both": y.sum() + h.sum(), "square of y": (y ** 2).sum()}[of]
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(loss, x, create_graph=True, retain_graph=True)
+    assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
