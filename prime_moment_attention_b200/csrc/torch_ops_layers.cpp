@@ -54,8 +54,16 @@ void check_cuda(const Tensor &t, const char *name) {
     TORCH_CHECK(t.is_cuda(), "pma: ", name, " must be a CUDA tensor (no CPU fallback)");
 }
 
+// Nothing here has a forward-mode derivative: a dual operand is refused, not stripped of its tangent.
+void check_no_tangent(const char *fn, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), fn, " has no forward-mode derivative");
+}
+const Tensor *ptr_of(const OptTensor &t) { return t ? &*t : nullptr; }
+
 // The operators without a gradient say so instead of dropping it.
 void check_no_grad(const char *fn, std::initializer_list<const Tensor *> ts) {
+    check_no_tangent(fn, ts);
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor *t : ts)
         TORCH_CHECK(!t->requires_grad(), fn, " is inference-only: run under torch.no_grad() or torch.inference_mode()");
@@ -235,6 +243,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
 
 std::tuple<Tensor, Tensor> gated_scan_autograd(const Tensor &x, const Tensor &f, const OptTensor &bias,
                                                const OptTensor &gate, const OptTensor &h0, const OptTensor &reset) {
+    check_no_tangent("gated_scan", {&x, &f, ptr_of(bias), ptr_of(gate), ptr_of(h0)});
     auto needs = [](const OptTensor &t) { return t && t->requires_grad(); };
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || f.requires_grad() || needs(bias) || needs(gate) || needs(h0))) {
@@ -269,6 +278,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor &x, const Tensor &f, con
                                            const OptTensor &gate) {
     check_common(x, f, bias, gate, 2);
     check_no_grad("gated_scan_step", {&x, &f, &h});
+    check_no_tangent("gated_scan_step", {ptr_of(bias), ptr_of(gate)});
     check_like(h, "h", x.sizes(), at::kFloat, x.device());
     const Tensor in = h.contiguous();
     Tensor out = at::empty_like(in);
@@ -280,6 +290,7 @@ Tensor gated_scan_step_(const Tensor &x, const Tensor &f, const Tensor &h, const
                         const OptTensor &rows) {
     check_common(x, f, bias, gate, 2);
     check_no_grad("gated_scan_step", {&x, &f, &h});
+    check_no_tangent("gated_scan_step", {ptr_of(bias), ptr_of(gate)});
     if (rows) {
         check_like(*rows, "rows", {x.size(0)}, at::kInt, x.device());
         TORCH_CHECK_VALUE(h.dim() == 2, "h must be [pool rows, channels]");
@@ -443,6 +454,7 @@ PyObject *py_gated_scan(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor &x = a.tensor(0), &f = a.tensor(1);
     const OptTensor bias = a.opt(2), gate = a.opt(3), h0 = a.opt(4), reset = a.opt(5);
     if (!a.plain) return not_here();
+    check_no_tangent("gated_scan", {&x, &f, ptr_of(bias), ptr_of(gate), ptr_of(h0)});
     auto needs = [](const OptTensor &t) { return t && t->requires_grad(); };
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || f.requires_grad() || needs(bias) || needs(gate) || needs(h0))) {

@@ -186,3 +186,31 @@ def test_second_derivatives_are_refused_whatever_the_first_depends_on(of):
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(loss, x, create_graph=True, retain_graph=True)
     assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
+
+
+def test_forward_mode_is_refused():
+    """No tangent is dropped: a dual operand raises, in the direct call and through the dispatcher."""
+    import torch.autograd.forward_ad as fwd
+    x, f, gate = (torch.randn(2, 20, 8, device="cuda") for _ in range(3))
+    bias, h0 = torch.randn(8, device="cuda"), torch.randn(2, 8, device="cuda")
+    scan = recurrence._ops()[0]
+    with fwd.dual_level():
+        for i in range(5):
+            ops = [x, f, bias, gate, h0]
+            ops[i] = fwd.make_dual(ops[i], torch.ones_like(ops[i]))
+            for call in (lambda: recurrence.gated_scan(*ops), lambda: scan(*ops, None)):
+                for grad in (False, True):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward"):
+                        call()
+        ops = [x[:, 0], f[:, 0], h0, bias, gate[:, 0]]
+        for i in range(5):
+            dual = list(ops)
+            dual[i] = fwd.make_dual(ops[i].contiguous(), torch.ones_like(ops[i]))
+            for kw in ({}, {"inplace": True}):
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                    recurrence.gated_scan_step(*dual, **kw)
+        q, s = fp8.quantize_weight(torch.randn(32, 8, device="cuda"))
+        a = fwd.make_dual(x[0].clone(), torch.ones_like(x[0]))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+            fp8.linear(a, q, s)
+    recurrence.gated_scan(x, f, bias, gate, h0)
