@@ -66,7 +66,7 @@ void check_no_grad(const char *fn, std::initializer_list<const Tensor *> ts) {
     check_no_tangent(fn, ts);
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor *t : ts)
-        TORCH_CHECK(!t->requires_grad(), fn, " is inference-only: run under torch.no_grad() or torch.inference_mode()");
+        TORCH_CHECK(!t || !t->requires_grad(), fn, " is inference-only: run under torch.no_grad() or torch.inference_mode()");
 }
 
 void check_like(const Tensor &t, const char *name, at::IntArrayRef shape, at::ScalarType dtype, const at::Device &dev) {
@@ -277,8 +277,7 @@ Tensor step_into(const Tensor &x_in, const Tensor &f_in, const Tensor &h_in, con
 std::tuple<Tensor, Tensor> gated_scan_step(const Tensor &x, const Tensor &f, const Tensor &h, const OptTensor &bias,
                                            const OptTensor &gate) {
     check_common(x, f, bias, gate, 2);
-    check_no_grad("gated_scan_step", {&x, &f, &h});
-    check_no_tangent("gated_scan_step", {ptr_of(bias), ptr_of(gate)});
+    check_no_grad("gated_scan_step", {&x, &f, &h, ptr_of(bias), ptr_of(gate)});
     check_like(h, "h", x.sizes(), at::kFloat, x.device());
     const Tensor in = h.contiguous();
     Tensor out = at::empty_like(in);
@@ -289,8 +288,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor &x, const Tensor &f, con
 Tensor gated_scan_step_(const Tensor &x, const Tensor &f, const Tensor &h, const OptTensor &bias, const OptTensor &gate,
                         const OptTensor &rows) {
     check_common(x, f, bias, gate, 2);
-    check_no_grad("gated_scan_step", {&x, &f, &h});
-    check_no_tangent("gated_scan_step", {ptr_of(bias), ptr_of(gate)});
+    check_no_grad("gated_scan_step", {&x, &f, &h, ptr_of(bias), ptr_of(gate)});
     if (rows) {
         check_like(*rows, "rows", {x.size(0)}, at::kInt, x.device());
         TORCH_CHECK_VALUE(h.dim() == 2, "h must be [pool rows, channels]");

@@ -214,3 +214,17 @@ def test_forward_mode_is_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
             fp8.linear(a, q, s)
     recurrence.gated_scan(x, f, bias, gate, h0)
+
+
+@pytest.mark.parametrize("which", ["x", "f", "h", "bias", "gate"])
+def test_every_operand_of_a_step_that_wants_a_gradient_is_refused(which):
+    a = {k: torch.randn(4, 64, device="cuda") for k in ("x", "f", "h", "gate")}
+    a["bias"] = torch.randn(64, device="cuda")
+    a[which].requires_grad_()
+    calls = [lambda kw=kw: recurrence.gated_scan_step(a["x"], a["f"], a["h"], bias=a["bias"], gate=a["gate"], **kw)
+             for kw in ({}, {"inplace": True}, {"rows": torch.arange(4, dtype=torch.int32, device="cuda")})]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+        with torch.no_grad():
+            call()
