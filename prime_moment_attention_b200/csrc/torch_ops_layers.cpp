@@ -335,7 +335,7 @@ Tensor fp8_linear(const Tensor &x_in, const Tensor &wq_in, const Tensor &ws_in, 
     check_cuda(x_in, "x");
     check_cuda(wq_in, "wq");
     check_cuda(ws_in, "ws");
-    check_no_grad("fp8_linear", {&x_in});
+    check_no_grad("fp8_linear", {&x_in, &ws_in});
     TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.size(-1) > 0, "x must have at least one column; got ", x_in.sizes());
     const at::Device dev = x_in.device();
     const int dtype = dtype_of(x_in);

@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, torch_ops
 from .ops import _DT, _require_cuda, _stream, check_faults
@@ -27,6 +28,14 @@ def _blocks(n: int) -> int:
 def _storage(rows: int, K: int, dev) -> torch.Tensor:
     """[rows, K] e4m3 whose rows start on 16-byte boundaries."""
     return torch.empty(rows, -(-K // 16) * 16, dtype=E4M3, device=dev)[:, :K]
+
+
+def _inference_only(name: str, *ts: torch.Tensor) -> None:
+    """No gradient or tangent is dropped in silence."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} is inference-only: run under torch.no_grad() or torch.inference_mode()")
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _dense(name: str, x: torch.Tensor) -> torch.Tensor:
@@ -68,6 +77,7 @@ def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[M, K] bf16 or float32 -> (e4m3 [M, K], scales [M, ceil(K/128)]).  The scales' storage is
     [ceil(K/128), M], the order the product reads them in."""
     dev = _require_cuda(x)
+    _inference_only("fp8.quantize", x)
     x = _dense("x", x)
     M, K = x.shape
     q, s = _storage(M, K, dev), torch.empty(_blocks(K), M, dtype=torch.float32, device=dev).t()
@@ -77,7 +87,8 @@ def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """[N, K] bf16 or float32 -> (e4m3 [N, K], scales [ceil(N/128), ceil(K/128)])."""
+    """[N, K] bf16 or float32 -> (e4m3 [N, K], scales [ceil(N/128), ceil(K/128)]).  A parameter is taken
+    as it is, without its gradient."""
     dev = _require_cuda(w)
     w = _dense("w", w)
     N, K = w.shape
@@ -102,6 +113,7 @@ def matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tenso
            out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x @ w.T of quantised x [M, K] (scales [M, ceil(K/128)]) and w [N, K] (scales per 128 x 128)."""
     dev = _require_cuda(xq, xs, wq, ws)
+    _inference_only("fp8.matmul", xs, ws)
     check_faults("fp8.matmul")
     if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] == 0:
         raise ValueError("xq and wq must be matrices with at least one column")

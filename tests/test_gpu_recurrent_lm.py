@@ -228,3 +228,31 @@ def test_every_operand_of_a_step_that_wants_a_gradient_is_refused(which):
             call()
         with torch.no_grad():
             call()
+
+
+def test_every_operand_of_an_8_bit_product_that_wants_a_gradient_is_refused():
+    x, w = torch.randn(4, 64, device="cuda"), torch.randn(32, 64, device="cuda", requires_grad=True)
+    (xq, xs), (wq, ws) = fp8.quantize(x), fp8.quantize_weight(w)  # weights are taken from parameters
+    out = torch.empty(4, 32, device="cuda")
+    on = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for call in (lambda: fp8.linear(on(x), wq, ws), lambda: fp8.linear(on(x), wq, ws, out=out),
+                 lambda: fp8.linear(x, wq, on(ws)), lambda: fp8.linear(x, wq, on(ws), out=out),
+                 lambda: fp8.quantize(on(x)), lambda: fp8.matmul(xq, on(xs), wq, ws),
+                 lambda: fp8.matmul(xq, xs, wq, on(ws))):
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+def test_8_bit_products_refuse_dual_operands():
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(4, 64, device="cuda")
+    (xq, xs), (wq, ws) = fp8.quantize(x), fp8.quantize_weight(torch.randn(32, 64, device="cuda"))
+    with fwd.dual_level(), torch.no_grad():
+        a, s = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(ws, torch.ones_like(ws))
+        for call in (lambda: fp8.quantize(a), lambda: fp8.linear(a, wq, ws, out=torch.empty(4, 32, device="cuda")),
+                     lambda: fp8.linear(x, wq, s), lambda: fp8.matmul(xq, xs, wq, s)):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        fp8.matmul(xq, xs, wq, ws)
