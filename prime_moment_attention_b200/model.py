@@ -173,7 +173,8 @@ class PrimeForCausalLM(nn.Module):
                  uniforms: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Same sampling rule as model.py:203-242 (greedy when temperature == 0), drawn by
         torch.multinomial.  With `uniforms` [max_new_tokens, B], float32 in [0, 1), the tokens come
-        from sampling.sample instead: given numbers, and top_p and min_p as well as top_k."""
+        from sampling.sample instead: given numbers, and top_p and min_p as well as top_k; a row whose
+        logits are NaN or -inf throughout gets token -1."""
         self.eval()
         if uniforms is None and (top_p < 1.0 or min_p > 0.0):
             raise ValueError("top_p and min_p need uniforms")
@@ -198,9 +199,15 @@ class PrimeForCausalLM(nn.Module):
             generated = torch.cat([generated, nxt], dim=-1)
             if eos_token_id is not None and (nxt == eos_token_id).all():
                 break
-            out = self.forward(nxt, states=states, return_states=True)
+            out = self.forward(_lookup(nxt), states=states, return_states=True)
             states, logits = out["states"], out["logits"][:, -1, :]
         return generated
+
+
+def _lookup(tokens: torch.Tensor) -> torch.Tensor:
+    """Tokens to embed: a row that the sampler found nothing in (-1: its logits are NaN or -inf throughout)
+    goes on with token 0, so that the other rows of the batch can."""
+    return tokens.clamp(min=0)
 
 
 class DecodeGraph:
@@ -214,7 +221,8 @@ class DecodeGraph:
     temperature 0.
 
     With a `sampler` (sampling.Sampler) the step samples instead: `step(u)` takes the step's uniform
-    numbers [B] and leaves the tokens' log-probabilities in `self.logprobs`.  With fp8=True the
+    numbers [B] and leaves the tokens' log-probabilities in `self.logprobs` (token -1 and -inf for a row
+    whose logits are NaN or -inf throughout; the other rows are not touched by it).  With fp8=True the
     projections and the head run on e4m3 copies of the weights (fp8.Fp8Weight)."""
 
     def __init__(self, model: PrimeForCausalLM, states: List[Tuple[torch.Tensor, ...]], tokens: torch.Tensor,
@@ -261,7 +269,7 @@ class DecodeGraph:
 
     def _body(self, write: bool):
         m = self.model
-        h = m.embed_tokens(self.tokens)  # [B, 1, hidden]
+        h = m.embed_tokens(self.tokens if self.sampler is None else _lookup(self.tokens))  # [B, 1, hidden]
         h = h[:, 0]  # [B, hidden]
         for layer, st, w_qkv, w_gu, w_o, w_down in zip(m.layers, self.states, self.w_qkv, self.w_gu, self.w_o,
                                                        self.w_down):

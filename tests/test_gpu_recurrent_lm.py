@@ -256,3 +256,39 @@ def test_8_bit_products_refuse_dual_operands():
             with pytest.raises(RuntimeError, match="forward"):
                 call()
         fp8.matmul(xq, xs, wq, ws)
+
+
+def test_a_nan_row_does_not_end_a_generation():
+    """A prompt that ends in NaN gives -1 from there on; the other rows are what they are without it."""
+    m = _model().eval()
+    with torch.no_grad():
+        m.embed_tokens.weight[7] = float("nan")
+    ids = torch.randint(8, 301, (4, 9), device="cuda")
+    u = torch.rand(12, 4, device="cuda")
+    kw = dict(max_new_tokens=12, temperature=0.9, top_k=30, top_p=0.95, uniforms=u)
+    want = m.generate(ids, **kw)
+    bad = ids.clone()
+    bad[1, 4] = 7
+    got = m.generate(bad, **kw)
+    assert (got[1, 9:] == -1).all() and torch.equal(got[[0, 2, 3]], want[[0, 2, 3]])
+    assert ((want >= 0) & (want < 301)).all()
+
+
+@pytest.mark.parametrize("use_fp8", [False, True])
+def test_a_nan_row_does_not_end_a_decode_graph(use_fp8):
+    m = _model(torch.bfloat16).eval()
+    ids = torch.randint(301, (5, 17), device="cuda")
+    settings = sampling.Sampler(temperature=0.8, top_k=40)
+    with torch.no_grad():
+        out = m(ids, return_states=True, last_logits_only=True)
+        first = out["logits"][:, -1].argmax(-1)
+        good = DecodeGraph(m, out["states"], first, sampler=settings, fp8=use_fp8)
+        for (h,) in out["states"]:
+            h[2] = float("nan")
+        graph = DecodeGraph(m, out["states"], first, sampler=settings, fp8=use_fp8)
+        rest = [0, 1, 3, 4]
+        for _ in range(4):
+            u = torch.rand(5, device="cuda")
+            got, want = graph.step(u)[:, 0], good.step(u)[:, 0]
+            assert got[2] == -1 and torch.isneginf(graph.logprobs[2])
+            assert torch.equal(got[rest], want[rest]) and torch.equal(graph.logits[rest], good.logits[rest])
