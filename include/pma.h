@@ -547,8 +547,9 @@ PMA_API int pma_sample(int B, int V, const void *logits, int64_t row_stride, int
  *     j * scale_stride_k]; weights: one per 128 rows and 128 of K, [ceil(N/128), ceil(K/128)]
  *     with a row stride.
  *   quantisation: amax over the block (at least 2^-100), scale = amax / 448, element =
- *     e4m3(448 x / amax), rounded to nearest even.  A block with a NaN or an infinity
- *     gives NaN.
+ *     e4m3(448 x / amax), rounded to nearest even from the float32 quotient of the float32
+ *     product (for bf16 x: the nearest to the exact quotient).  A block with a NaN or an
+ *     infinity gives NaN.
  *   pma_fp8_matmul: y[m, n] = sum_k x[m, k] w[n, k], each K block summed by the tensor
  *     cores, scaled and accumulated in float32, rounded once to y's dtype.
  *   pma_fp8_linear: quantises x [M, K] (PMA_BF16 or PMA_F32) and multiplies, with scratch

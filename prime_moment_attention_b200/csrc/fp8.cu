@@ -33,15 +33,16 @@ namespace {
 using namespace tc;
 
 // -------------------------------------------------------------------------------- quantisation
-// e4m3 of x * 448 / amax, rounded once from the correctly rounded quotient: an x that lies half-way
-// between two e4m3 values on the block's scale is exactly half-way after the division too.
+// e4m3 of 448 x / amax, nearest even, where float32 x has the product and the quotient rounded to float32
+// first, as the same expression in any float32 arithmetic has (an x within 2 ulp of half-way between two
+// e4m3 values on the block's scale may go to either); for bf16 x that is the nearest to the exact quotient.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
 //
-// float32: the division is only made where it can matter: x (448 / amax) is within 2 ulp of the quotient,
+// float32: the division is only made where it can matter: x (448 / amax) is within 3 ulp of the quotient,
 // which rounds to the same e4m3 value unless it lies that close to the middle of two (or is below 2^-6,
 // where e4m3's spacing is fixed).
 // bf16: never made. x and amax have 8 significant bits X and A, a middle t has 5, T: a quotient 7 X / A 2^n

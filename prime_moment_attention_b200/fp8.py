@@ -75,7 +75,8 @@ class Fp8Weight:
 
 def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[M, K] bf16 or float32 -> (e4m3 [M, K], scales [M, ceil(K/128)]).  The scales' storage is
-    [ceil(K/128), M], the order the product reads them in."""
+    [ceil(K/128), M], the order the product reads them in.  Elements are e4m3(448 x / amax) of float32
+    arithmetic, with amax the largest magnitude of a row's 128."""
     dev = _require_cuda(x)
     _inference_only("fp8.quantize", x)
     x = _dense("x", x)

@@ -210,3 +210,24 @@ def test_scales_of_any_strides(M, N, K):
         _check_product(fp8.linear(x, wq, ws, out_dtype=torch.float32), xq, xs, wq, dense)
     for one in (xs[:1].expand(M, kb), xs[:, :1].expand(M, kb)):  # and those of x
         _check_product(fp8.matmul(xq, one, wq, dense), xq, one, wq, dense)
+
+
+def test_float32_ties_go_by_the_float32_quotient():
+    """Float32 values whose exact quotient lies half-way between two e4m3 values, and their neighbours: the bytes of the
+    float32 expression, and never farther from x than half a step of e4m3 (2^-4 of a binade) and the two
+    roundings, 2^-23 of the value."""
+    g = torch.Generator().manual_seed(3)
+    n = 4096
+    m = torch.randint(1 << 18, 1 << 19, (n, 1), generator=g).double()       # 448 (m t) / (7 m) = 64 t
+    t = torch.randint(8, 16, (n, 40), generator=g).double() * 2 + 1          # between two significands of 4 bits
+    x = (m * t * 2.0 ** torch.randint(-13, -2, (n, 40), generator=g).double()).float()  # 24 bits: 448 x has more
+    amax, none = (7 * m).float(), torch.zeros(())
+    both = torch.cat([amax, x, x.nextafter(none), x.nextafter(none + 1e9)], 1)
+    both = torch.cat([both, torch.tensor([[2089626.0, 79293.84375] + [0.0] * (both.shape[1] - 2)])]).cuda()
+    q, s = fp8.quantize(both)
+    pq, ps = _plain_rows(both)
+    assert torch.equal(q.view(torch.uint8), pq.view(torch.uint8)) and torch.equal(s, ps)
+    back = q.double() * both.double().amax(1, keepdim=True) / 448
+    v = both.double() * 448 / both.double().amax(1, keepdim=True)
+    step = torch.exp2(torch.floor(torch.log2(v.clamp_min(2.0 ** -6))) - 3)
+    assert ((back - both.double()).abs() * 448 / both.double().amax(1, keepdim=True) <= step / 2 + 2.0 ** -23 * v).all()
