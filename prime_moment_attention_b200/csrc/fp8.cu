@@ -12,7 +12,7 @@
 // 2.2 PFLOP/s).
 //
 // The operand with 128 rows a tile (the tensor core's M) is x for many tokens and w for few: then a
-// tile is 128 weight rows by all the tokens (16 to 128), the weights stream once, and K is split over
+// tile is 128 weight rows by all the tokens (16 to 64), the weights stream once, and K is split over
 // a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order (so it is for few
 // tiles of many tokens and a long K).  64 x 32000 x 768:
 // 10.9 us, against 3.8 for its bytes: latency of set-up, six K blocks and the stores.
@@ -767,10 +767,10 @@ template <int BN, bool FEW> cudaError_t matmul_t(Fp8Params &p, int sms, bool aft
 }  // namespace
 
 cudaError_t launch_fp8_quantize(const void *x, int64_t xs, int dtype, int M, int K, uint8_t *q, int64_t qs,
-                                float *scale, int64_t si, int64_t sj, cudaStream_t st) {
+                                float *scale, int64_t si, int64_t sj, int sms, cudaStream_t st) {
     const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
     // two blocks a lane group once that still fills the GPU
-    const int groups = (int64_t)M * blocks >= 148 * 128 * 4 && blocks > 1 ? 2 : 1;
+    const int groups = (int64_t)M * blocks >= (int64_t)sms * 128 * 4 && blocks > 1 ? 2 : 1;
     const uint32_t per_row = (uint32_t)((blocks + groups - 1) / groups);
     const int64_t items = (int64_t)M * per_row;
     if (items > 0xfffffff0ll) return cudaErrorInvalidValue;

@@ -27,7 +27,7 @@ struct Fp8Params {
 };
 
 cudaError_t launch_fp8_quantize(const void *x, int64_t xs, int dtype, int M, int K, uint8_t *q, int64_t qs,
-                                float *scale, int64_t si, int64_t sj, cudaStream_t st);
+                                float *scale, int64_t si, int64_t sj, int sms, cudaStream_t st);
 cudaError_t launch_fp8_quantize_weight(const void *w, int64_t ws, int dtype, int N, int K, uint8_t *q, int64_t qs,
                                        float *scale, cudaStream_t st);
 // after_quantize: the last kernel in the stream is launch_fp8_quantize's, with which it may overlap.

@@ -980,7 +980,7 @@ int pma_fp8_quantize(int M, int K, const void *x, int64_t x_stride, int dtype, v
     DevInfo di;
     if ((rc = device_info(&di))) return rc;
     const cudaError_t e = launch_fp8_quantize(x, x_stride, dtype, M, K, static_cast<uint8_t *>(q), q_stride, scale,
-                                              scale_stride_m, scale_stride_k, reinterpret_cast<cudaStream_t>(stream));
+                                              scale_stride_m, scale_stride_k, di.sms, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? PMA_OK : cuda_fail(e);
 }
 
