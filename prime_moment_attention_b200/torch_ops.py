@@ -37,6 +37,8 @@ def _scan_bytes(words: int) -> int:
     return (runs_at + 8 * words + 255) // 256 * 256
 
 
+# (run, not traced, where torch.compile meets it: a program's first use may be inside a compiled function)
+@torch.compiler.assume_constant_result
 def load() -> None:
     """Load the operator library (once) and register the operators' shape functions."""
     global _loaded
