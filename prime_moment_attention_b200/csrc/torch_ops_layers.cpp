@@ -26,6 +26,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
 
+#include <atomic>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -42,6 +43,20 @@ void check_rc(int rc, const char *fn) {
     std::string msg = std::string(fn) + " failed: " + pma_status_string(rc);
     if (rc == PMA_ERR_CUDA) msg += std::string(": ") + pma_cuda_error_string(pma_last_cuda_error());
     TORCH_CHECK(false, msg);
+}
+
+// The fault word as the host reads it (watch_faults; pinned host memory).  The operators whose kernels wait
+// look at it: calls of a compiled program pass by the Python layer's check.
+std::atomic<int *> g_watched{nullptr};
+
+void check_faults(const char *fn) {
+    int *word = g_watched.load(std::memory_order_acquire);
+    if (!word) return;
+    const int code = *static_cast<volatile int *>(word);
+    if (code == 0) return;
+    *static_cast<volatile int *>(word) = 0;
+    TORCH_CHECK(false, fn, ": an earlier launch recorded fault code ", code,
+                " (a bounded wait expired; its outputs are void)");
 }
 
 int dtype_of(const Tensor &t) {
@@ -150,6 +165,7 @@ ScanArgs scan_args(const Tensor &x, const Tensor &f, const OptTensor &bias, cons
 
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor &x_in, const Tensor &f_in, const OptTensor &bias,
                                                 const OptTensor &gate, const OptTensor &h0, const OptTensor &reset) {
+    check_faults("gated_scan");
     const ScanArgs a = scan_args(x_in, f_in, bias, gate, h0, reset);
     const at::Device dev = a.x.device();
     const c10::cuda::CUDAGuard guard(dev);
@@ -171,6 +187,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> scan_backward(const Tensor &x
                                                                  const OptTensor &h0, const OptTensor &reset,
                                                                  const Tensor &ws, const OptTensor &dy_in,
                                                                  const OptTensor &dh_in, bool want_bias, bool want_h0) {
+    check_faults("gated_scan_backward");
     const ScanArgs a = scan_args(x_in, f_in, bias, gate, h0, reset);
     const at::Device dev = a.x.device();
     const c10::cuda::CUDAGuard guard(dev);
@@ -336,6 +353,7 @@ Tensor fp8_linear(const Tensor &x_in, const Tensor &wq_in, const Tensor &ws_in, 
     check_cuda(wq_in, "wq");
     check_cuda(ws_in, "ws");
     check_no_grad("fp8_linear", {&x_in, &ws_in});
+    check_faults("fp8_linear");
     TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.size(-1) > 0, "x must have at least one column; got ", x_in.sizes());
     const at::Device dev = x_in.device();
     const int dtype = dtype_of(x_in);
@@ -523,10 +541,21 @@ PyObject *py_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// watch_faults(address of the pinned host int that is registered as the fault word)
+PyObject *py_watch_faults(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 1)) return nullptr;
+    void *word = PyLong_AsVoidPtr(args[0]);
+    if (!word && PyErr_Occurred()) throw python_error();
+    g_watched.store(static_cast<int *>(word), std::memory_order_release);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 #define PMA_FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {PMA_FAST("gated_scan", py_gated_scan), PMA_FAST("gated_scan_step", py_step),
                          PMA_FAST("gated_scan_step_", py_step_), PMA_FAST("sample", py_sample),
-                         PMA_FAST("fp8_linear", py_fp8_linear), {nullptr, nullptr, 0, nullptr}};
+                         PMA_FAST("fp8_linear", py_fp8_linear), PMA_FAST("watch_faults", py_watch_faults), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pma_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

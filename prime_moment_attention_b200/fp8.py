@@ -148,8 +148,8 @@ def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out_dtype: torch
             r = _c.fp8_linear(x, wq, ws, out_dtype == torch.float32)
             if r is not NotImplemented:
                 return r
-        torch_ops.load()
         _require_cuda(x, wq, ws)
+        torch_ops.watch_faults()
         return torch.ops.pma.fp8_linear.default(x, wq, ws, out_dtype)
     _require_cuda(x, wq, ws)
     if x.dim() != 2:

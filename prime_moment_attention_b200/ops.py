@@ -180,6 +180,12 @@ def _arm_faults() -> None:
         _fault, _fault_view = word, word.numpy()
 
 
+def fault_address() -> int:
+    """Address of the fault word (registered here on first use): pinned host memory."""
+    _arm_faults()
+    return _fault.data_ptr()
+
+
 def pending_fault() -> int:
     """Code recorded by a finished tensor-core prefill launch since the last check (0 if none).
     Does not synchronise: a launch still running has not reported yet."""

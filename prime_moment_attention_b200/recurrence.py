@@ -59,6 +59,7 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, bias: Optional[torch.Tensor] = 
         if r is not NotImplemented:
             return r
     _require_cuda(x, f)
+    torch_ops.watch_faults()
     return _ops()[0](x, f, bias, gate, h0, reset)
 
 

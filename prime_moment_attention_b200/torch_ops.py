@@ -24,6 +24,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_pma_torch.so")
 _loaded = False
+_watching = False
 
 
 def _state_like(B: int, H: int, D: int, device):
@@ -97,6 +98,17 @@ def load() -> None:
         return x.new_empty((*x.shape[:-1], wq.shape[0]), dtype=out_dtype)
 
     _loaded = True
+
+
+@torch.compiler.assume_constant_result
+def watch_faults() -> None:
+    """Load, and let the operators whose kernels wait (the recurrence's tiles, the 8-bit product) look at the
+    fault word themselves: a compiled program calls them without the Python layer's check."""
+    global _watching
+    if not _watching:
+        from . import ops
+        direct().watch_faults(ops.fault_address())
+        _watching = True
 
 
 def direct():

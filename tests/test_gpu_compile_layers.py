@@ -7,7 +7,7 @@ import sys
 import pytest
 import torch
 
-from prime_moment_attention_b200 import fp8, recurrence, sampling
+from prime_moment_attention_b200 import _lib, fp8, ops, recurrence, sampling
 
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -73,3 +73,24 @@ def test_the_first_use_may_be_compiled(name):
             "    assert t._same(got, f(*t._args()))\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-1500:]
+
+
+@pytest.mark.parametrize("name,code", [("scan", 120), ("linear", 130)])
+def test_a_compiled_program_sees_an_expired_wait(name, code):
+    """The test hook makes a launch give up; the compiled program's next call says so, once."""
+    with torch.no_grad():
+        f = torch.compile(CALLS[name], backend="aot_eager", fullgraph=True)
+        want = f(*_args())
+        ops.check_faults(synchronize=True)
+        _lib.load().pma_test_expire_waits(1_000_000)
+        try:
+            f(*_args())
+        except RuntimeError:  # its own second launch may have seen the first's already
+            pass
+        finally:
+            _lib.load().pma_test_expire_waits(0)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match=f"fault code {code}"):
+            f(*_args())
+        assert _same(f(*_args()), want)
+        ops.check_faults(synchronize=True)
