@@ -322,6 +322,7 @@ class DecodeGraph:
         return y
 
     def step(self, u: Optional[torch.Tensor] = None) -> torch.Tensor:
+        ops.check_faults("DecodeGraph.step")  # the 8-bit products of an earlier replay
         if (u is None) != (self.sampler is None):
             raise ValueError("step() takes uniform numbers exactly when the graph samples")
         if u is not None:

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from prime_moment_attention_b200 import fp8, recurrence, sampling
+from prime_moment_attention_b200 import fp8, ops, recurrence, sampling
 from prime_moment_attention_b200.model import DecodeGraph, PrimeConfig, PrimeForCausalLM
 
 pytestmark = pytest.mark.gpu
@@ -292,3 +292,19 @@ def test_a_nan_row_does_not_end_a_decode_graph(use_fp8):
             got, want = graph.step(u)[:, 0], good.step(u)[:, 0]
             assert got[2] == -1 and torch.isneginf(graph.logprobs[2])
             assert torch.equal(got[rest], want[rest]) and torch.equal(graph.logits[rest], good.logits[rest])
+
+
+def test_a_decode_graph_reports_a_fault_at_the_next_step():
+    """A replay's kernels record an expired wait in the fault word (written here by hand); step() raises it, once."""
+    m = _model(torch.bfloat16).eval()
+    ids = torch.randint(301, (2, 5), device="cuda")
+    with torch.no_grad():
+        out = m(ids, return_states=True, last_logits_only=True)
+        graph = DecodeGraph(m, out["states"], out["logits"][:, -1].argmax(-1), fp8=True)
+    graph.step()
+    ops.check_faults(synchronize=True)
+    ops._fault_view[0] = 131
+    with pytest.raises(ops.KernelFault) as e:
+        graph.step()
+    assert e.value.code == 131
+    graph.step()
