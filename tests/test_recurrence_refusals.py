@@ -42,3 +42,14 @@ def test_workspace_sizes():
     assert L.pma_gated_scan_workspace_bytes(4, 129, 64) >= 4 * 2 * 64 * 12
     # 64-bit sizes: 2^20 tokens of 4096 channels in 16 rows
     assert L.pma_gated_scan_workspace_bytes(16, 1 << 20, 4096) > 6 << 30
+
+
+def test_traced_workspace_sizes_are_the_librarys():
+    """The shape function restates the library's rule, in whole numbers that may be symbols."""
+    from prime_moment_attention_b200 import torch_ops
+    L = _lib.load()
+    for B in (1, 3, 16):
+        for n in (1, 127, 128, 129, 300, 4096, 99999):
+            for C in (1, 5, 64, 515, 4096):
+                words = B * ((n + 127) // 128) * C
+                assert (0 if n <= 128 else torch_ops._scan_bytes(words)) == L.pma_gated_scan_workspace_bytes(B, n, C)
