@@ -156,13 +156,13 @@ def _stream(device) -> int:
 
 
 class KernelFault(RuntimeError):
-    """A tensor-core prefill launch gave up: one of its bounded waits expired, so its outputs
-    were not written.  `code` identifies the wait."""
+    """A launch with bounded waits (a tensor-core prefill, the recurrence's tiles, the 8-bit product) gave
+    up: one of them expired, so its outputs are void.  `code` identifies the wait."""
 
     def __init__(self, code: int, where: str):
         self.code = code
-        super().__init__(f"{where}: a tensor-core prefill launch recorded fault code {code} "
-                         "(a bounded wait expired; its outputs were not written)")
+        super().__init__(f"{where}: an earlier launch recorded fault code {code} "
+                         "(a bounded wait expired; its outputs are void)")
 
 
 _fault: Optional[torch.Tensor] = None  # pinned host int32 registered as the library's fault word
