@@ -13,7 +13,8 @@
 // The same functions are the Python extension module _pma_torch (this library, imported): a call
 // there skips the dispatcher's argument boxing.  A small call's time is host time: a 64 x 768 step
 // takes 6 us so, 9 through torch.ops, 25 through ctypes.  Calls with anything but plain tensors, or
-// under a dispatch mode, return NotImplemented, and the modules go through torch.ops.
+// under a dispatch mode, a tracer or a function transform, return NotImplemented, and the modules go
+// through torch.ops.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -423,11 +424,16 @@ TORCH_LIBRARY_IMPL(pma, Autograd, m) { m.impl("gated_scan", &gated_scan_autograd
 // ------------------------------------------------------------------------------ Python extension
 namespace {
 
-// Plain tensors (or None where `optional`) and no dispatch mode: otherwise the dispatcher's business.
+// Plain tensors (or None where `optional`), no dispatch mode, no tracer and no function transform: otherwise
+// the dispatcher's business (a tracer would see the results as constants).
 struct Args {
     PyObject *const *a;
     bool plain = true;
-    explicit Args(PyObject *const *args) : a(args) { plain = !c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+    explicit Args(PyObject *const *args) : a(args) {
+        constexpr c10::DispatchKeySet above{c10::DispatchKey::Tracer, c10::DispatchKey::FuncTorchDynamicLayerFrontMode};
+        plain = !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                !c10::impl::tls_local_dispatch_key_set().included_.has_any(above);
+    }
     const Tensor &tensor(int i) {
         static const Tensor none;
         if (!THPVariable_CheckExact(a[i]) && !Py_IS_TYPE(a[i], reinterpret_cast<PyTypeObject *>(ParameterClass))) {

@@ -94,3 +94,23 @@ def test_a_compiled_program_sees_an_expired_wait(name, code):
             f(*_args())
         assert _same(f(*_args()), want)
         ops.check_faults(synchronize=True)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_traced_calls_are_calls(name):
+    """torch.jit.trace records the operators, not their results on the example."""
+    with torch.no_grad():
+        f = torch.jit.trace(lambda *a: CALLS[name](*a), _args(), check_trace=False)
+        other = tuple(a.flip(0) if i < 3 else a for i, a in enumerate(_args()))
+        assert _same(f(*other), CALLS[name](*other)) and not _same(f(*other), f(*_args()))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_calls_under_vmap():
+    x, b, u, wq, ws = _args()
+    xs = torch.stack([x, x.flip(1), -x])
+    with torch.no_grad():
+        got = torch.func.vmap(lambda q: recurrence.gated_scan(q, q * 2, b))(xs)
+        want = [recurrence.gated_scan(q, q * 2, b) for q in xs]
+        assert all(torch.equal(got[i], torch.stack([w[i] for w in want])) for i in range(2))
