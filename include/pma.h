@@ -477,7 +477,8 @@ PMA_API int pma_swiglu(int64_t rows, int inter, const void *gate, int64_t gate_s
  * (float32 [C]), h0 (float32 [B, C], else zero) and reset (uint8 [B, L]; nonzero
  * replaces h_{t-1} by zero: a document starts at t) may be NULL.  h_last (float32
  * [B, C]) may be NULL and receives h_L (h0, or zero, where L is 0).  States are float32;
- * y is rounded once to its dtype.  Results do not depend on timing.
+ * y is rounded once to its dtype.  Results do not depend on timing.  Outputs do not
+ * overlap inputs (h_last may be h0 where L is 0, dh0 dh_last).
  * The workspace (256-byte aligned) holds one float32 state per channel and 128 tokens,
  * among others; pma_gated_scan_backward of the same call takes it back as `forward_ws`.
  */

@@ -848,6 +848,7 @@ int pma_gated_scan(int B, int L, int C, const pma_seq_tensor *x, const pma_seq_t
     if ((rc = check_blc(x, x, empty)) || (rc = check_blc(f, x, empty)) || (gate && (rc = check_blc(gate, x, empty))) ||
         (rc = check_blc(y, x, empty)))
         return rc;
+    if (!empty && h_last && h_last == h0) return PMA_ERR_ARGUMENT;  // every warp of the first tiles reads h0
     DevInfo di;
     if ((rc = device_info(&di))) return rc;
     if (B == 0) return PMA_OK;
@@ -883,6 +884,7 @@ int pma_gated_scan_backward(int B, int L, int C, const pma_seq_tensor *x, const 
     for (const pma_seq_tensor *t : {x, f, dy, dx, df})
         if ((rc = check_blc(t, x, empty))) return rc;
     if (gate && ((rc = check_blc(gate, x, empty)) || (rc = check_blc(dgate, x, empty)))) return rc;
+    if (!empty && dh0 && (dh0 == dh_last || dh0 == h0)) return PMA_ERR_ARGUMENT;
     DevInfo di;
     if ((rc = device_info(&di))) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -53,3 +53,12 @@ def test_traced_workspace_sizes_are_the_librarys():
             for C in (1, 5, 64, 515, 4096):
                 words = B * ((n + 127) // 128) * C
                 assert (0 if n <= 128 else torch_ops._scan_bytes(words)) == L.pma_gated_scan_workspace_bytes(B, n, C)
+
+
+def test_states_in_place_are_refused():
+    """The last state's tile may finish before every warp of the first has read the first state."""
+    L = _lib.load()
+    assert L.pma_gated_scan(1, 300, 64, _t(), _t(), None, None, 512, None, _t(), 512, 256, 1 << 20, None) == 1
+    for dh_last, h0 in ((512, None), (None, 512)):
+        assert L.pma_gated_scan_backward(1, 300, 64, _t(), _t(), None, None, h0, None, _t(), dh_last, _t(), _t(), None,
+                                         None, 512, 256, 1 << 20, 256, 1 << 20, None) == 1
