@@ -138,7 +138,7 @@ PMA_API const char *pma_cuda_error_string(int cuda_error);
  * which the host can read at any time without synchronising), as the process-wide
  * fault word: every later launch of a kernel with bounded waits (the tensor-core
  * prefills: pma_prefill, pma_prefill_ex, pma_prefill_no_alloc, pma_selective_prefill,
- * pma_delta_prefill) stores the code of the first wait that expires into it when it
+ * pma_delta_prefill; pma_gated_scan and its backward pass; pma_fp8_matmul, pma_fp8_linear) stores the code of the first wait that expires into it when it
  * still reads 0.  The library never clears it; NULL unregisters.  No counterpart in
  * the reference, which has no device waits (its only failure signals are NaN checks,
  * c/main.c:92-98 and model.py:221,228).
@@ -151,7 +151,8 @@ PMA_API void pma_set_fault_word(int *word);
  * pma_prefill_no_alloc, pma_selective_prefill; not the delta-rule prefill) first waits,
  * with that bound, for a barrier phase that nothing completes;
  * the wait expires before any copy or GEMM is issued, the launch records code 90
- * (workspace status word and fault word) and returns without writing outputs.
+ * (workspace status word and fault word) and returns without writing outputs.  The
+ * recurrence and the 8-bit product do likewise (codes 120 and 130, fault word only).
  * 0 restores normal operation.  For tests only; no counterpart in the reference.
  */
 PMA_API void pma_test_expire_waits(unsigned long long limit_ns);

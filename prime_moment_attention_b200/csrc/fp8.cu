@@ -8,14 +8,14 @@
 // float32 registers while the tensor core fills the other.  One warp moves tiles by TMA (128-byte
 // swizzle; the tensor map's extents fill ragged edges with zeros, which are zeros in e4m3), one
 // issues the products, one copies the scales.  What bounds it is the epilogue: a K block's 128 x 256
-// sums take some 1000 cycles to read, scale and add, against 540 for the products (8192^3: 500 us,
+// sums take some 1000 cycles to read, scale and add, against 540 for the products (8192^3: 508 us,
 // 2.2 PFLOP/s).
 //
 // The operand with 128 rows a tile (the tensor core's M) is x for many tokens and w for few: then a
 // tile is 128 weight rows by all the tokens (16 to 64), the weights stream once, and K is split over
 // a cluster of up to 8 CTAs whose partial sums meet in shared memory in a fixed order (so it is for few
 // tiles of many tokens and a long K).  64 x 32000 x 768:
-// 10.9 us, against 3.8 for its bytes: latency of set-up, six K blocks and the stores.
+// 11.6 us, against 4.4 for its bytes: latency of set-up, six K blocks and the stores.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -165,7 +165,7 @@ __device__ __forceinline__ uint2 quant8(const Eight<__nv_bfloat16> &x, const Qua
 // Lets the product that follows in the stream start: it waits for this grid before it reads q.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// 8192 x 8192: bf16 in 37 us, 5.4 TB/s; float32 in 51 us, bound by the instructions of its checks. 16 lanes a
+// 8192 x 8192: bf16 in 38 us, 5.3 TB/s; float32 in 51 us, 6.5 TB/s, the rate of a copy. 16 lanes a
 // block and 8 elements a lane, with twice the shuffles and work per block: 47 and 64. bf16 with float32's
 // checks 61, with a division an element 71.
 // 8 lanes a block of 128, two pieces of 8 elements each; a lane group takes GROUPS neighbouring blocks of a

@@ -710,8 +710,9 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward(const ScanParams p) {
 // a thread), and another thread stores the outputs, which lie where x lay, and frees the stage.
 // Against the kernel above there are no addresses to compute, x and the gate need no registers, and
 // a tile is on its way while three are at work.
-// 262144 tokens x 1024 channels, bf16, gated: 500 us, 4.3 TB/s (2.15 GB; the kernel above takes 738).  What
-// bounds it is the chain of states through the tiles: without the waiting 367 us.
+// 262144 tokens x 1024 channels, bf16, gated: 498 us, 4.3 TB/s (2.15 GB; the kernel above takes 760 on rows
+// that TMA refuses).  No pipe is full (issue slots and special functions 46 %): what bounds it is the chain of
+// states through the tiles.
 struct ScanMaps {
     CUtensorMap x, f, gate, y;
 };
@@ -933,8 +934,8 @@ __global__ void __launch_bounds__(FwdCfg<T, GATE>::THREADS, 1)
 // As the forward kernel, from the last tile to the first: x, f, dy and the gate in, and the gradients
 // out where x, f and the gate lay.  A thread keeps, of its 16 rows, the runs before every fourth one; z,
 // the states and the gate's sigmoid are computed again, four rows at a time, which costs less than the
-// registers that would hold them.  8 x 4096 tokens x 768 channels, bf16, gated: 97 us, 3.6 TB/s, issue
-// slots half full (the kernel above: 183 us).
+// registers that would hold them.  8 x 4096 tokens x 768 channels, bf16, gated: 99 us, 3.6 TB/s, issue
+// slots 54 % (the kernel above: 189 us).
 struct ScanBackMaps {
     CUtensorMap x, f, gate, dy, dx, df, dgate;
 };
@@ -1148,7 +1149,7 @@ __global__ void __launch_bounds__(512) scan_bias_sum(const float *part, int64_t 
 }
 
 // --------------------------------------------------------------------------------- one token
-// One pass over x, f, gate and the state.  64 x 768: 2.1 us, a launch's time.
+// One pass over x, f, gate and the state.  64 x 768: 1.9 us, a launch's time.
 template <typename T, int V>
 __global__ void __launch_bounds__(128) scan_step(const ScanStepParams p) {
     const int per = p.C / V;
@@ -1293,7 +1294,7 @@ template <typename T, int V> cudaError_t backward_t(ScanParams p, bool cluster, 
 }  // namespace
 
 // Sequences of 2 to 8 tiles while the tiles fit the GPU at once: a cluster a sequence, in one launch and
-// without words to set up (301 tokens of 768 channels: 6.3 against 9.0 us).  More tiles: TMA.
+// without words to set up (301 tokens of 768 channels: 5.9 against 9.1 us).  More tiles: TMA.
 bool scan_by_cluster(int B, int L, int C, int dtype, int sms) {
     const int chunks = scan_chunks(L);
     const int64_t cols = (int64_t)B * ((C + 31) / 32);  // at most, whatever the vector width

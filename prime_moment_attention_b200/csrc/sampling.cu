@@ -25,9 +25,10 @@
 // range holds the goal walks it.  Where the candidates of a row are few, the cluster's first CTA goes on
 // with them alone.
 //
-// Bound by instructions (some 25 a logit for its weight) in a large batch: 256 x 131072 bf16 take 63 us
-// without filters, 104 with top-p 0.95, of 10.3 that the bytes need; by the latency of its phases in a
-// small one: a row of 32000 with top-k 50 takes 15.5 us.
+// 256 x 131072 bf16 take 61 us without filters, 106 with top-p 0.95 (a language model's rows), of 10.3 that
+// the bytes need.  No pipe is full: the 25 instructions a logit for its weight are 23 us of issue; the rest is the
+// other passes over the row, the phases' barriers and a last wave of CTAs that is half empty.  A small
+// batch is bound by the latency of its phases: a row of 32000 with top-k 50 takes 14.4 us.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"

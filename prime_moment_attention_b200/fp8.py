@@ -3,8 +3,9 @@
     wq, ws = quantize_weight(linear.weight)      # once: [N, K] e4m3, [ceil(N/128), ceil(K/128)]
     y = fp8.linear(x, wq, ws)                    # x [..., K] is quantised inside the call
 
-Weights take half the bytes of bf16, which is what a decode step reads, and the tensor cores run
-e4m3 at twice the rate of bf16.  Inference only.
+Weights take half the bytes of bf16, and the tensor cores run e4m3 at twice the rate of bf16: products of
+many tokens are faster than in bf16 (777 x 1530 x 1000 12 against 26 us, 8192^3 565 against 690); those of a
+decode step save memory only (64 x 32000 x 768 12 against 7 us).  Inference only.
 """
 from __future__ import annotations
 
