@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from prime_moment_attention_b200 import fp8, ops, recurrence, sampling
+from prime_moment_attention_b200 import fp8, recurrence, sampling
 from prime_moment_attention_b200.model import DecodeGraph, PrimeConfig, PrimeForCausalLM
 
 pytestmark = pytest.mark.gpu
@@ -296,6 +296,7 @@ def test_a_nan_row_does_not_end_a_decode_graph(use_fp8):
 
 def test_a_decode_graph_reports_a_fault_at_the_next_step():
     """A replay's kernels record an expired wait in the fault word (written here by hand); step() raises it, once."""
+    from prime_moment_attention_b200 import ops
     m = _model(torch.bfloat16).eval()
     ids = torch.randint(301, (2, 5), device="cuda")
     with torch.no_grad():
